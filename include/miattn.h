@@ -24,6 +24,10 @@
  *   mi_greedy_advance(_tiles), bookkeeping     greedy argmax, tokens, history, positions
  *   mi_argmax_rows                             (reference model/paged.py:474-501, the
  *                                              generate loop's argmax)
+ *   mi_kv_slot_write_fp4,  the paged cache in  the write, the read back, the decode step's epilogue
+ *   mi_kv_slot_read_fp4,   4 bits              and the block-table decode over a 4-bit cache (no
+ *   mi_qk_norm_rope_write_fp4, mi_paged_decode_fp4   reference counterpart)
+ *   mi_copy_pages      page copies             forks and compactions of a paged cache (none either)
  *
  * Conventions shared by every entry point:
  *   - every pointer except the `host_*` arguments is a device pointer;
@@ -333,6 +337,57 @@ int mi_varlen_prefill(const void* q, const void* k, const void* v, void* out,
  * near the default; a small limit forces the give-up path, whose launch still ends normally
  * with its output not to be trusted and 1 (tall) or 2 (duo) in the error word. */
 int mi_prefill_wait_limit(int polls);
+
+/* ------------------------------------------------------------------ the paged cache in 4 bits
+ * A pool of n_blocks blocks is uint8 (n_blocks, H_kv, page_bytes), contiguous, 16-byte aligned, one for K and
+ * one for V; D = 64, 128 or 256; block_size a power of two of at least 16 (else MI_ERR_UNSUPPORTED).
+ * A page of one KV head (mi_fp4_page_bytes = block_size * 17 D / 32) is block_size rows of D / 2 code bytes (element
+ * 2i in the low half of byte i), then D / 32 rows of block_size scale bytes. Each group of 32 elements of a row
+ * shares the scale 2^e, e + 127 its byte; a code is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0-7)
+ * times it. e: the smallest integer with max|x| <= 7 * 2^e, held to [-120, 125]; x * 2^-e goes to the
+ * nearest level, ties to the even code, past 6 to 6. A group with a value that is not finite has the
+ * byte 255 and reads back as NaN. Slots, slot_bits and error_word as for mi_kv_slot_write.
+ * mi_kv_slot_write_fp4: k, v (n_tokens, H_kv, D) in `dtype` with element strides src_strides = {k_s0, k_s1,
+ *   k_s2, v_s0, v_s1, v_s2}; distinct slots are the caller's contract.
+ * mi_kv_slot_read_fp4: k, v (n_tokens, H_kv, D) contiguous in `dtype` receive the rows at the slots (repeats
+ *   allowed); past fp16's largest value that value; zeros for a slot outside the pool, which is reported.
+ * mi_qk_norm_rope_write_fp4: mi_qk_norm_rope_write over such a pool, with the same arguments (n_blocks and block_size
+ *   in place of n_slots) and the same idle and refused rows. The norm and the rotation are fp32 and
+ *   rounded to `dtype` once (mi_qk_norm_rope_write rounds after every op); the pool holds the 4-bit form of
+ *   the rounded k (what mi_kv_slot_write_fp4 of k_out would store). q_out, k_out and v_out 16-byte aligned. */
+int64_t mi_fp4_page_bytes(int block_size, int D);
+int mi_kv_slot_write_fp4(const void* k, const void* v, const void* slot_ids, int slot_bits, void* k_pool,
+                         void* v_pool, int64_t n_tokens, int H_kv, int D, int64_t n_blocks, int block_size,
+                         const int64_t* src_strides, int dtype, int32_t* error_word, void* stream);
+int mi_kv_slot_read_fp4(const void* k_pool, const void* v_pool, const void* slot_ids, int slot_bits, void* k,
+                        void* v, int64_t n_tokens, int H_kv, int D, int64_t n_blocks, int block_size, int dtype,
+                        int32_t* error_word, void* stream);
+int mi_qk_norm_rope_write_fp4(const void* qkv, int64_t row_stride, int qkv_parts, const void* q_norm_w,
+                              const void* k_norm_w, const void* cos_tab, const void* sin_tab, int64_t n_pos,
+                              int rotary_dim, const int64_t* pos, const void* slot_ids, int slot_bits, void* q_out,
+                              void* k_pool, void* v_pool, void* k_out, void* v_out, int B, int H, int H_kv, int D,
+                              int64_t n_blocks, int block_size, float eps, int norm_mode, int dtype,
+                              int32_t* error_word, void* stream);
+/* mi_paged_decode over a 4-bit pool: out[b, h] = softmax(scale * q[b, h] K^T) V over the first seqlen[b] tokens
+ * (clamped to [0, max_blocks * block_size]; zeros for none), fp32 sums, rounded to `dtype` once.
+ * strides = {q_s0, q_s1, k_s0, k_s1, v_s0, v_s1, o_s0, o_s1, bt_s0}: q and out (B, H, D) in elements with D
+ * contiguous, the pools' block and head strides in bytes, the table's row stride; every row, head and page
+ * 16-byte aligned. B * max_blocks * block_size below 2^31. Block ids are trusted. Workspace:
+ * mi_paged_decode_fp4_workspace_size() bytes, 16-byte aligned; calls that share one must be ordered. */
+size_t mi_paged_decode_fp4_workspace_size(int B, int H, int H_kv, int D, int block_size, int max_blocks, int dtype);
+int mi_paged_decode_fp4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                        const int32_t* seqlen, void* out, int B, int H, int H_kv, int D, int block_size,
+                        int max_blocks, const int64_t* strides, float scale, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------ page copies
+ * For each pool p and move i: block host_src[i] of host_pools[p] copied to its block host_dst[i], page_bytes
+ * each (n_blocks blocks per pool; ids outside are MI_ERR_INVALID and nothing is launched). The pointers and
+ * ids are read before the call returns and travel with the launch (one per 64 pools and 192 moves), so a
+ * captured copy repeats them. The moves run at once: a destination named twice, or that is also a source, gets
+ * an unspecified mix. */
+int mi_copy_pages(void* const* host_pools, int n_pools, int64_t page_bytes, int64_t n_blocks,
+                  const int32_t* host_src, const int32_t* host_dst, int n_moves, void* stream);
 
 #ifdef __cplusplus
 }

@@ -8,6 +8,8 @@ Drop-in modules, each mirroring one reference interface:
   ``backend_for`` (reference ``model/attention/varlen.py``);
 * :mod:`miattn.paged`   -- ``PagedPool``, ``PagedKV``, ``PagedWriteSink`` (reference
   ``model/paged.py`` and ``serve/engine.py``'s sink);
+* :mod:`miattn.fp4`     -- ``Fp4PagedPool``, ``paged_decode_fp4``, ``paged_decode_fp4_plan``: the paged cache in
+  4 bits (no reference counterpart);
 * :mod:`miattn.packed`  -- ``PackedPrefill`` (reference ``model/packed.py``).
 
 Device work on a HIP device goes through ``libmiattn.so`` (C ABI in ``include/miattn.h``);
@@ -17,6 +19,7 @@ way. Host (CPU) pools and the CPU prefill arm behave as the reference's own host
 
 from ._lib import HIP_AVAILABLE, LIB_PATH, LOAD_ERROR
 from .decode import TRITON_AVAILABLE, PagedDecodePlan, paged_decode, paged_decode_plan
+from .fp4 import Fp4DecodePlan, Fp4PagedPool, paged_decode_fp4, paged_decode_fp4_plan
 from .packed import PackedPrefill, as_packed_prefill
 from .paged import PagedKV, PagedPool, PagedWriteSink
 from .varlen import FlashVarlen, HipVarlen, SdpaVarlen, backend_for
@@ -24,5 +27,6 @@ from .varlen import FlashVarlen, HipVarlen, SdpaVarlen, backend_for
 __all__ = [
     "HIP_AVAILABLE", "LIB_PATH", "LOAD_ERROR", "TRITON_AVAILABLE", "PagedDecodePlan", "paged_decode",
     "paged_decode_plan", "PackedPrefill", "as_packed_prefill", "PagedKV", "PagedPool", "PagedWriteSink",
-    "FlashVarlen", "HipVarlen", "SdpaVarlen", "backend_for",
+    "FlashVarlen", "HipVarlen", "SdpaVarlen", "backend_for", "Fp4DecodePlan", "Fp4PagedPool", "paged_decode_fp4",
+    "paged_decode_fp4_plan",
 ]

@@ -11,6 +11,7 @@ entry point raises ``RuntimeError`` naming the load error.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -47,6 +48,7 @@ _c_size_t = ctypes.c_size_t
 _c_float = ctypes.c_float
 _p_int64 = ctypes.POINTER(ctypes.c_int64)
 _p_int32 = ctypes.POINTER(ctypes.c_int32)
+_p_void_p = ctypes.POINTER(ctypes.c_void_p)
 
 # Exported symbol -> (restype, argtypes). Kept in step with include/miattn.h; the CPU test
 # suite checks that every function the header declares is exported and bound here.
@@ -132,9 +134,36 @@ SIGNATURES: dict[str, tuple] = {
          _c_int, _c_void_p, _c_size_t, _c_void_p, _c_void_p],
     ),
     "mi_prefill_wait_limit": (_c_int, [_c_int]),
+    "mi_fp4_page_bytes": (_c_int64, [_c_int, _c_int]),
+    "mi_kv_slot_write_fp4": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int64, _c_int, _c_int, _c_int64, _c_int,
+         _p_int64, _c_int, _c_void_p, _c_void_p],
+    ),
+    "mi_kv_slot_read_fp4": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int64, _c_int, _c_int, _c_int64, _c_int,
+         _c_int, _c_void_p, _c_void_p],
+    ),
+    "mi_qk_norm_rope_write_fp4": (
+        _c_int,
+        [_c_void_p, _c_int64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int, _c_void_p,
+         _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
+         _c_int, _c_int64, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_void_p],
+    ),
+    "mi_paged_decode_fp4_workspace_size": (_c_size_t, [_c_int] * 7),
+    "mi_paged_decode_fp4": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_int, _p_int64, _c_float, _c_int, _c_void_p, _c_size_t, _c_void_p],
+    ),
+    "mi_copy_pages": (
+        _c_int,
+        [_p_void_p, _c_int, _c_int64, _c_int64, _p_int32, _p_int32, _c_int, _c_void_p],
+    ),
 }
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 
 def _load():
@@ -178,6 +207,17 @@ def current_stream(device: torch.device) -> int:
     if _RAW_STREAM is None or device.index is None:
         return torch.cuda.current_stream(device).cuda_stream
     return _RAW_STREAM(device.index)
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one: a launch goes to its stream, and a workspace or
+    output taken inside belongs to it."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _CURRENT
+    return torch.cuda.device(device)
+
+
+_CURRENT = contextlib.nullcontext()
 
 
 def last_error() -> str:

@@ -37,7 +37,7 @@ HIPCC_FLAGS = [
 ]
 
 SOURCES = ["capi.hip", "slot_write.hip", "paged_decode.hip", "varlen_prefill.hip", "decode_epilogue.hip",
-           "decode_step.hip", "rows_gemm.hip"]
+           "decode_step.hip", "rows_gemm.hip", "fp4_cache.hip", "paged_decode_fp4.hip", "copy_pages.hip"]
 
 
 def _hipcc() -> str:

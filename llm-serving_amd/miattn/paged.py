@@ -25,6 +25,7 @@ host synchronisation.
 
 from __future__ import annotations
 
+import ctypes
 import os
 from types import SimpleNamespace
 
@@ -84,13 +85,20 @@ class PagedPool:
         if strict_writes is None:
             strict_writes = os.environ.get("MIATTN_STRICT_WRITES", "0") == "1"
         self.strict_writes = bool(strict_writes)
-        block_shape = (self.n_blocks, self.block_size, self.n_kv_head, self.head_dim)
-        self.keys = [torch.zeros(block_shape, dtype=dtype, device=self.device) for _ in range(self.n_layer)]
-        self.values = [torch.zeros(block_shape, dtype=dtype, device=self.device) for _ in range(self.n_layer)]
+        self._check_storage()
+        self.keys = [self._layer_store() for _ in range(self.n_layer)]
+        self.values = [self._layer_store() for _ in range(self.n_layer)]
         self._on_device = self.device.type == "cuda"
         # device word: 1 + index of the first token a HIP write skipped, 0 when none
         self._write_error = torch.zeros(1, dtype=torch.int32, device=self.device) if self._on_device else None
         self._slot_memo: tuple[tuple, torch.Tensor] | None = None
+
+    def _check_storage(self) -> None:
+        """What a pool of another storage requires of its sizes, dtype and device."""
+
+    def _layer_store(self) -> torch.Tensor:
+        shape = (self.n_blocks, self.block_size, self.n_kv_head, self.head_dim)
+        return torch.zeros(shape, dtype=self.dtype, device=self.device)
 
     # ------------------------------------------------------------------ tables and slots
     def _layer(self, layer) -> int:
@@ -242,19 +250,24 @@ class PagedPool:
         slot_ids = slot_ids.contiguous()
         pos = pos.contiguous()
         q = torch.empty((B, H, D), dtype=self.dtype, device=self.device)
-        rc = _lib.lib.mi_qk_norm_rope_write(
-            source.data_ptr(), row_stride, n_parts, q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(),
-            sin.data_ptr(), cos.shape[0], rotary, pos.data_ptr(), slot_ids.data_ptr(), 8 * slot_ids.element_size(),
-            q.data_ptr(), self.keys[layer].data_ptr(), self.values[layer].data_ptr(),
-            None if k_out is None else k_out.data_ptr(), None if v_out is None else v_out.data_ptr(),
-            B, H, H_kv, D, self.n_slots, float(eps), int(bool(zero_centred_norm)), _lib.dtype_code(self.dtype),
-            self._write_error.data_ptr(),
-            _lib.current_stream(source.device),
-        )
+        rc = self._launch_epilogue(layer, source, row_stride, n_parts, q_norm_w, k_norm_w, cos, sin, rotary, pos,
+                                   slot_ids, q, k_out, v_out, eps, zero_centred_norm)
         _lib.check(rc, "PagedPool.write_qk_norm_rope")
         if self.strict_writes:
             self.check_writes()
         return q
+
+    def _launch_epilogue(self, layer, source, row_stride, n_parts, q_norm_w, k_norm_w, cos, sin, rotary, pos, slot_ids,
+                         q, k_out, v_out, eps, zero_centred_norm) -> int:
+        B, H, D = q.shape
+        return _lib.lib.mi_qk_norm_rope_write(
+            source.data_ptr(), row_stride, n_parts, q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], rotary, pos.data_ptr(), slot_ids.data_ptr(), 8 * slot_ids.element_size(),
+            q.data_ptr(), self.keys[layer].data_ptr(), self.values[layer].data_ptr(),
+            None if k_out is None else k_out.data_ptr(), None if v_out is None else v_out.data_ptr(),
+            B, H, self.n_kv_head, D, self.n_slots, float(eps), int(bool(zero_centred_norm)),
+            _lib.dtype_code(self.dtype), self._write_error.data_ptr(), _lib.current_stream(source.device),
+        )
 
     @property
     def write_error_word(self) -> torch.Tensor | None:
@@ -292,6 +305,43 @@ class PagedPool:
             return
         self._check_block_ids(block_table, self._blocks_for(start, length))
         self.write_prefill_slots(layer, self._slot_ids(block_table, start, length), k, v)
+
+    # ------------------------------------------------------------------ pages
+    def copy_blocks(self, src, dst) -> None:
+        """Copy block ``src[i]`` to block ``dst[i]``, K and V of every layer: a forked request's partly
+        filled last block, or blocks that a compaction moves (``miattn.serve.BlockFreeList.fork`` and
+        ``compact`` give the pairs). ``src`` and ``dst`` are equally long sequences of block ids (ints; a source may
+        repeat). A destination may be neither named twice nor a source: the copies run at once. One
+        launch per 64 pools and 192 pairs; the ids travel with the launch, so a captured copy repeats them."""
+        src, dst = list(src), list(dst)
+        if len(src) != len(dst):
+            raise ValueError(f"copy_blocks needs one destination per source, got {len(src)} / {len(dst)}")
+        self._check_block_ids(src + dst, 0)
+        if len(set(dst)) != len(dst):
+            raise ValueError("copy_blocks: a destination block is named twice")
+        both = set(src) & set(dst)
+        if both:
+            raise ValueError(f"copy_blocks: block {min(both)} is both a source and a destination")
+        if not src:
+            return
+        stores = self.keys + self.values
+        if not self._on_device:
+            a, b = torch.tensor(src), torch.tensor(dst)
+            for store in stores:
+                store[b] = store[a]
+            return
+        _lib.require_library("PagedPool.copy_blocks on a HIP pool")
+        pools = (ctypes.c_void_p * len(stores))(*[t.data_ptr() for t in stores])
+        page = stores[0][0].numel() * stores[0].element_size()
+        with _lib.on_device(self.keys[0].device):
+            rc = _lib.lib.mi_copy_pages(pools, len(stores), page, self.n_blocks, (ctypes.c_int32 * len(src))(*src),
+                                        (ctypes.c_int32 * len(dst))(*dst), len(src),
+                                        _lib.current_stream(self.keys[0].device))
+        _lib.check(rc, "PagedPool.copy_blocks")
+
+    def decode_plan(self, q, block_table, seqlen, *, scale=None):
+        """The decode plan of this pool's layers (``paged_decode_plan`` over ``keys`` and ``values``)."""
+        return paged_decode_plan(q, self.keys, self.values, block_table, seqlen, scale=scale)
 
     # ------------------------------------------------------------------ accounting
     def bytes(self) -> int:
@@ -463,8 +513,7 @@ class PagedKV:
             raise ValueError(f"attend needs q {want}, got {tuple(q.shape)}")
         q3 = q.squeeze(2).contiguous()
         if self._plan is None:
-            self._plan = paged_decode_plan(q3, self.pool.keys, self.pool.values, self._block_table_tensor,
-                                           self._seqlen, scale=self.head_dim ** -0.5)
+            self._plan = self.pool.decode_plan(q3, self._block_table_tensor, self._seqlen, scale=self.head_dim ** -0.5)
         return self._plan.run(layer, q3).unsqueeze(2)
 
     def advance(self) -> None:

@@ -30,7 +30,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .decode import paged_decode_plan
+from .fp4 import Fp4PagedPool
 from .packed import PackedPrefill
 from .paged import PagedKV, PagedPool
 from .rows import Parts, argmax_rows, glu_weight, rows_linear, rows_supported, rows_swiglu, rows_tile_best
@@ -231,10 +231,14 @@ class Qwen3:
         self.cos, self.sin = rope_table(cfg.head_dim, cfg.rope_theta, max_pos, self.device, self.dtype)
 
     # ------------------------------------------------------------------ pieces
-    def new_pool(self, n_blocks: int, block_size: int = 16) -> PagedPool:
+    def new_pool(self, n_blocks: int, block_size: int = 16, *, kv_bits: int = 16) -> PagedPool:
+        """A pool for this model: in the model's dtype, or with ``kv_bits=4`` in 4 bits (``miattn.fp4``)."""
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16, got {kv_bits!r}")
         c = self.cfg
-        return PagedPool(c.n_layer, n_blocks, block_size, c.n_kv_head, c.head_dim, dtype=self.dtype,
-                         device=self.device, n_head=c.n_head)
+        pool = Fp4PagedPool if kv_bits == 4 else PagedPool
+        return pool(c.n_layer, n_blocks, block_size, c.n_kv_head, c.head_dim, dtype=self.dtype, device=self.device,
+                    n_head=c.n_head)
 
     # ------------------------------------------------------------------ prefill
     def prefill(self, prompts: list[list[int]], pool: PagedPool, tables: list[list[int]]) -> torch.Tensor:
@@ -359,8 +363,7 @@ class GraphDecoder:
         self.max_new = max_new
         self.B = B
         q0 = torch.zeros(B, c.n_head, c.head_dim, dtype=model.dtype, device=dev)
-        self.plan = paged_decode_plan(q0, pool.keys, pool.values, self.table, self.seqlen,
-                                      scale=1.0 / math.sqrt(c.head_dim))
+        self.plan = pool.decode_plan(q0, self.table, self.seqlen, scale=1.0 / math.sqrt(c.head_dim))
         # q/k norm + RoPE + K/V write fused into the decode launch where the shape allows
         self.fused = self.plan.fused_supported(model.dtype, 2 * int(model.cos.shape[-1]))
         self.graph = None

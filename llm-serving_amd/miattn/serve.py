@@ -46,7 +46,6 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from .decode import paged_decode_plan
 from .paged import PagedPool
 from .qwen3 import Qwen3, decode_step_begin, greedy_advance, greedy_advance_tiles
 from .rows import rows_supported, rows_tile_best
@@ -79,11 +78,14 @@ def poisson_trace(n: int, *, rate: float, vocab: int, median: float = 256, sigma
 class BlockFreeList:
     """Physical block ids of one pool: a request takes all its blocks or none; freed ids go
     back to the front, so a pool that cycles through short requests keeps reusing the
-    same low blocks."""
+    same low blocks. Requests may share blocks (:meth:`fork`): a block is free again when every
+    request that holds it has given it back."""
 
     def __init__(self, n_blocks: int, block_size: int) -> None:
         self.block_size = int(block_size)
+        self._n_blocks = int(n_blocks)
         self._free = list(range(n_blocks - 1, -1, -1))  # pop() hands out 0, 1, 2, ...
+        self._holders: dict[int, int] = {}  # blocks held more than once -> how often
 
     @property
     def n_free(self) -> int:
@@ -98,7 +100,59 @@ class BlockFreeList:
         return [self._free.pop() for _ in range(count)]
 
     def give_back(self, blocks: list[int]) -> None:
-        self._free.extend(reversed(blocks))
+        if not self._holders:
+            self._free.extend(reversed(blocks))
+            return
+        for b in reversed(blocks):
+            held = self._holders.pop(b, 1) - 1
+            if held == 0:
+                self._free.append(b)
+            elif held > 1:
+                self._holders[b] = held
+
+    def fork(self, blocks: list[int], length: int, capacity: int | None = None):
+        """A second request that continues ``blocks``' first ``length`` tokens on its own: ``(table, src, dst)``,
+        or None when the pool lacks the blocks. The table has room for ``capacity`` tokens (default: as
+        many blocks as ``blocks``); its full blocks are shared with ``blocks``, the partly filled one and
+        those to come are its own. ``src``/``dst`` (one pair, or none at a block boundary) go to
+        ``PagedPool.copy_blocks`` before either request writes its next token."""
+        length = int(length)
+        full, part = divmod(length, self.block_size)
+        if length < 0 or full + (part > 0) > len(blocks):
+            raise ValueError(f"a table of {len(blocks)} blocks of {self.block_size} does not hold {length} tokens")
+        want = len(blocks) if capacity is None else self.blocks_for(capacity)
+        if want * self.block_size < length:
+            raise ValueError(f"a capacity of {capacity} tokens does not hold the {length} forked ones")
+        own = self.take(want - full)
+        if own is None:
+            return None
+        for b in blocks[:full]:
+            self._holders[b] = self._holders.get(b, 1) + 1
+        return blocks[:full] + own, blocks[full: full + (part > 0)], own[: part > 0]
+
+    def compact(self, tables: list[list[int]]):
+        """Move the blocks in use to the lowest ids: ``(src, dst)`` for ``PagedPool.copy_blocks``, with
+        ``tables`` (every live request's) rewritten in place; afterwards ids from the number of blocks in
+        use on are free. The copy has to run, and device tables to be uploaded again, before the next
+        launch that reads or writes a moved block. Raises when ``tables`` are not what is held."""
+        times: dict[int, int] = {}
+        for table in tables:
+            for b in table:
+                times[b] = times.get(b, 0) + 1
+        free = set(self._free)
+        if len(times) + len(free) != self._n_blocks or any(b in free for b in times) or \
+                any(n != self._holders.get(b, 1) for b, n in times.items()):
+            raise ValueError("compact needs the table of every live request: these tables hold other blocks than "
+                             "were handed out")
+        used = len(times)
+        src = sorted(b for b in times if b >= used)
+        dst = sorted(b for b in free if b < used)
+        moved = dict(zip(src, dst))
+        for table in tables:
+            table[:] = [moved.get(b, b) for b in table]
+        self._holders = {moved.get(b, b): n for b, n in self._holders.items()}
+        self._free = list(range(self._n_blocks - 1, used - 1, -1))
+        return src, dst
 
 
 class SeatDecoder:
@@ -126,8 +180,7 @@ class SeatDecoder:
         self.x = torch.empty(self.S, c.hidden, dtype=model.dtype, device=dev)
         self.h0 = torch.empty_like(self.x)
         q0 = torch.zeros(self.S, c.n_head, c.head_dim, dtype=model.dtype, device=dev)
-        self.plan = paged_decode_plan(q0, pool.keys, pool.values, self.table, self.seqlen,
-                                      scale=1.0 / math.sqrt(c.head_dim))
+        self.plan = pool.decode_plan(q0, self.table, self.seqlen, scale=1.0 / math.sqrt(c.head_dim))
         # q/k norm + RoPE + K/V write fused into the decode launch where the shape allows
         self.fused = self.plan.fused_supported(model.dtype, 2 * int(model.cos.shape[-1]))
         self.graph = None
@@ -242,9 +295,10 @@ class ContinuousServer:
     """The loop of the module docstring over one model, pool and seat decoder."""
 
     def __init__(self, model: Qwen3, *, max_batch: int = 32, n_blocks: int = 8192, block_size: int = 16,
-                 max_prompt: int = 2048, max_new: int = 128, max_prefill_tokens: int = 8192, stream=None) -> None:
+                 max_prompt: int = 2048, max_new: int = 128, max_prefill_tokens: int = 8192, stream=None,
+                 kv_bits: int = 16) -> None:
         self.model = model
-        self.pool = model.new_pool(n_blocks, block_size)
+        self.pool = model.new_pool(n_blocks, block_size, **({} if kv_bits == 16 else {"kv_bits": kv_bits}))
         self.blocks = BlockFreeList(n_blocks, block_size)
         self.max_batch = int(max_batch)
         self.max_new = int(max_new)
