@@ -199,6 +199,20 @@ __device__ __forceinline__ float group_allreduce(float x) {
   return x;
 }
 
+// Inclusive prefix sum over the 64 lanes of a wave, in DPP moves (no LDS round trips):
+// shifts by 1, 2, 4 and 8 inside each row of 16 lanes (lanes shifted in from outside the
+// row read 0), then lane 15 of rows 0 and 2 added into rows 1 and 3, and lane 31 into rows
+// 2 and 3.
+__device__ __forceinline__ int wave_inclusive_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 -> rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 -> rows 2, 3
+  return v;
+}
+
 // Round an fp32 result to T (the rounding a tensor op of dtype T applies to its result).
 // The value goes through an empty asm first: without it the compiler may fold
 // round_T(op_f32(a, b)) into the native fp16 op (division, square root), whose rounding

@@ -164,20 +164,6 @@ __device__ __forceinline__ int clamp_len(int len, int capacity) {
   return len > 0 ? len : 0;
 }
 
-// Inclusive prefix sum over the 64 lanes of a wave, in DPP moves (no LDS round trips):
-// shifts by 1, 2, 4 and 8 inside each row of 16 lanes (lanes shifted in from outside the
-// row read 0), then lane 15 of rows 0 and 2 added into rows 1 and 3, and lane 31 into rows
-// 2 and 3.
-__device__ __forceinline__ int wave_inclusive_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 -> rows 1, 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 -> rows 2, 3
-  return v;
-}
-
 // Floors of the split size, in tokens, for batches with a row of more than 32 of its batches of loads (the
 // splits that the merge folds per round trip; shorter rows are cut as finely as the workgroups allow: 8
 // rows of 224 tokens 8.4 us per layer with splits of 8, 8.9 of 24; H 8 / H_kv 2 / D 256, 6 of 200, 8.7 / 9.5). A

@@ -1,6 +1,31 @@
 // Block-table paged-decode attention over the 4-bit cache (format in fp4.h): one query token per row,
 //   out[b, h] = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale * q[b, h] . k_t - max),  t < seqlen[b],
 // with k_t, v_t the rows of KV head h / (H / H_kv); a row of length 0 gives zeros.
+//
+// A token of one KV head is 17 D / 32 bytes each of K and V for 4 D operations per query head, and turning a 4-bit
+// element into an operand costs vector instructions that a 16-bit cache does not pay, at a quarter
+// of its bytes: with the products on the vector unit too, that unit would bound the kernel and not the
+// memory. So both products run on the matrix cores, and the elements are converted once for all
+// query heads of their KV head:
+//   * a wave works on tiles of 32 tokens of one KV head. The columns of both products are the query heads,
+//     each in NC columns (below);
+//   * S = K Q^T: 16 tokens are the rows of a 16x16x32 product. A lane holds D / 8 bytes of one token's row
+//     (D / 4 elements under one or two scales), and v_cvt_scalef32_pk_bf16_fp4 turns two elements, scale applied,
+//     into a bf16 pair in one instruction: exact, E2M1 has two significant bits. The order of the D
+//     elements in the products' depth is free, so a lane's elements are in memory order and Q is laid out to match;
+//   * O^T = V^T P^T: the rows are 16 elements of D, the depth 32 tokens. A lane holds D / 16 elements of each of 8
+//     tokens; converted pairs lie along D and are exchanged between two tokens by v_perm_b32 (one
+//     instruction per pair), so a register holds one element of two tokens. The 8 tokens are those whose scores
+//     the same lane holds of S, so P needs no exchange between lanes;
+//   * exactness: q of a 16-bit type in one bf16 operand (bf16) or a high and a low one (fp16), fp32 in three. p in
+//     fp32 is cut into a high and a low bf16 part, 16 bits together (three parts, 24 bits, for fp32
+//     outputs), so no precision is lost against fp32 products. The parts are columns of the same product
+//     that would be empty otherwise: NC = 2 columns per query head (4 for fp32), 8 (4) heads at a time;
+//   * the running maximum is raised only when a tile's is past it by 2^8 (p stays below 2^8, nothing
+//     overflows), so the accumulators are rarely rescaled; sums are fp32.
+// Rows are cut into splits of whole rounds (one tile per wave of the workgroup), planned on the device from the row
+// lengths so that the splits of all rows fill the chip however ragged the batch is; the waves of a
+// workgroup take a split's tiles in turn and are merged through LDS, splits of one row by a second small launch.
 #include <type_traits>
 
 #include "fp4.h"
@@ -9,69 +34,437 @@ namespace miattn {
 namespace {
 
 struct Fp4DecodeArgs {
-  int B, H, H_kv, G, bs_log2, max_blocks;
+  int B, H, H_kv, G, n_hchunks, bs_log2, max_blocks, target, min_chunk, slots;
   int64_t qs0, qs1, ks0, ks1, vs0, vs1, os0, os1, bts0;
   float scale_log2;
 };
 
-// One workgroup per (query head, row): D / 8 lanes per token, an online softmax per lane group.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_decode_fp4_kernel(const T* __restrict__ q, const uint8_t* __restrict__ kc,
-                                                               const uint8_t* __restrict__ vc,
-                                                               const int32_t* __restrict__ block_table,
-                                                               const int32_t* __restrict__ seqlen, T* __restrict__ out,
-                                                               Fp4DecodeArgs a) {
-  constexpr int LPR = D / 8, NG = 256 / LPR;  // lanes per token, tokens at a time
-  __shared__ float sm_ml[NG][2];
-  __shared__ float sm_acc[NG][D];
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int c = threadIdx.x % LPR, grp = threadIdx.x / LPR;
-  const int kvh = h / a.G;
-  const int bs = 1 << a.bs_log2;
-  const int cap = a.max_blocks << a.bs_log2;
-  int len = seqlen[b];
-  len = len < cap ? len : cap;
-  float qv[8];
-  load8<T, false>(q + b * a.qs0 + h * a.qs1 + c * 8, 1, qv);
-  float m = -INFINITY, l = 0.0f, acc[8] = {};
-  for (int t = grp; t < len; t += NG) {
-    const int64_t page = block_table[b * a.bts0 + (t >> a.bs_log2)];
-    const int at = t & (bs - 1);
-    const int64_t code = int64_t(at) * (D / 2) + c * 4, sc = int64_t(bs) * (D / 2) + int64_t(c >> 2) * bs + at;
-    const uint8_t* kp = kc + page * a.ks0 + kvh * a.ks1;
-    const uint8_t* vp = vc + page * a.vs0 + kvh * a.vs1;
-    float kv[8], vv[8];
-    fp4_decode(*reinterpret_cast<const uint32_t*>(kp + code), fp4_scale(kp[sc]), kv);
-    fp4_decode(*reinterpret_cast<const uint32_t*>(vp + code), fp4_scale(vp[sc]), vv);
-    float dot = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dot = fmaf(qv[j], kv[j], dot);
-    const float s = group_allreduce<LPR, SumOp>(dot) * a.scale_log2;
-    const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.0f : mn;
-    const float alpha = fast_exp2(m - mu), p = fast_exp2(s - mu);
-    m = mn;
-    l = l * alpha + p;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = fmaf(p, vv[j], acc[j] * alpha);
+constexpr int kW = 4;           // waves per workgroup
+constexpr int kTile = 32;       // tokens per wave and step
+constexpr int kRound = kW * kTile;
+constexpr float kRaise = 8.0f;  // log2 units a tile's maximum may be past the running one
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+// columns per query head (parts of q and p), query heads per pass
+template <typename T> constexpr int kCols = sizeof(T) == 4 ? 4 : 2;
+template <typename T> constexpr int kHeads = 16 / kCols<T>;
+
+__device__ __forceinline__ int clamp_len(int len, int capacity) {
+  len = len < capacity ? len : capacity;
+  return len > 0 ? len : 0;
+}
+
+__device__ __forceinline__ float hi_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+// the high halves of two floats as a bf16 pair (cut, not rounded)
+__device__ __forceinline__ uint32_t pack_hi(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ bf16x8_t operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(bf16x8_t, make_uint4(a, b, c, d));
+}
+// max / sum over lanes i, i ^ 16, i ^ 32 and i ^ 48 (the four lane groups of a column)
+template <typename Op>
+__device__ __forceinline__ float over_groups(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = Op::op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return Op::op(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+// sum over the NC columns of a query head
+template <int NC>
+__device__ __forceinline__ float over_parts(float x) {
+  x += dpp<kDppQuadXor1>(x);
+  if constexpr (NC == 4) x += dpp<kDppQuadXor2>(x);
+  return x;
+}
+
+// Tokens per split: total / target in whole rounds, at least min_chunk. The splits are then at most target
+// and one partial split per row.
+__device__ __forceinline__ int chunk_of(int total, const Fp4DecodeArgs& a) {
+  const int even = int((uint32_t(total) + uint32_t(a.target) - 1u) / uint32_t(a.target));
+  const int rounds = (even + kRound - 1) / kRound * kRound;
+  return rounds > a.min_chunk ? rounds : a.min_chunk;
+}
+
+struct Fp4Split {
+  int b, split, n_split, first, chunk, len;
+};
+// This workgroup's (row, split): every wave derives it from the row lengths, 64 rows at a time.
+__device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, const Fp4DecodeArgs& a, int w,
+                                           Fp4Split& si) {
+  const int lane = __lane_id();
+  const int capacity = a.max_blocks << a.bs_log2;
+  const int len_first = lane < a.B ? clamp_len(seqlen[lane], capacity) : 0;
+  int total = __builtin_amdgcn_readlane(wave_inclusive_scan(len_first), 63);
+  for (int r0 = 64; r0 < a.B; r0 += 64) {
+    const int row = r0 + lane;
+    total += __builtin_amdgcn_readlane(wave_inclusive_scan(row < a.B ? clamp_len(seqlen[row], capacity) : 0), 63);
   }
-  if (c == 0) {
-    sm_ml[grp][0] = m;
-    sm_ml[grp][1] = l;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) sm_acc[grp][c * 8 + j] = acc[j];
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float M = -INFINITY, L = 0.0f, A = 0.0f;
-    for (int g = 0; g < NG; ++g) M = fmaxf(M, sm_ml[g][0]);
-    const float mu = M == -INFINITY ? 0.0f : M;
-    for (int g = 0; g < NG; ++g) {
-      const float w = fast_exp2(sm_ml[g][0] - mu);
-      L = fmaf(sm_ml[g][1], w, L);
-      A = fmaf(sm_acc[g][d], w, A);
+  const int chunk = chunk_of(total, a);
+  int len = len_first, base = 0;
+  for (int r0 = 0;;) {
+    const int n = int((uint32_t(len) + uint32_t(chunk) - 1u) / uint32_t(chunk));
+    const int incl = wave_inclusive_scan(n);
+    const uint64_t owner = __ballot(w >= base + incl - n && w < base + incl);
+    if (owner != 0) {
+      const int o = __ffsll(static_cast<unsigned long long>(owner)) - 1;
+      const int excl = __builtin_amdgcn_readlane(incl - n, o);
+      si.b = r0 + o;
+      si.split = w - base - excl;
+      si.n_split = __builtin_amdgcn_readlane(n, o);
+      si.first = base + excl;
+      si.chunk = chunk;
+      si.len = __builtin_amdgcn_readlane(len, o);
+      return true;
     }
-    out[b * a.os0 + h * a.os1 + d] = from_f32<T>(fp4_saturate<T>(len > 0 ? A / L : 0.0f));
+    r0 += 64;
+    if (r0 >= a.B) return false;
+    base += __builtin_amdgcn_readlane(incl, 63);
+    const int row = r0 + lane;
+    len = row < a.B ? clamp_len(seqlen[row], capacity) : 0;
   }
+}
+
+template <typename T, int D>
+struct Fp4Tile {
+  static constexpr int KW = D / 32;                  // code dwords of K per lane and 16 tokens
+  static constexpr int KS = D == 256 ? 2 : 1;        // scales of those
+  static constexpr int VE = D / 16;                  // V elements per lane and token
+  static constexpr int VW = VE >= 8 ? VE / 8 : 1;    // dwords they take (D 64: half of one)
+  uint32_t k[2][KW], ks[2][KS], v[2][4][VW], vs[2];
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
+    const T* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+    const int32_t* __restrict__ block_table, const int32_t* __restrict__ seqlen, T* __restrict__ out,
+    int32_t* __restrict__ ws_rows, float* __restrict__ ws_ml, float* __restrict__ ws_acc, Fp4DecodeArgs a) {
+  using Tile = Fp4Tile<T, D>;
+  constexpr int KW = Tile::KW, KS = Tile::KS, VE = Tile::VE, VW = Tile::VW;
+  constexpr int NC = kCols<T>, HB = kHeads<T>;
+  extern __shared__ __align__(16) float smem[];  // per wave: (m, l) of HB heads, then nh x D sums
+
+  Fp4Split si;
+  if (!plan_split(seqlen, a, blockIdx.x, si)) return;  // uniform
+  const int b = si.b;
+  const int t_begin = si.split * si.chunk;
+  const int t_end = min(si.len, t_begin + si.chunk);
+  if (si.split == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    ws_rows[2 * b] = si.first;
+    ws_rows[2 * b + 1] = si.n_split;
+  }
+  const int kvh = blockIdx.y / a.n_hchunks;
+  const int hch = blockIdx.y - kvh * a.n_hchunks;
+  const int nh = min(HB, a.G - hch * HB);  // query heads of this workgroup
+  const int h0 = kvh * a.G + hch * HB;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, lg = lane >> 4;  // of the products: row or column, and depth group
+  const int part = col % NC;
+  const int bs = 1 << a.bs_log2;
+
+  // Q as the depth x column operand: this lane's column, elements lg D / 4 + 8 kk + j. A negative scale
+  // is moved into q, so that the largest score is the largest product.
+  const float flip = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+  const float c2 = a.scale_log2 * flip;
+  bf16x8_t qf[KW];
+  {
+    const bool there = col / NC < nh;
+    const T* src = q + b * a.qs0 + (h0 + (there ? col / NC : 0)) * a.qs1 + lg * (D / 4);
+#pragma unroll
+    for (int kk = 0; kk < KW; ++kk) {
+      float x[8];
+      load8<T, true>(src + 8 * kk, 1, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = there ? x[j] * flip : 0.0f;
+        if constexpr (!std::is_same<T, bf16_t>::value) {
+          // part i holds the bits left by the parts before it; past the last part nothing is left
+          for (int i = 0; i < NC - 1; ++i) x[j] = i < part ? x[j] - hi_bf16(x[j]) : x[j];
+          if (NC == 4 && part == 3) x[j] = 0.0f;
+        }
+      }
+      qf[kk] = operand(pack_hi(x[0], x[1]), pack_hi(x[2], x[3]), pack_hi(x[4], x[5]), pack_hi(x[6], x[7]));
+    }
+  }
+
+  const int32_t* bt_row = block_table + b * a.bts0;
+  const int k_lane = col * (D / 2) + lg * (D / 8);
+  const int ks_lane = bs * (D / 2) + (lg * (D / 4) / kFp4Group) * bs + col;
+  const int v_lane = lg * 4 * (D / 2) + col * (D / 32);
+  const int vs_lane = bs * (D / 2) + (col * VE / kFp4Group) * bs + lg * 4;
+
+  // first token of 16-token half u of the tile at t0; a half past the end repeats the first (masked out)
+  auto half_at = [&](int t0, int u) { return t0 + 16 * u < t_end ? t0 + 16 * u : t0; };
+  auto load_pages = [&](int t0, int (&pg)[2]) {
+    t0 = t0 < t_end ? t0 : t_begin;  // past the split: a page that is there, not used
+#pragma unroll
+    for (int u = 0; u < 2; ++u) pg[u] = bt_row[half_at(t0, u) >> a.bs_log2];
+  };
+  auto issue = [&](int t0, const int (&pg)[2], Tile& t) {
+    t0 = t0 < t_end ? t0 : t_begin;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int at = half_at(t0, u) & (bs - 1);
+      const uint8_t* kp = kc + (int64_t(pg[u]) * a.ks0 + kvh * a.ks1);
+      const uint8_t* vp = vc + (int64_t(pg[u]) * a.vs0 + kvh * a.vs1);
+      const uint8_t* kr = kp + (at * (D / 2) + k_lane);
+#pragma unroll
+      for (int i = 0; i < KW; i += 4) {
+        if constexpr (KW >= 4) {
+          const uint4 w = load16_nt(kr + 4 * i);
+          t.k[u][i] = w.x; t.k[u][i + 1] = w.y; t.k[u][i + 2] = w.z; t.k[u][i + 3] = w.w;
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(kr);
+          t.k[u][0] = w.x; t.k[u][1] = w.y;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) t.ks[u][i] = kp[at + ks_lane + i * bs];
+      const uint8_t* vr = vp + (at * (D / 2) + v_lane);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (VE == 4) {
+          t.v[u][j][0] = *reinterpret_cast<const uint16_t*>(vr + j * (D / 2));
+        } else if constexpr (VE == 8) {
+          t.v[u][j][0] = *reinterpret_cast<const uint32_t*>(vr + j * (D / 2));
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(vr + j * (D / 2));
+          t.v[u][j][0] = w.x; t.v[u][j][1] = w.y;
+        }
+      }
+      t.vs[u] = *reinterpret_cast<const uint32_t*>(vp + at + vs_lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  f32x4_t o[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) o[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, mc = 0.0f, l = 0.0f;  // the running maximum (of q . k), times c2, and the sum of p
+  const float raise = fminf(kRaise / c2, 3.0e38f);
+  const uint32_t cut1 = part >= 1 ? 0xffff0000u : 0u, cut2 = part >= 2 ? 0xffff0000u : 0u;
+
+  auto compute = [&](int t0, const Tile& t, auto masked) {
+    constexpr bool kMasked = decltype(masked)::value;
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4_t s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int kk = 0; kk < KW; ++kk) {
+        const float sc = fp4_scale(t.ks[u][kk * 8 * KS / (D / 4)]);
+        const uint32_t w = t.k[u][kk];
+        const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0);
+        const auto p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1);
+        const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2);
+        const auto p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3);
+        const bf16x8_t kf = operand(__builtin_bit_cast(uint32_t, p0), __builtin_bit_cast(uint32_t, p1),
+                                    __builtin_bit_cast(uint32_t, p2), __builtin_bit_cast(uint32_t, p3));
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[kk], s[u], 0, 0, 0);
+      }
+    }
+    // this lane's 8 tokens: t0 + 16 u + 4 lg + i
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (!std::is_same<T, bf16_t>::value) s[u][i] = over_parts<NC>(s[u][i]);
+        if constexpr (kMasked) {
+          if (t0 + 16 * u + 4 * lg + i >= t_end) s[u][i] = -INFINITY;
+        }
+        most = fmaxf(most, s[u][i]);
+      }
+    }
+    most = over_groups<MaxOp>(most);
+    if (__any(!(most - m <= raise))) {  // also the first tile
+      const float up = fmaxf(m, most);
+      const float alpha = m == -INFINITY ? 0.0f : fast_exp2((m - up) * c2);
+      m = up;
+      mc = up == -INFINITY ? 0.0f : up * c2;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) o[i] *= alpha;
+    }
+    float p[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = fast_exp2(fmaf(s[u][i], c2, -mc));
+        if constexpr (kMasked) x = t0 + 16 * u + 4 * lg + i < t_end ? x : 0.0f;
+        l += x;
+        x -= __uint_as_float(__float_as_uint(x) & cut1);
+        if constexpr (NC == 4) {
+          x -= __uint_as_float(__float_as_uint(x) & cut2);
+          if (part == 3) x = 0.0f;
+        }
+        p[4 * u + i] = x;
+      }
+    }
+    const bf16x8_t pf = operand(pack_hi(p[0], p[1]), pack_hi(p[2], p[3]), pack_hi(p[4], p[5]), pack_hi(p[6], p[7]));
+    // the scale of token i of a half is byte i of its dword, shifted under the exponent (the conversion
+    // reads no other bit of it)
+    float vsc[8];
+    uint32_t vw[8][VW];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = t.vs[u];
+        uint32_t x = i == 3 ? w >> 1 : w << (23 - 8 * i);
+        bool in = true;
+        if constexpr (kMasked) {  // garbage past the end may be a NaN scale, which 0 * NaN would keep
+          in = t0 + 16 * u + 4 * lg + i < t_end;
+          x = in ? x : 0x3f800000u;
+        }
+        vsc[4 * u + i] = __uint_as_float(x);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) vw[4 * u + i][k] = in ? t.v[u][i][k] : 0u;
+      }
+    }
+    auto byte_of = [&](auto which, int k) {
+      constexpr int kByte = decltype(which)::value;
+      uint32_t x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[j][k], vsc[j], kByte));
+      }
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        lo[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
+        hi[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
+      }
+      const int e = 8 * k + 2 * kByte;
+      o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(lo[0], lo[1], lo[2], lo[3]), pf, o[e], 0, 0, 0);
+      o[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(hi[0], hi[1], hi[2], hi[3]), pf, o[e + 1], 0, 0, 0);
+    };
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      byte_of(std::integral_constant<int, 0>{}, k);
+      byte_of(std::integral_constant<int, 1>{}, k);
+      if constexpr (VE >= 8) {
+        byte_of(std::integral_constant<int, 2>{}, k);
+        byte_of(std::integral_constant<int, 3>{}, k);
+      }
+    }
+  };
+
+  // Two register sets in turn: while one tile is computed the next is in flight, its pages known a step ahead. Every
+  // issue is unconditional (past the split it repeats the split's first page), so nothing is sunk into a branch.
+  int t0 = t_begin + wave * kTile;
+  if (t0 < t_end) {
+    int pgA[2], pgB[2];
+    Tile A, Bt;
+    load_pages(t0, pgA);
+    load_pages(t0 + kRound, pgB);
+    issue(t0, pgA, A);
+    issue(t0 + kRound, pgB, Bt);
+    load_pages(t0 + 2 * kRound, pgA);
+    for (;;) {
+      // A holds t0, Bt holds t0 + kRound
+      if (t0 + kTile <= t_end) compute(t0, A, std::false_type{});
+      else compute(t0, A, std::true_type{});
+      t0 += kRound;
+      if (t0 >= t_end) break;
+      load_pages(t0 + 2 * kRound, pgB);
+      issue(t0 + kRound, pgA, A);
+      if (t0 + kTile <= t_end) compute(t0, Bt, std::false_type{});
+      else compute(t0, Bt, std::true_type{});
+      t0 += kRound;
+      if (t0 >= t_end) break;
+      load_pages(t0 + 2 * kRound, pgA);
+      issue(t0 + kRound, pgB, Bt);
+    }
+  }
+
+  // ---- the waves' states through LDS: (m, l) per head, then the sums, parts added up
+  l = over_groups<SumOp>(l);
+  float* sm_ml = smem;                  // [wave][HB][2]
+  float* sm_o = smem + kW * HB * 2;     // [wave][nh][D]
+  const int g = col / NC;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[i][r] = over_parts<NC>(o[i][r]);
+  }
+  if (part == 0 && g < nh) {
+    if (lg == 0) *reinterpret_cast<float2*>(sm_ml + (wave * HB + g) * 2) = make_float2(m, l);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {  // rows 4 lg + r of the products: VE consecutive elements of D
+      float* dst = sm_o + (wave * nh + g) * D + (4 * lg + r) * VE;
+#pragma unroll
+      for (int i = 0; i < VE; i += 4) {
+        *reinterpret_cast<float4*>(dst + i) = make_float4(o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]);
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nh * (D / 4); i += 64 * kW) {
+    const int gg = i / (D / 4), d = (i - gg * (D / 4)) * 4;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) M = fmaxf(M, sm_ml[(w * HB + gg) * 2]);
+    float L = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      const float2 ml = *reinterpret_cast<const float2*>(sm_ml + (w * HB + gg) * 2);
+      const float wt = ml.x == -INFINITY ? 0.0f : fast_exp2((ml.x - M) * c2);
+      const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * nh + gg) * D + d);
+      L = fmaf(ml.y, wt, L);
+      acc.x = fmaf(x.x, wt, acc.x);
+      acc.y = fmaf(x.y, wt, acc.y);
+      acc.z = fmaf(x.z, wt, acc.z);
+      acc.w = fmaf(x.w, wt, acc.w);
+    }
+    const int h = h0 + gg;
+    if (si.n_split == 1) {
+      const float inv = 1.0f / L;
+      const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+      T* row = out + b * a.os0 + h * a.os1 + d;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) row[j] = from_f32<T>(fp4_saturate<T>(y[j]));
+    } else {
+      const int64_t ph = int64_t(h) * a.slots + si.first + si.split;
+      *reinterpret_cast<float4*>(ws_acc + ph * D + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(ws_ml + ph * 2) = make_float2(M == -INFINITY ? M : M * c2, L);
+    }
+  }
+}
+
+// One workgroup per (query head, row): zeros for an empty row, the fold of a row's splits otherwise (rows of one
+// split are finished).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_decode_fp4_merge_kernel(const int32_t* __restrict__ seqlen,
+                                                                     const int32_t* __restrict__ ws_rows,
+                                                                     const float* __restrict__ ws_ml,
+                                                                     const float* __restrict__ ws_acc,
+                                                                     T* __restrict__ out, Fp4DecodeArgs a) {
+  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
+  const int len = clamp_len(seqlen[b], a.max_blocks << a.bs_log2);
+  T* row = out + b * a.os0 + h * a.os1;
+  if (len == 0) {
+    row[d] = from_f32<T>(0.0f);
+    return;
+  }
+  const int first = ws_rows[2 * b], n_split = ws_rows[2 * b + 1];
+  if (n_split == 1) return;
+  const float* ml = ws_ml + (int64_t(h) * a.slots + first) * 2;
+  const float* acc = ws_acc + (int64_t(h) * a.slots + first) * D + d;
+  float M = -INFINITY, L = 0.0f, A = 0.0f;
+  for (int s = 0; s < n_split; ++s) M = fmaxf(M, ml[2 * s]);
+  for (int s = 0; s < n_split; ++s) {
+    const float wt = ml[2 * s] == -INFINITY ? 0.0f : fast_exp2(ml[2 * s] - M);
+    L = fmaf(ml[2 * s + 1], wt, L);
+    A = fmaf(acc[int64_t(s) * D], wt, A);
+  }
+  row[d] = from_f32<T>(fp4_saturate<T>(A / L));
 }
 
 int esize_of(int dtype) { return dtype == MI_F32 ? 4 : dtype == MI_F16 || dtype == MI_BF16 ? 2 : 0; }
@@ -80,21 +473,54 @@ bool fp4_dim(int D) { return D == 64 || D == 128 || D == 256; }
 
 bool fp4_block(int bs) { return bs >= 16 && (bs & (bs - 1)) == 0; }
 
+struct Fp4Plan {
+  int n_hchunks, cols, target, min_chunk, slots;
+  size_t rows_bytes, ml_bytes, acc_bytes;
+  size_t bytes() const { return rows_bytes + ml_bytes + acc_bytes; }
+};
+
+constexpr int kGroupsAimed = 768;  // three four-wave workgroups on each of the 256 CUs
+
+Fp4Plan make_plan(int B, int H, int H_kv, int D, int dtype) {
+  Fp4Plan p;
+  const int heads = dtype == MI_F32 ? kHeads<float> : kHeads<bf16_t>;
+  p.n_hchunks = (H / H_kv + heads - 1) / heads;
+  p.cols = H_kv * p.n_hchunks;
+  p.target = kGroupsAimed / p.cols > 1 ? kGroupsAimed / p.cols : 1;
+  p.min_chunk = kRound;
+  p.slots = p.target + B;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  p.rows_bytes = up(size_t(B) * 2 * sizeof(int32_t));
+  p.ml_bytes = up(size_t(p.slots) * H * 2 * sizeof(float));
+  p.acc_bytes = size_t(p.slots) * H * D * sizeof(float);
+  return p;
+}
+
 template <typename T, int D>
 int launch_d(const void* q, const void* k, const void* v, const int32_t* bt, const int32_t* seqlen, void* out,
-             const Fp4DecodeArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((paged_decode_fp4_kernel<T, D>), dim3(a.H, a.B), dim3(256), 0, s, static_cast<const T*>(q),
-                     static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), bt, seqlen, static_cast<T*>(out), a);
-  return launch_status("mi_paged_decode_fp4");
+             void* workspace, const Fp4DecodeArgs& a, const Fp4Plan& p, hipStream_t s) {
+  int32_t* ws_rows = static_cast<int32_t*>(workspace);
+  float* ws_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.rows_bytes);
+  float* ws_acc = ws_ml + p.ml_bytes / sizeof(float);
+  const int nh = a.G < kHeads<T> ? a.G : kHeads<T>;
+  const size_t lds = size_t(kW) * (kHeads<T> * 2 + nh * D) * sizeof(float);
+  hipLaunchKernelGGL((paged_decode_fp4_kernel<T, D>), dim3(p.slots, p.cols), dim3(64 * kW), lds, s,
+                     static_cast<const T*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), bt, seqlen,
+                     static_cast<T*>(out), ws_rows, ws_ml, ws_acc, a);
+  const int rc = launch_status("mi_paged_decode_fp4 (split kernel)");
+  if (rc != MI_OK) return rc;
+  hipLaunchKernelGGL((paged_decode_fp4_merge_kernel<T, D>), dim3(a.H, a.B), dim3(D), 0, s, seqlen, ws_rows, ws_ml, ws_acc,
+                     static_cast<T*>(out), a);
+  return launch_status("mi_paged_decode_fp4 (merge kernel)");
 }
 
 template <typename T>
 int launch_t(int D, const void* q, const void* k, const void* v, const int32_t* bt, const int32_t* seqlen, void* out,
-             const Fp4DecodeArgs& a, hipStream_t s) {
+             void* workspace, const Fp4DecodeArgs& a, const Fp4Plan& p, hipStream_t s) {
   switch (D) {
-    case 64: return launch_d<T, 64>(q, k, v, bt, seqlen, out, a, s);
-    case 128: return launch_d<T, 128>(q, k, v, bt, seqlen, out, a, s);
-    default: return launch_d<T, 256>(q, k, v, bt, seqlen, out, a, s);
+    case 64: return launch_d<T, 64>(q, k, v, bt, seqlen, out, workspace, a, p, s);
+    case 128: return launch_d<T, 128>(q, k, v, bt, seqlen, out, workspace, a, p, s);
+    default: return launch_d<T, 256>(q, k, v, bt, seqlen, out, workspace, a, p, s);
   }
 }
 
@@ -103,8 +529,12 @@ int launch_t(int D, const void* q, const void* k, const void* v, const int32_t* 
 
 extern "C" size_t mi_paged_decode_fp4_workspace_size(int B, int H, int H_kv, int D, int block_size, int max_blocks,
                                                      int dtype) {
-  (void)B, (void)H, (void)H_kv, (void)D, (void)block_size, (void)max_blocks, (void)dtype;
-  return 0;
+  using namespace miattn;
+  if (B < 1 || H < 1 || H_kv < 1 || H % H_kv != 0 || !fp4_dim(D) || !fp4_block(block_size) || max_blocks < 1 ||
+      esize_of(dtype) == 0) {
+    return 0;
+  }
+  return make_plan(B, H, H_kv, D, dtype).bytes();
 }
 
 extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
@@ -112,7 +542,6 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
                                    int max_blocks, const int64_t* strides, float scale, int dtype, void* workspace,
                                    size_t workspace_bytes, void* stream) {
   using namespace miattn;
-  (void)workspace, (void)workspace_bytes;
   if (esize_of(dtype) == 0) return fail(MI_ERR_INVALID, "mi_paged_decode_fp4: unknown dtype %d", dtype);
   if (B < 0 || H < 1 || H_kv < 1 || H % H_kv != 0) {
     return fail(MI_ERR_INVALID, "mi_paged_decode_fp4: n_head (%d) must be a multiple of n_kv_head (%d)", H, H_kv);
@@ -134,7 +563,8 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
   if ((long long)max_blocks * block_size * B > 2147483647LL) {
     return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: B * max_blocks * block_size must stay below 2^31 tokens");
   }
-  if (B > 65535 || H > 65535) {
+  const Fp4Plan p = make_plan(B, H, H_kv, D, dtype);
+  if (B > 65535 || H > 65535 || p.cols > 65535) {
     return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: grid too large (B=%d, H=%d)", B, H);
   }
   const int64_t* st = strides;
@@ -146,7 +576,14 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
   if (!ok) {
     return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: q, out, k_cache and v_cache need 16-byte aligned rows and heads");
   }
+  if (workspace == nullptr || workspace_bytes < p.bytes()) {
+    return fail(MI_ERR_WORKSPACE, "mi_paged_decode_fp4: workspace of %zu bytes < %zu needed", workspace_bytes, p.bytes());
+  }
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+    return fail(MI_ERR_WORKSPACE, "mi_paged_decode_fp4: workspace must be 16-byte aligned");
+  }
   Fp4DecodeArgs a;
+  a.n_hchunks = p.n_hchunks; a.target = p.target; a.min_chunk = p.min_chunk; a.slots = p.slots;
   a.B = B; a.H = H; a.H_kv = H_kv; a.G = H / H_kv; a.max_blocks = max_blocks;
   a.bs_log2 = __builtin_ctz(unsigned(block_size));
   a.qs0 = st[0]; a.qs1 = st[1]; a.ks0 = st[2]; a.ks1 = st[3]; a.vs0 = st[4]; a.vs1 = st[5];
@@ -154,8 +591,8 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
   a.scale_log2 = scale * 1.4426950408889634f;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case MI_BF16: return launch_t<bf16_t>(D, q, k_cache, v_cache, block_table, seqlen, out, a, s);
-    case MI_F16: return launch_t<f16_t>(D, q, k_cache, v_cache, block_table, seqlen, out, a, s);
-    default: return launch_t<float>(D, q, k_cache, v_cache, block_table, seqlen, out, a, s);
+    case MI_BF16: return launch_t<bf16_t>(D, q, k_cache, v_cache, block_table, seqlen, out, workspace, a, p, s);
+    case MI_F16: return launch_t<f16_t>(D, q, k_cache, v_cache, block_table, seqlen, out, workspace, a, p, s);
+    default: return launch_t<float>(D, q, k_cache, v_cache, block_table, seqlen, out, workspace, a, p, s);
   }
 }
