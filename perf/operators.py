@@ -221,17 +221,17 @@ def prepare(case, seed):
         s["q"] = [_normal(dg, case["B"], H, D, dtype=dt) for _ in range(L)]
         if own:
             plan = _package().paged_decode_fp4_plan(s["q"][0], s["k"], s["v"], s["table"], s["seqlen"])
-            s["step"] = lambda: [plan.run(i, s["q"][i]) for i in range(L)]
+            qs = s["q"]  # no call below holds the state itself: a cycle would keep its graph until some later capture
+            s["step"] = lambda: [plan.run(i, qs[i]) for i in range(L)]
     elif case["kind"] == "write":
         lengths, s["slots"], n_pages = _prompt_slots(case, g)
         s["k"] = [_normal(dg, sum(lengths), H_kv, D, dtype=dt) for _ in range(L)]
         s["v"] = [_normal(dg, sum(lengths), H_kv, D, dtype=dt) for _ in range(L)]
         s["pool"] = pool = _new_pool(case, n_pages)
         if own:
-            def step():
-                return [(pool.write_slots(i, s["slots"], s["k"][i], s["v"][i]), pool.read_slots(i, s["slots"]))[1]
-                        for i in range(L)]
-            s["step"] = step
+            slots, ks, vs = s["slots"], s["k"], s["v"]
+            s["step"] = lambda: [(pool.write_slots(i, slots, ks[i], vs[i]), pool.read_slots(i, slots))[1]
+                                 for i in range(L)]
     elif case["kind"] == "epilogue":
         lengths, s["slots"], n_pages = _prompt_slots(case, g)
         T = sum(lengths)
@@ -247,12 +247,13 @@ def prepare(case, seed):
         s["kw"] = (1 + 0.1 * _normal(dg, D)).to(dt)
         s["pool"] = pool = _new_pool(case, n_pages)
         if own:
+            slots, qkv, args, packed = s["slots"], s["qkv"], [s[n] for n in ("qw", "kw", "cos", "sin", "pos")], case["packed"]
+
             def one(i):
-                k = torch.empty(T, H_kv, D, dtype=dt, device=DEV) if case["packed"] else None
-                v = torch.empty(T, H_kv, D, dtype=dt, device=DEV) if case["packed"] else None
-                q = pool.write_qk_norm_rope(i, s["slots"], s["qkv"][i], s["qw"], s["kw"], s["cos"], s["sin"],
-                                            s["pos"], EPS, k_out=k, v_out=v)
-                return [q, *([k, v] if case["packed"] else []), *pool.read_slots(i, s["slots"])]
+                k = torch.empty(T, H_kv, D, dtype=dt, device=DEV) if packed else None
+                v = torch.empty(T, H_kv, D, dtype=dt, device=DEV) if packed else None
+                q = pool.write_qk_norm_rope(i, slots, qkv[i], *args, EPS, k_out=k, v_out=v)
+                return [q, *([k, v] if packed else []), *pool.read_slots(i, slots)]
             s["step"] = lambda: [one(i) for i in range(L)]
     else:
         order = torch.randperm(case["pages"], generator=g)
@@ -266,7 +267,8 @@ def prepare(case, seed):
         if own:
             pool = _package().PagedPool(L, case["pages"], case["block"], H_kv, D, dtype=dt, device=DEV)
             pool.keys, pool.values = s["keys"], s["values"]
-            s["step"] = lambda: (pool.copy_blocks(s["src"], s["dst"]), pool.keys, pool.values)[1:]
+            src, dst = s["src"], s["dst"]
+            s["step"] = lambda: (pool.copy_blocks(src, dst), pool.keys, pool.values)[1:]
     if own and case.get("graph"):
         s["graph"], s["outs"] = _captured(s["step"])
     return s
