@@ -34,14 +34,12 @@ namespace miattn {
 namespace {
 
 struct Fp4DecodeArgs {
-  int B, H, H_kv, G, n_hchunks, bs_log2, max_blocks, target, min_chunk, slots;
+  int B, H, H_kv, G, n_hchunks, bs_log2, max_blocks, target, slots;
   int64_t qs0, qs1, ks0, ks1, vs0, vs1, os0, os1, bts0;
   float scale_log2;
 };
 
-constexpr int kW = 4;           // waves per workgroup
 constexpr int kTile = 32;       // tokens per wave and step
-constexpr int kRound = kW * kTile;
 constexpr float kRaise = 8.0f;  // log2 units a tile's maximum may be past the running one
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -80,18 +78,14 @@ __device__ __forceinline__ float over_parts(float x) {
   return x;
 }
 
-// Tokens per split: total / target in whole rounds, at least min_chunk. The splits are then at most target
-// and one partial split per row.
-__device__ __forceinline__ int chunk_of(int total, const Fp4DecodeArgs& a) {
-  const int even = int((uint32_t(total) + uint32_t(a.target) - 1u) / uint32_t(a.target));
-  const int rounds = (even + kRound - 1) / kRound * kRound;
-  return rounds > a.min_chunk ? rounds : a.min_chunk;
-}
-
 struct Fp4Split {
   int b, split, n_split, first, chunk, len;
 };
-// This workgroup's (row, split): every wave derives it from the row lengths, 64 rows at a time.
+// This workgroup's (row, split), derived by every wave from the row lengths, 64 rows at a time. Tokens per split:
+// total / target in whole rounds; as long as the splits of the first 64 rows (one per row at least, an
+// empty row's writes its zeros) are more than target the chunk grows, up to kFitSteps times.
+constexpr int kFitSteps = 8;
+template <int kRound>
 __device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, const Fp4DecodeArgs& a, int w,
                                            Fp4Split& si) {
   const int lane = __lane_id();
@@ -102,11 +96,22 @@ __device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, c
     const int row = r0 + lane;
     total += __builtin_amdgcn_readlane(wave_inclusive_scan(row < a.B ? clamp_len(seqlen[row], capacity) : 0), 63);
   }
-  const int chunk = chunk_of(total, a);
+  const uint32_t even = (uint32_t(total) + uint32_t(a.target) - 1u) / uint32_t(a.target);
+  int chunk = int((even + kRound - 1) / kRound) * kRound;
+  chunk = chunk > kRound ? chunk : kRound;
+  auto count = [&](int len, int row) {
+    const int n = int((uint32_t(len) + uint32_t(chunk) - 1u) / uint32_t(chunk));
+    return row < a.B ? (n > 1 ? n : 1) : 0;
+  };
+  int n = count(len_first, lane), incl = wave_inclusive_scan(n);
+  const int step = (chunk / 16 + kRound) / kRound * kRound;
+  for (int i = 0; i < kFitSteps && __builtin_amdgcn_readlane(incl, 63) > a.target; ++i) {
+    chunk += step;
+    n = count(len_first, lane);
+    incl = wave_inclusive_scan(n);
+  }
   int len = len_first, base = 0;
   for (int r0 = 0;;) {
-    const int n = int((uint32_t(len) + uint32_t(chunk) - 1u) / uint32_t(chunk));
-    const int incl = wave_inclusive_scan(n);
     const uint64_t owner = __ballot(w >= base + incl - n && w < base + incl);
     if (owner != 0) {
       const int o = __ffsll(static_cast<unsigned long long>(owner)) - 1;
@@ -124,37 +129,43 @@ __device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, c
     base += __builtin_amdgcn_readlane(incl, 63);
     const int row = r0 + lane;
     len = row < a.B ? clamp_len(seqlen[row], capacity) : 0;
+    n = count(len, row);
+    incl = wave_inclusive_scan(n);
   }
 }
 
-template <typename T, int D>
-struct Fp4Tile {
-  static constexpr int KW = D / 32;                  // code dwords of K per lane and 16 tokens
-  static constexpr int KS = D == 256 ? 2 : 1;        // scales of those
-  static constexpr int VE = D / 16;                  // V elements per lane and token
-  static constexpr int VW = VE >= 8 ? VE / 8 : 1;    // dwords they take (D 64: half of one)
-  uint32_t k[2][KW], ks[2][KS], v[2][4][VW], vs[2];
-};
+// One split's partial of one column: sums of nh heads, then (m, l) of each; whole 16 bytes.
+__host__ __device__ constexpr int partial_floats(int nh, int D) { return nh * D + (2 * nh + 3) / 4 * 4; }
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
+// Device-scope 16- and 8-byte accesses of the partials: written through to, and read from, the level that all XCDs share,
+// so no cache has to be written back or dropped for them.
+constexpr int kSc1 = 16;
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ auto partial_rsrc(float* p, int64_t floats) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, (short)0, int(floats * 4), 0x00020000);
+}
+
+#ifndef FP4_MINW
+#define FP4_MINW 1
+#endif
+template <typename T, int D, int kW>
+__global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
     const T* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const int32_t* __restrict__ block_table, const int32_t* __restrict__ seqlen, T* __restrict__ out,
-    int32_t* __restrict__ ws_rows, float* __restrict__ ws_ml, float* __restrict__ ws_acc, Fp4DecodeArgs a) {
-  using Tile = Fp4Tile<T, D>;
-  constexpr int KW = Tile::KW, KS = Tile::KS, VE = Tile::VE, VW = Tile::VW;
+    int32_t* __restrict__ counters, float* __restrict__ partials, Fp4DecodeArgs a) {
+  constexpr int kRound = kW * kTile;
+  constexpr int KW = D / 32;                // code dwords of K per lane and 16 tokens
+  constexpr int KS = D == 256 ? 2 : 1;      // scales of those
+  constexpr int VE = D / 16;                // V elements per lane and token
+  constexpr int VW = VE >= 8 ? VE / 8 : 1;  // dwords they take (D 64: half of one)
   constexpr int NC = kCols<T>, HB = kHeads<T>;
   extern __shared__ __align__(16) float smem[];  // per wave: (m, l) of HB heads, then nh x D sums
 
   Fp4Split si;
-  if (!plan_split(seqlen, a, blockIdx.x, si)) return;  // uniform
+  if (!plan_split<kRound>(seqlen, a, blockIdx.x, si)) return;  // uniform
   const int b = si.b;
   const int t_begin = si.split * si.chunk;
   const int t_end = min(si.len, t_begin + si.chunk);
-  if (si.split == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
-    ws_rows[2 * b] = si.first;
-    ws_rows[2 * b + 1] = si.n_split;
-  }
   const int kvh = blockIdx.y / a.n_hchunks;
   const int hch = blockIdx.y - kvh * a.n_hchunks;
   const int nh = min(HB, a.G - hch * HB);  // query heads of this workgroup
@@ -196,46 +207,56 @@ __global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
   const int v_lane = lg * 4 * (D / 2) + col * (D / 32);
   const int vs_lane = bs * (D / 2) + (col * VE / kFp4Group) * bs + lg * 4;
 
-  // first token of 16-token half u of the tile at t0; a half past the end repeats the first (masked out)
-  auto half_at = [&](int t0, int u) { return t0 + 16 * u < t_end ? t0 + 16 * u : t0; };
+  // First token of 16-token half u of the tile at t0; a half past the end repeats the first (masked out), a
+  // tile past the end the split's first.
+  auto half_at = [&](int t0, int u) {
+    t0 = t0 < t_end ? t0 : t_begin;
+    return t0 + 16 * u < t_end ? t0 + 16 * u : t0;
+  };
   auto load_pages = [&](int t0, int (&pg)[2]) {
-    t0 = t0 < t_end ? t0 : t_begin;  // past the split: a page that is there, not used
 #pragma unroll
     for (int u = 0; u < 2; ++u) pg[u] = bt_row[half_at(t0, u) >> a.bs_log2];
   };
-  auto issue = [&](int t0, const int (&pg)[2], Tile& t) {
-    t0 = t0 < t_end ? t0 : t_begin;
+  uint32_t tk[2][KW], tks[2][KS], tv[2][4][VW], tvs[2];  // one tile: codes and scales of K, of V
+  auto issue_k = [&](int t0, const int (&pg)[2]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int at = half_at(t0, u) & (bs - 1);
       const uint8_t* kp = kc + (int64_t(pg[u]) * a.ks0 + kvh * a.ks1);
-      const uint8_t* vp = vc + (int64_t(pg[u]) * a.vs0 + kvh * a.vs1);
       const uint8_t* kr = kp + (at * (D / 2) + k_lane);
 #pragma unroll
       for (int i = 0; i < KW; i += 4) {
         if constexpr (KW >= 4) {
           const uint4 w = load16_nt(kr + 4 * i);
-          t.k[u][i] = w.x; t.k[u][i + 1] = w.y; t.k[u][i + 2] = w.z; t.k[u][i + 3] = w.w;
+          tk[u][i] = w.x; tk[u][i + 1] = w.y; tk[u][i + 2] = w.z; tk[u][i + 3] = w.w;
         } else {
           const uint2 w = *reinterpret_cast<const uint2*>(kr);
-          t.k[u][0] = w.x; t.k[u][1] = w.y;
+          tk[u][0] = w.x; tk[u][1] = w.y;
         }
       }
 #pragma unroll
-      for (int i = 0; i < KS; ++i) t.ks[u][i] = kp[at + ks_lane + i * bs];
+      for (int i = 0; i < KS; ++i) tks[u][i] = kp[at + ks_lane + i * bs];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto issue_v = [&](int t0, const int (&pg)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int at = half_at(t0, u) & (bs - 1);
+      const uint8_t* vp = vc + (int64_t(pg[u]) * a.vs0 + kvh * a.vs1);
       const uint8_t* vr = vp + (at * (D / 2) + v_lane);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (VE == 4) {
-          t.v[u][j][0] = *reinterpret_cast<const uint16_t*>(vr + j * (D / 2));
+          tv[u][j][0] = *reinterpret_cast<const uint16_t*>(vr + j * (D / 2));
         } else if constexpr (VE == 8) {
-          t.v[u][j][0] = *reinterpret_cast<const uint32_t*>(vr + j * (D / 2));
+          tv[u][j][0] = *reinterpret_cast<const uint32_t*>(vr + j * (D / 2));
         } else {
           const uint2 w = *reinterpret_cast<const uint2*>(vr + j * (D / 2));
-          t.v[u][j][0] = w.x; t.v[u][j][1] = w.y;
+          tv[u][j][0] = w.x; tv[u][j][1] = w.y;
         }
       }
-      t.vs[u] = *reinterpret_cast<const uint32_t*>(vp + at + vs_lane);
+      tvs[u] = *reinterpret_cast<const uint32_t*>(vp + at + vs_lane);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -247,7 +268,9 @@ __global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
   const float raise = fminf(kRaise / c2, 3.0e38f);
   const uint32_t cut1 = part >= 1 ? 0xffff0000u : 0u, cut2 = part >= 2 ? 0xffff0000u : 0u;
 
-  auto compute = [&](int t0, const Tile& t, auto masked) {
+  // One tile: the scores from K, the running maximum, the sums from V; `next` issues the loads that come into K's, then
+  // into V's registers.
+  auto compute = [&](int t0, auto masked, auto&& next_k, auto&& next_v) {
     constexpr bool kMasked = decltype(masked)::value;
     __builtin_amdgcn_sched_barrier(0);
     f32x4_t s[2];
@@ -256,8 +279,8 @@ __global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
       s[u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int kk = 0; kk < KW; ++kk) {
-        const float sc = fp4_scale(t.ks[u][kk * 8 * KS / (D / 4)]);
-        const uint32_t w = t.k[u][kk];
+        const float sc = fp4_scale(tks[u][kk * 8 * KS / (D / 4)]);
+        const uint32_t w = tk[u][kk];
         const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0);
         const auto p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1);
         const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2);
@@ -267,6 +290,7 @@ __global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
         s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[kk], s[u], 0, 0, 0);
       }
     }
+    next_k();
     // this lane's 8 tokens: t0 + 16 u + 4 lg + i
     float most = -INFINITY;
 #pragma unroll
@@ -315,7 +339,7 @@ __global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t w = t.vs[u];
+        const uint32_t w = tvs[u];
         uint32_t x = i == 3 ? w >> 1 : w << (23 - 8 * i);
         bool in = true;
         if constexpr (kMasked) {  // garbage past the end may be a NaN scale, which 0 * NaN would keep
@@ -324,7 +348,7 @@ __global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
         }
         vsc[4 * u + i] = __uint_as_float(x);
 #pragma unroll
-        for (int k = 0; k < VW; ++k) vw[4 * u + i][k] = in ? t.v[u][i][k] : 0u;
+        for (int k = 0; k < VW; ++k) vw[4 * u + i][k] = in ? tv[u][i][k] : 0u;
       }
     }
     auto byte_of = [&](auto which, int k) {
@@ -353,34 +377,26 @@ __global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
         byte_of(std::integral_constant<int, 3>{}, k);
       }
     }
+    next_v();
   };
 
-  // Two register sets in turn: while one tile is computed the next is in flight, its pages known a step ahead. Every
-  // issue is unconditional (past the split it repeats the split's first page), so nothing is sunk into a branch.
+  // Loads stay one tile ahead of their use: the next tile's K is on its way from when this tile's scores are made, its
+  // V from when the sums are, and its pages are known a tile earlier. Every load of the loop is unconditional.
   int t0 = t_begin + wave * kTile;
   if (t0 < t_end) {
-    int pgA[2], pgB[2];
-    Tile A, Bt;
-    load_pages(t0, pgA);
-    load_pages(t0 + kRound, pgB);
-    issue(t0, pgA, A);
-    issue(t0 + kRound, pgB, Bt);
-    load_pages(t0 + 2 * kRound, pgA);
-    for (;;) {
-      // A holds t0, Bt holds t0 + kRound
-      if (t0 + kTile <= t_end) compute(t0, A, std::false_type{});
-      else compute(t0, A, std::true_type{});
-      t0 += kRound;
-      if (t0 >= t_end) break;
-      load_pages(t0 + 2 * kRound, pgB);
-      issue(t0 + kRound, pgA, A);
-      if (t0 + kTile <= t_end) compute(t0, Bt, std::false_type{});
-      else compute(t0, Bt, std::true_type{});
-      t0 += kRound;
-      if (t0 >= t_end) break;
-      load_pages(t0 + 2 * kRound, pgA);
-      issue(t0 + kRound, pgB, Bt);
+    auto none = [] {};
+    int pg[2], pn[2];
+    load_pages(t0, pg);
+    load_pages(t0 + kRound, pn);
+    issue_k(t0, pg);
+    issue_v(t0, pg);
+    for (; t0 + kRound < t_end; t0 += kRound) {  // a tile with another behind it is whole
+      const int t1 = t0 + kRound;
+      compute(t0, std::false_type{}, [&] { issue_k(t1, pn); pg[0] = pn[0]; pg[1] = pn[1]; load_pages(t1 + kRound, pn); },
+              [&] { issue_v(t1, pg); });
     }
+    if (t0 + kTile <= t_end) compute(t0, std::false_type{}, none, none);
+    else compute(t0, std::true_type{}, none, none);
   }
 
   // ---- the waves' states through LDS: (m, l) per head, then the sums, parts added up
@@ -405,6 +421,8 @@ __global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
     }
   }
   __syncthreads();
+  const int part_floats = partial_floats(min(HB, a.G), D);
+  const auto mine = partial_rsrc(partials + (int64_t(blockIdx.x) * gridDim.y + blockIdx.y) * part_floats, part_floats);
   for (int i = threadIdx.x; i < nh * (D / 4); i += 64 * kW) {
     const int gg = i / (D / 4), d = (i - gg * (D / 4)) * 4;
     float M = -INFINITY;
@@ -423,48 +441,113 @@ __global__ __launch_bounds__(64 * kW) void paged_decode_fp4_kernel(
       acc.z = fmaf(x.z, wt, acc.z);
       acc.w = fmaf(x.w, wt, acc.w);
     }
-    const int h = h0 + gg;
     if (si.n_split == 1) {
-      const float inv = 1.0f / L;
+      const float inv = si.len > 0 ? 1.0f / L : 0.0f;
       const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-      T* row = out + b * a.os0 + h * a.os1 + d;
+      T* row = out + b * a.os0 + (h0 + gg) * a.os1 + d;
 #pragma unroll
       for (int j = 0; j < 4; ++j) row[j] = from_f32<T>(fp4_saturate<T>(y[j]));
     } else {
-      const int64_t ph = int64_t(h) * a.slots + si.first + si.split;
-      *reinterpret_cast<float4*>(ws_acc + ph * D + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(ws_ml + ph * 2) = make_float2(M == -INFINITY ? M : M * c2, L);
+      const u32x4_nt val = {__float_as_uint(acc.x), __float_as_uint(acc.y), __float_as_uint(acc.z), __float_as_uint(acc.w)};
+      __builtin_amdgcn_raw_buffer_store_b128(val, mine, (gg * D + d) * 4, 0, kSc1);
+      if (d == 0) {
+        const u32x2_t ml = {__float_as_uint(M == -INFINITY ? M : M * c2), __float_as_uint(L)};
+        __builtin_amdgcn_raw_buffer_store_b64(ml, mine, (nh * D + gg * 2) * 4, 0, kSc1);
+      }
     }
   }
-}
+  if (si.n_split == 1) return;
 
-// One workgroup per (query head, row): zeros for an empty row, the fold of a row's splits otherwise (rows of one
-// split are finished).
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_decode_fp4_merge_kernel(const int32_t* __restrict__ seqlen,
-                                                                     const int32_t* __restrict__ ws_rows,
-                                                                     const float* __restrict__ ws_ml,
-                                                                     const float* __restrict__ ws_acc,
-                                                                     T* __restrict__ out, Fp4DecodeArgs a) {
-  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const int len = clamp_len(seqlen[b], a.max_blocks << a.bs_log2);
-  T* row = out + b * a.os0 + h * a.os1;
-  if (len == 0) {
-    row[d] = from_f32<T>(0.0f);
-    return;
+  // ---- the last of the row's workgroups to get here folds their partials: each has its own at the shared level
+  // before it counts itself, and the last one reads them from there
+  int* sm_last = reinterpret_cast<int*>(smem);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int* counter = counters + int64_t(b) * gridDim.y + blockIdx.y;
+    const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *sm_last = before == si.n_split - 1;
+    if (before == si.n_split - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  const int first = ws_rows[2 * b], n_split = ws_rows[2 * b + 1];
-  if (n_split == 1) return;
-  const float* ml = ws_ml + (int64_t(h) * a.slots + first) * 2;
-  const float* acc = ws_acc + (int64_t(h) * a.slots + first) * D + d;
-  float M = -INFINITY, L = 0.0f, A = 0.0f;
-  for (int s = 0; s < n_split; ++s) M = fmaxf(M, ml[2 * s]);
-  for (int s = 0; s < n_split; ++s) {
-    const float wt = ml[2 * s] == -INFINITY ? 0.0f : fast_exp2(ml[2 * s] - M);
-    L = fmaf(ml[2 * s + 1], wt, L);
-    A = fmaf(acc[int64_t(s) * D], wt, A);
+  __syncthreads();
+  if (!*sm_last) return;  // uniform
+  __syncthreads();        // sm_last has been read by every wave; its words are used again below
+  const auto row_parts = partial_rsrc(partials + (int64_t(si.first) * gridDim.y + blockIdx.y) * part_floats,
+                                      (int64_t(si.n_split - 1) * gridDim.y + 1) * part_floats);
+  // NG groups of threads take the splits in turn, kFold at a time, and are folded through LDS
+  const int lanes = nh * (D / 4);                       // threads that hold one split's sums, 4 each
+  const int ng = max(1, 64 * kW / lanes);               // 64 kW threads, lanes a multiple of 16
+  float* sm_f = smem;                                   // [group][lanes] sums, then [group][lanes] (m, l)
+  float* sm_g = smem + ng * lanes * 4;
+  constexpr int kFold = 4;
+  for (int i0 = 0; i0 < lanes; i0 += 64 * kW) {  // more than one pass where a column has more sums than threads
+    const int grp = ng > 1 ? threadIdx.x / lanes : 0;
+    const int i = ng > 1 ? threadIdx.x - grp * lanes : i0 + threadIdx.x;
+    const bool mine_too = grp < ng && i < lanes;
+    const int gg = mine_too ? i / (D / 4) : 0, d = mine_too ? (i - gg * (D / 4)) * 4 : 0;
+    float M = -INFINITY, L = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = grp; s0 < si.n_split; s0 += kFold * ng) {
+      u32x2_t ml[kFold];
+      u32x4_nt x[kFold];
+#pragma unroll
+      for (int j = 0; j < kFold; ++j) {
+        const int s = min(s0 + j * ng, si.n_split - 1);
+        const int at = (s * int(gridDim.y) * part_floats + gg * D + d) * 4;
+        const int at_ml = (s * int(gridDim.y) * part_floats + nh * D + gg * 2) * 4;
+        ml[j] = __builtin_amdgcn_raw_buffer_load_b64(row_parts, at_ml, 0, kSc1);
+        x[j] = __builtin_amdgcn_raw_buffer_load_b128(row_parts, at, 0, kSc1);
+      }
+      float mj[kFold], top = M;
+#pragma unroll
+      for (int j = 0; j < kFold; ++j) {
+        mj[j] = s0 + j * ng < si.n_split ? __uint_as_float(ml[j].x) : -INFINITY;
+        top = fmaxf(top, mj[j]);
+      }
+      const float again = M == -INFINITY ? 0.0f : fast_exp2(M - top);
+      M = top;
+      L *= again;
+      acc.x *= again; acc.y *= again; acc.z *= again; acc.w *= again;
+#pragma unroll
+      for (int j = 0; j < kFold; ++j) {
+        if (s0 + j * ng < si.n_split) {
+          const float wt = mj[j] == -INFINITY ? 0.0f : fast_exp2(mj[j] - top);
+          L = fmaf(__uint_as_float(ml[j].y), wt, L);
+          acc.x = fmaf(__uint_as_float(x[j].x), wt, acc.x);
+          acc.y = fmaf(__uint_as_float(x[j].y), wt, acc.y);
+          acc.z = fmaf(__uint_as_float(x[j].z), wt, acc.z);
+          acc.w = fmaf(__uint_as_float(x[j].w), wt, acc.w);
+        }
+      }
+    }
+    if (ng > 1) {
+      if (mine_too) {
+        *reinterpret_cast<float4*>(sm_f + (grp * lanes + i) * 4) = acc;
+        *reinterpret_cast<float2*>(sm_g + (grp * lanes + i) * 2) = make_float2(M, L);
+      }
+      __syncthreads();
+      if (grp > 0) return;
+      for (int w = 1; w < min(ng, si.n_split); ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(sm_f + (w * lanes + i) * 4);
+        const float2 ml = *reinterpret_cast<const float2*>(sm_g + (w * lanes + i) * 2);
+        const float top = fmaxf(M, ml.x);
+        const float w0 = M == -INFINITY ? 0.0f : fast_exp2(M - top), w1 = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
+        M = top;
+        L = L * w0 + ml.y * w1;
+        acc.x = acc.x * w0 + x.x * w1;
+        acc.y = acc.y * w0 + x.y * w1;
+        acc.z = acc.z * w0 + x.z * w1;
+        acc.w = acc.w * w0 + x.w * w1;
+      }
+    }
+    if (mine_too) {
+      const float inv = 1.0f / L;
+      const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+      T* row = out + b * a.os0 + (h0 + gg) * a.os1 + d;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) row[j] = from_f32<T>(fp4_saturate<T>(y[j]));
+    }
   }
-  row[d] = from_f32<T>(fp4_saturate<T>(A / L));
 }
 
 int esize_of(int dtype) { return dtype == MI_F32 ? 4 : dtype == MI_F16 || dtype == MI_BF16 ? 2 : 0; }
@@ -473,45 +556,52 @@ bool fp4_dim(int D) { return D == 64 || D == 128 || D == 256; }
 
 bool fp4_block(int bs) { return bs >= 16 && (bs & (bs - 1)) == 0; }
 
+#ifndef FP4_GROUPS8
+#define FP4_GROUPS8 256
+#endif
+#ifndef FP4_GROUPS4
+#define FP4_GROUPS4 512
+#endif
+#ifndef FP4_LIMIT8
+#define FP4_LIMIT8 256
+#endif
 struct Fp4Plan {
-  int n_hchunks, cols, target, min_chunk, slots;
-  size_t rows_bytes, ml_bytes, acc_bytes;
-  size_t bytes() const { return rows_bytes + ml_bytes + acc_bytes; }
+  int n_hchunks, cols, waves, target, slots, nh;
+  size_t counter_bytes, partial_bytes;
+  size_t bytes() const { return counter_bytes + partial_bytes; }
 };
-
-constexpr int kGroupsAimed = 768;  // three four-wave workgroups on each of the 256 CUs
 
 Fp4Plan make_plan(int B, int H, int H_kv, int D, int dtype) {
   Fp4Plan p;
   const int heads = dtype == MI_F32 ? kHeads<float> : kHeads<bf16_t>;
   p.n_hchunks = (H / H_kv + heads - 1) / heads;
   p.cols = H_kv * p.n_hchunks;
-  p.target = kGroupsAimed / p.cols > 1 ? kGroupsAimed / p.cols : 1;
-  p.min_chunk = kRound;
+  p.nh = H / H_kv < heads ? H / H_kv : heads;
+  p.waves = int64_t(B) * p.cols <= FP4_LIMIT8 ? 8 : 4;
+  const int groups = p.waves == 8 ? FP4_GROUPS8 : FP4_GROUPS4;
+  p.target = groups / p.cols > 1 ? groups / p.cols : 1;
   p.slots = p.target + B;
-  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  p.rows_bytes = up(size_t(B) * 2 * sizeof(int32_t));
-  p.ml_bytes = up(size_t(p.slots) * H * 2 * sizeof(float));
-  p.acc_bytes = size_t(p.slots) * H * D * sizeof(float);
+  p.counter_bytes = (size_t(B) * p.cols * sizeof(int32_t) + 255) / 256 * 256;
+  p.partial_bytes = size_t(p.slots) * p.cols * partial_floats(p.nh, D) * sizeof(float);
   return p;
 }
 
 template <typename T, int D>
 int launch_d(const void* q, const void* k, const void* v, const int32_t* bt, const int32_t* seqlen, void* out,
              void* workspace, const Fp4DecodeArgs& a, const Fp4Plan& p, hipStream_t s) {
-  int32_t* ws_rows = static_cast<int32_t*>(workspace);
-  float* ws_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.rows_bytes);
-  float* ws_acc = ws_ml + p.ml_bytes / sizeof(float);
-  const int nh = a.G < kHeads<T> ? a.G : kHeads<T>;
-  const size_t lds = size_t(kW) * (kHeads<T> * 2 + nh * D) * sizeof(float);
-  hipLaunchKernelGGL((paged_decode_fp4_kernel<T, D>), dim3(p.slots, p.cols), dim3(64 * kW), lds, s,
-                     static_cast<const T*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), bt, seqlen,
-                     static_cast<T*>(out), ws_rows, ws_ml, ws_acc, a);
-  const int rc = launch_status("mi_paged_decode_fp4 (split kernel)");
-  if (rc != MI_OK) return rc;
-  hipLaunchKernelGGL((paged_decode_fp4_merge_kernel<T, D>), dim3(a.H, a.B), dim3(D), 0, s, seqlen, ws_rows, ws_ml, ws_acc,
-                     static_cast<T*>(out), a);
-  return launch_status("mi_paged_decode_fp4 (merge kernel)");
+  int32_t* counters = static_cast<int32_t*>(workspace);
+  float* partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.counter_bytes);
+  auto go = [&](auto waves) {
+    constexpr int kW = decltype(waves)::value;
+    // the waves' states; the fold of the splits needs 6 floats per thread at most
+    const size_t states = size_t(kW) * (kHeads<T> * 2 + p.nh * D), fold = size_t(64 * kW) * 6;
+    const size_t lds = (states > fold ? states : fold) * sizeof(float);
+    hipLaunchKernelGGL((paged_decode_fp4_kernel<T, D, kW>), dim3(p.slots, p.cols), dim3(64 * kW), lds, s,
+                       static_cast<const T*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), bt, seqlen,
+                       static_cast<T*>(out), counters, partials, a);
+  };
+  if (p.waves == 8) go(std::integral_constant<int, 8>{}); else go(std::integral_constant<int, 4>{});
+  return launch_status("mi_paged_decode_fp4");
 }
 
 template <typename T>
@@ -583,7 +673,7 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
     return fail(MI_ERR_WORKSPACE, "mi_paged_decode_fp4: workspace must be 16-byte aligned");
   }
   Fp4DecodeArgs a;
-  a.n_hchunks = p.n_hchunks; a.target = p.target; a.min_chunk = p.min_chunk; a.slots = p.slots;
+  a.n_hchunks = p.n_hchunks; a.target = p.target; a.slots = p.slots;
   a.B = B; a.H = H; a.H_kv = H_kv; a.G = H / H_kv; a.max_blocks = max_blocks;
   a.bs_log2 = __builtin_ctz(unsigned(block_size));
   a.qs0 = st[0]; a.qs1 = st[1]; a.ks0 = st[2]; a.ks1 = st[3]; a.vs0 = st[4]; a.vs1 = st[5];

@@ -222,7 +222,7 @@ def paged_decode_fp4(q, k_cache, v_cache, block_table, seqlen, *, scale: float |
     with _lib.on_device(q.device):
         out = torch.empty_like(q)
         n_ws = _workspace_bytes(g, q.dtype)
-        ws = torch.empty(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
+        ws = torch.zeros(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
         rc = _lib.lib.mi_paged_decode_fp4(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lens.data_ptr(), out.data_ptr(),
             *g.dims(), _strides(q, k_cache, v_cache, out, table),
@@ -262,7 +262,7 @@ class Fp4DecodePlan:
         self._table, self._seqlen = block_table, seqlen
         self._strides = _strides(q, ks[0], vs[0], q, block_table)
         n_ws = _workspace_bytes(g, q.dtype)
-        self._ws = torch.empty(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
+        self._ws = torch.zeros(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
         self._frozen = (*g.dims(), self._strides, float(1.0 / math.sqrt(g.head_dim) if scale is None else scale),
                         _lib.dtype_code(q.dtype), None if self._ws is None else self._ws.data_ptr(), n_ws)
 
