@@ -53,25 +53,22 @@ __global__ __launch_bounds__(256) void fp4_write_kernel(const T* __restrict__ k,
                                                         int64_t vs1, int64_t vs2, int32_t* err) {
   constexpr int LPR = D / 8, TPW = 64 / LPR;
   const int lane = threadIdx.x & 63, c = lane % LPR;
-  const int64_t waves = int64_t(gridDim.x) * 4;
-  const int64_t total = (n_tokens + TPW - 1) / TPW * H_kv;
-  for (int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); i < total; i += waves) {
-    const int64_t grp = i / H_kv;
-    const int head = int(i - grp * H_kv);
-    const int64_t token = grp * TPW + lane / LPR;
-    if (token >= n_tokens) continue;  // whole quads leave together
-    float x[8], y[8];
-    load8<T, kVec>(k + token * ks0 + head * ks1 + c * 8 * ks2, ks2, x);
-    load8<T, kVec>(v + token * vs0 + head * vs1 + c * 8 * vs2, vs2, y);
-    const int64_t slot = int64_t(slots[token]);
-    if (slot < 0 || slot >= pool.n_slots) {
-      report(err, token);
-      continue;
-    }
-    const Fp4Place at = fp4_place<D>(pool, slot, head, c);
-    fp4_put<D>(pool.k, at, c, x);
-    fp4_put<D>(pool.v, at, c, y);
+  const uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 6);  // this wave's (group, head), the same for its lanes
+  const uint32_t grp = i / uint32_t(H_kv);
+  const int head = int(i - grp * uint32_t(H_kv));
+  const int64_t token = int64_t(grp) * TPW + lane / LPR;
+  if (token >= n_tokens) return;  // whole quads leave together
+  float x[8], y[8];
+  load8<T, kVec>(k + token * ks0 + head * ks1 + c * 8 * ks2, ks2, x);
+  load8<T, kVec>(v + token * vs0 + head * vs1 + c * 8 * vs2, vs2, y);
+  const int64_t slot = int64_t(slots[token]);
+  if (slot < 0 || slot >= pool.n_slots) {
+    report(err, token);
+    return;
   }
+  const Fp4Place at = fp4_place<D>(pool, slot, head, c);
+  fp4_put<D>(pool.k, at, c, x);
+  fp4_put<D>(pool.v, at, c, y);
 }
 
 template <typename T, int D, typename IdxT>
@@ -80,33 +77,30 @@ __global__ __launch_bounds__(256) void fp4_read_kernel(Fp4Pool pool, const IdxT*
                                                        int32_t* err) {
   constexpr int LPR = D / 8, TPW = 64 / LPR;
   const int lane = threadIdx.x & 63, c = lane % LPR;
-  const int64_t waves = int64_t(gridDim.x) * 4;
-  const int64_t total = (n_tokens + TPW - 1) / TPW * H_kv;
-  for (int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); i < total; i += waves) {
-    const int64_t grp = i / H_kv;
-    const int head = int(i - grp * H_kv);
-    const int64_t token = grp * TPW + lane / LPR;
-    if (token >= n_tokens) continue;
-    const int64_t slot = int64_t(slots[token]);
-    float x[8] = {}, y[8] = {};
-    if (slot < 0 || slot >= pool.n_slots) {
-      report(err, token);  // its rows come back as zeros
-    } else {
-      const Fp4Place at = fp4_place<D>(pool, slot, head, c);
-      const uint32_t wk = *reinterpret_cast<const uint32_t*>(pool.k + at.code);
-      const uint32_t wv = *reinterpret_cast<const uint32_t*>(pool.v + at.code);
-      fp4_decode(wk, fp4_scale(pool.k[at.scale]), x);
-      fp4_decode(wv, fp4_scale(pool.v[at.scale]), y);
+  const uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const uint32_t grp = i / uint32_t(H_kv);
+  const int head = int(i - grp * uint32_t(H_kv));
+  const int64_t token = int64_t(grp) * TPW + lane / LPR;
+  if (token >= n_tokens) return;
+  const int64_t slot = int64_t(slots[token]);
+  float x[8] = {}, y[8] = {};
+  if (slot < 0 || slot >= pool.n_slots) {
+    report(err, token);  // its rows come back as zeros
+  } else {
+    const Fp4Place at = fp4_place<D>(pool, slot, head, c);
+    const uint32_t wk = *reinterpret_cast<const uint32_t*>(pool.k + at.code);
+    const uint32_t wv = *reinterpret_cast<const uint32_t*>(pool.v + at.code);
+    fp4_decode(wk, fp4_scale(pool.k[at.scale]), x);
+    fp4_decode(wv, fp4_scale(pool.v[at.scale]), y);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = fp4_saturate<T>(x[j]);
-        y[j] = fp4_saturate<T>(y[j]);
-      }
+    for (int j = 0; j < 8; ++j) {
+      x[j] = fp4_saturate<T>(x[j]);
+      y[j] = fp4_saturate<T>(y[j]);
     }
-    const int64_t dst = (token * H_kv + head) * D + c * 8;
-    store8(k + dst, x);
-    store8(v + dst, y);
   }
+  const int64_t dst = (token * H_kv + head) * D + c * 8;
+  store8(k + dst, x);
+  store8(v + dst, y);
 }
 
 struct EpilogueArgs {
@@ -240,13 +234,12 @@ bool aligned16(std::initializer_list<const void*> all) {
   return x % 16 == 0;
 }
 
-// Workgroups of four waves for `rows` (token, head) rows: every row its own lanes up to eight rounds of a
-// full chip, a loop beyond.
+// Workgroups of four waves that give every (token, head) row its own lanes; 0 where the threads of the grid
+// would not count in 32 bits (2^24 workgroups, 64 GB of 16-bit rows).
 unsigned row_grid(int64_t n_tokens, int H_kv, int D) {
   const int64_t tpw = 64 / (D / 8);
-  const int64_t waves = (n_tokens + tpw - 1) / tpw * H_kv;
-  const int64_t groups = (waves + 3) / 4;
-  return unsigned(groups < (1 << 20) ? groups : (1 << 20));
+  const int64_t groups = ((n_tokens + tpw - 1) / tpw * H_kv + 3) / 4;
+  return groups < (1 << 24) ? unsigned(groups) : 0u;
 }
 
 template <typename F>
@@ -298,6 +291,10 @@ extern "C" int mi_kv_slot_write_fp4(const void* k, const void* v, const void* sl
   const int es = esize_of(dtype);
   bool vec = aligned16({k, v}) && st[2] == 1 && st[5] == 1;
   for (int i : {0, 1, 3, 4}) vec = vec && (st[i] * es) % 16 == 0;
+  const unsigned grid = row_grid(n_tokens, H_kv, D);
+  if (grid == 0) {
+    return fail(MI_ERR_UNSUPPORTED, "mi_kv_slot_write_fp4: %lld tokens in one call", (long long)n_tokens);
+  }
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     return by_dim(D, [&](auto d) {
@@ -305,7 +302,7 @@ extern "C" int mi_kv_slot_write_fp4(const void* k, const void* v, const void* sl
         return by_flag(vec, [&](auto is_vec) {
           using IdxT = std::conditional_t<decltype(narrow)::value, int32_t, int64_t>;
           hipLaunchKernelGGL((fp4_write_kernel<T, decltype(d)::value, IdxT, decltype(is_vec)::value>),
-                             dim3(row_grid(n_tokens, H_kv, D)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                             dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream),
                              static_cast<const T*>(k), static_cast<const T*>(v), static_cast<const IdxT*>(slot_ids),
                              pool, n_tokens, H_kv, st[0], st[1], st[2], st[3], st[4], st[5], error_word);
           return launch_status("mi_kv_slot_write_fp4");
@@ -331,12 +328,16 @@ extern "C" int mi_kv_slot_read_fp4(const void* k_pool, const void* v_pool, const
   if (!aligned16({k_pool, v_pool, k, v})) {
     return fail(MI_ERR_UNSUPPORTED, "mi_kv_slot_read_fp4: the pools and outputs must be 16-byte aligned");
   }
+  const unsigned grid = row_grid(n_tokens, H_kv, D);
+  if (grid == 0) {
+    return fail(MI_ERR_UNSUPPORTED, "mi_kv_slot_read_fp4: %lld tokens in one call", (long long)n_tokens);
+  }
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     return by_dim(D, [&](auto d) {
       return by_flag(slot_bits == 32, [&](auto narrow) {
         using IdxT = std::conditional_t<decltype(narrow)::value, int32_t, int64_t>;
-        hipLaunchKernelGGL((fp4_read_kernel<T, decltype(d)::value, IdxT>), dim3(row_grid(n_tokens, H_kv, D)), dim3(256),
+        hipLaunchKernelGGL((fp4_read_kernel<T, decltype(d)::value, IdxT>), dim3(grid), dim3(256),
                            0, static_cast<hipStream_t>(stream), pool, static_cast<const IdxT*>(slot_ids),
                            static_cast<T*>(k), static_cast<T*>(v), n_tokens, H_kv, error_word);
         return launch_status("mi_kv_slot_read_fp4");

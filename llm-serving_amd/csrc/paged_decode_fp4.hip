@@ -34,7 +34,7 @@ namespace miattn {
 namespace {
 
 struct Fp4DecodeArgs {
-  int B, H, H_kv, G, n_hchunks, bs_log2, max_blocks, target, slots;
+  int B, H, H_kv, G, n_hchunks, bs_log2, max_blocks, target, cols, cols_log2;
   int64_t qs0, qs1, ks0, ks1, vs0, vs1, os0, os1, bts0;
   float scale_log2;
 };
@@ -78,14 +78,29 @@ __device__ __forceinline__ float over_parts(float x) {
   return x;
 }
 
+// ceil(x / y) for quotients of at most a few hundred, exact: the product is off by less than one either way.
+__device__ __forceinline__ int ceil_div(int x, int y) {
+  const uint32_t v = uint32_t(x) + uint32_t(y) - 1u;
+  const int n = int(float(v) * __builtin_amdgcn_rcpf(float(y)));
+  const int r = int(v - uint32_t(n) * uint32_t(y));
+  return n + (r < 0 ? -1 : r >= y ? 1 : 0);
+}
+
 struct Fp4Split {
-  int b, split, n_split, first, chunk, len;
+  int b, split, n_split, first, len, begin, end;
 };
-// This workgroup's (row, split), derived by every wave from the row lengths, 64 rows at a time. Tokens per split:
-// total / target in whole rounds; as long as the splits of the first 64 rows (one per row at least, an
-// empty row's writes its zeros) are more than target the chunk grows, up to kFitSteps times.
+// This workgroup's (row, split) and its tokens, derived by every wave from the row lengths, 64 rows at a time. Tokens
+// per split: total / target in whole rounds; as long as the splits of the first 64 rows (one per row at least,
+// an empty row's writes its zeros) are more than target the chunk grows, up to kFitSteps times. A row's tokens
+// are then shared out evenly over its splits, again in whole rounds.
+// A merge of splits costs 2-3 us (a partial's way to memory, the count's there and back, the partials' way back), a round of
+// tiles 0.75 (D 256: about 2), so rows of up to kWhole tokens stay whole and no split is shorter than kLeast. Measured,
+// us per layer, H 16 / H_kv 8 / D 128: 4 rows of 600 whole 6.9, cut at 512 8.8; one of 1000 8.5 either way; one of 8000 with
+// kLeast 512 10.2, 768 10.7; D 256, 16 rows of 128-2048: kLeast 256 11.7, 512 14.2.
 constexpr int kFitSteps = 8;
-template <int kRound>
+template <int D> constexpr int kLeast = D == 256 ? 256 : 512;
+template <int D> constexpr int kWhole = D == 256 ? 512 : 1024;
+template <int kRound, int D>
 __device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, const Fp4DecodeArgs& a, int w,
                                            Fp4Split& si) {
   const int lane = __lane_id();
@@ -96,19 +111,22 @@ __device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, c
     const int row = r0 + lane;
     total += __builtin_amdgcn_readlane(wave_inclusive_scan(row < a.B ? clamp_len(seqlen[row], capacity) : 0), 63);
   }
-  const uint32_t even = (uint32_t(total) + uint32_t(a.target) - 1u) / uint32_t(a.target);
-  int chunk = int((even + kRound - 1) / kRound) * kRound;
-  chunk = chunk > kRound ? chunk : kRound;
+  // total / target rounded up to whole rounds: the share of one split
+  int chunk = (int((uint32_t(total) + uint32_t(a.target) * kRound - 1u) / (uint32_t(a.target) * kRound))) * kRound;
+  chunk = chunk > kLeast<D> ? chunk : kLeast<D>;
   auto count = [&](int len, int row) {
-    const int n = int((uint32_t(len) + uint32_t(chunk) - 1u) / uint32_t(chunk));
-    return row < a.B ? (n > 1 ? n : 1) : 0;
+    const int n = ceil_div(len, chunk);
+    return row < a.B ? (len > kWhole<D> ? n : 1) : 0;
   };
   int n = count(len_first, lane), incl = wave_inclusive_scan(n);
-  const int step = (chunk / 16 + kRound) / kRound * kRound;
-  for (int i = 0; i < kFitSteps && __builtin_amdgcn_readlane(incl, 63) > a.target; ++i) {
-    chunk += step;
-    n = count(len_first, lane);
-    incl = wave_inclusive_scan(n);
+  if (2 * a.B <= a.target) {
+    const int step = (chunk / 16 + kRound) / kRound * kRound;
+#pragma unroll 1
+    for (int i = 0; i < kFitSteps && __builtin_amdgcn_readlane(incl, 63) > a.target; ++i) {
+      chunk += step;
+      n = count(len_first, lane);
+      incl = wave_inclusive_scan(n);
+    }
   }
   int len = len_first, base = 0;
   for (int r0 = 0;;) {
@@ -116,13 +134,16 @@ __device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, c
     if (owner != 0) {
       const int o = __ffsll(static_cast<unsigned long long>(owner)) - 1;
       const int excl = __builtin_amdgcn_readlane(incl - n, o);
+      const int of_row = __builtin_amdgcn_readlane(n, o);
+      si.len = __builtin_amdgcn_readlane(len, o);
+      const int each = ((si.len + of_row - 1) / of_row + kRound - 1) & -kRound;
       si.b = r0 + o;
       si.split = w - base - excl;
-      si.n_split = __builtin_amdgcn_readlane(n, o);
       si.first = base + excl;
-      si.chunk = chunk;
-      si.len = __builtin_amdgcn_readlane(len, o);
-      return true;
+      si.n_split = si.len > 0 ? (si.len + each - 1) / each : 1;
+      si.begin = si.split * each;
+      si.end = min(si.len, si.begin + each);
+      return si.split < si.n_split;  // rounding up may leave the last split nothing
     }
     r0 += 64;
     if (r0 >= a.B) return false;
@@ -145,11 +166,8 @@ __device__ __forceinline__ auto partial_rsrc(float* p, int64_t floats) {
   return __builtin_amdgcn_make_buffer_rsrc(p, (short)0, int(floats * 4), 0x00020000);
 }
 
-#ifndef FP4_MINW
-#define FP4_MINW 1
-#endif
 template <typename T, int D, int kW>
-__global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
+__global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
     const T* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const int32_t* __restrict__ block_table, const int32_t* __restrict__ seqlen, T* __restrict__ out,
     int32_t* __restrict__ counters, float* __restrict__ partials, Fp4DecodeArgs a) {
@@ -162,43 +180,52 @@ __global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
   extern __shared__ __align__(16) float smem[];  // per wave: (m, l) of HB heads, then nh x D sums
 
   Fp4Split si;
-  if (!plan_split<kRound>(seqlen, a, blockIdx.x, si)) return;  // uniform
+  // Columns (KV head and chunk of its query heads) are the fast index, so the workgroups that have a split come first and
+  // are dealt out evenly over the CUs; those without one come last.
+  const int slot = a.cols_log2 >= 0 ? int(blockIdx.x) >> a.cols_log2 : int(blockIdx.x / unsigned(a.cols));
+  const int column = int(blockIdx.x) - slot * a.cols;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // The pages of this wave's first two tiles if no row before this one is split, loaded beside the row lengths: one memory
+  // round trip less for such batches, the short ones. Entries inside the table, used only if the plan says so.
+  int page0, pg[2], pn[2];
+  {
+    const int32_t* row = block_table + int64_t(min(slot, a.B - 1)) * a.bts0;
+    page0 = row[0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      pg[u] = row[min((wave * kTile + 16 * u) >> a.bs_log2, a.max_blocks - 1)];
+      pn[u] = row[min((wave * kTile + kRound + 16 * u) >> a.bs_log2, a.max_blocks - 1)];
+    }
+  }
+  if (!plan_split<kRound, D>(seqlen, a, slot, si)) return;  // uniform
   const int b = si.b;
-  const int t_begin = si.split * si.chunk;
-  const int t_end = min(si.len, t_begin + si.chunk);
-  const int kvh = blockIdx.y / a.n_hchunks;
-  const int hch = blockIdx.y - kvh * a.n_hchunks;
+  const int t_begin = si.begin, t_end = si.end;
+  const int kvh = a.n_hchunks == 1 ? column : column / a.n_hchunks;
+  const int hch = column - kvh * a.n_hchunks;
   const int nh = min(HB, a.G - hch * HB);  // query heads of this workgroup
   const int h0 = kvh * a.G + hch * HB;
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, lg = lane >> 4;  // of the products: row or column, and depth group
   const int part = col % NC;
   const int bs = 1 << a.bs_log2;
 
-  // Q as the depth x column operand: this lane's column, elements lg D / 4 + 8 kk + j. A negative scale
-  // is moved into q, so that the largest score is the largest product.
-  const float flip = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
-  const float c2 = a.scale_log2 * flip;
-  bf16x8_t qf[KW];
-  {
-    const bool there = col / NC < nh;
-    const T* src = q + b * a.qs0 + (h0 + (there ? col / NC : 0)) * a.qs1 + lg * (D / 4);
+  if (si.len == 0) {  // uniform: the row has no tokens, and its table may name no page
+    for (int i = threadIdx.x; i < nh * D; i += 64 * kW) out[b * a.os0 + (h0 + i / D) * a.os1 + i % D] = from_f32<T>(0.0f);
+    return;
+  }
+
+  // Q as the depth x column operand: column `col`, elements lg D / 4 + 8 kk + j of depth step kk. Each wave loads
+  // some of the KW steps here, and converts them into LDS once its first K and V loads are out.
+  constexpr int QW = (KW + kW - 1) / kW;      // steps per wave
+  constexpr int QN = sizeof(T) == 4 ? 2 : 1;  // 16-byte loads per 8 elements
+  const bool there = col / NC < nh;
+  uint4 q_raw[QW][QN];
 #pragma unroll
-    for (int kk = 0; kk < KW; ++kk) {
-      float x[8];
-      load8<T, true>(src + 8 * kk, 1, x);
+  for (int i = 0; i < QW; ++i) {
+    const int kk = min(wave + i * kW, KW - 1);
+    const T* src = q + b * a.qs0 + (h0 + (there ? col / NC : 0)) * a.qs1 + lg * (D / 4) + 8 * kk;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = there ? x[j] * flip : 0.0f;
-        if constexpr (!std::is_same<T, bf16_t>::value) {
-          // part i holds the bits left by the parts before it; past the last part nothing is left
-          for (int i = 0; i < NC - 1; ++i) x[j] = i < part ? x[j] - hi_bf16(x[j]) : x[j];
-          if (NC == 4 && part == 3) x[j] = 0.0f;
-        }
-      }
-      qf[kk] = operand(pack_hi(x[0], x[1]), pack_hi(x[2], x[3]), pack_hi(x[4], x[5]), pack_hi(x[6], x[7]));
-    }
+    for (int n = 0; n < QN; ++n) q_raw[i][n] = load16(src + 4 * n);
   }
 
   const int32_t* bt_row = block_table + b * a.bts0;
@@ -261,6 +288,46 @@ __global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
     __builtin_amdgcn_sched_barrier(0);
   };
 
+  int t0 = t_begin + wave * kTile;
+  if (si.b != slot || t_begin != 0) {
+    load_pages(t0, pg);
+    load_pages(t0 + kRound, pn);
+  } else {  // as load_pages gives them
+    auto settle = [&](int t, int (&x)[2]) {
+      x[0] = t < t_end ? x[0] : page0;
+      x[1] = t + 16 < t_end ? x[1] : x[0];
+    };
+    settle(t0, pg);
+    settle(t0 + kRound, pn);
+  }
+  issue_k(t0, pg);
+  issue_v(t0, pg);
+  // A negative scale is moved into q, so that the largest score is the largest product.
+  const float flip = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+  const float c2 = a.scale_log2 * flip;
+  uint4* sm_q = reinterpret_cast<uint4*>(smem + kW * (HB * 2 + min(HB, a.G) * D));  // [KW][64 lanes]
+#pragma unroll
+  for (int i = 0; i < QW; ++i) {
+    const int kk = wave + i * kW;
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = Vec16<T>::get(q_raw[i][j / Vec16<T>::N], j % Vec16<T>::N);
+      x[j] = there ? x[j] * flip : 0.0f;
+      if constexpr (!std::is_same<T, bf16_t>::value) {
+        // part i holds the bits left by the parts before it; past the last part nothing is left
+        for (int n = 0; n < NC - 1; ++n) x[j] = n < part ? x[j] - hi_bf16(x[j]) : x[j];
+        if (NC == 4 && part == 3) x[j] = 0.0f;
+      }
+    }
+    if (kk < KW) {
+      sm_q[kk * 64 + lane] =
+          make_uint4(pack_hi(x[0], x[1]), pack_hi(x[2], x[3]), pack_hi(x[4], x[5]), pack_hi(x[6], x[7]));
+    }
+  }
+  // a barrier that does not wait for the loads on their way
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
   f32x4_t o[VE];
 #pragma unroll
   for (int i = 0; i < VE; ++i) o[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -273,24 +340,33 @@ __global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
   auto compute = [&](int t0, auto masked, auto&& next_k, auto&& next_v) {
     constexpr bool kMasked = decltype(masked)::value;
     __builtin_amdgcn_sched_barrier(0);
+    uint4 qf[KW];
+#pragma unroll
+    for (int kk = 0; kk < KW; ++kk) qf[kk] = sm_q[kk * 64 + lane];
     f32x4_t s[2];
+    uint4 kf[2][KW];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int kk = 0; kk < KW; ++kk) {
+        const float sc = fp4_scale(tks[u][kk * 8 * KS / (D / 4)]);
+        const uint32_t w = tk[u][kk];
+        kf[u][kk] = make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0)),
+                               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1)),
+                               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2)),
+                               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3)));
+      }
+    }
+    next_k();
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       s[u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int kk = 0; kk < KW; ++kk) {
-        const float sc = fp4_scale(tks[u][kk * 8 * KS / (D / 4)]);
-        const uint32_t w = tk[u][kk];
-        const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0);
-        const auto p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1);
-        const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2);
-        const auto p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3);
-        const bf16x8_t kf = operand(__builtin_bit_cast(uint32_t, p0), __builtin_bit_cast(uint32_t, p1),
-                                    __builtin_bit_cast(uint32_t, p2), __builtin_bit_cast(uint32_t, p3));
-        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[kk], s[u], 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[u][kk]),
+                                                       __builtin_bit_cast(bf16x8_t, qf[kk]), s[u], 0, 0, 0);
       }
     }
-    next_k();
     // this lane's 8 tokens: t0 + 16 u + 4 lg + i
     float most = -INFINITY;
 #pragma unroll
@@ -331,75 +407,72 @@ __global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
       }
     }
     const bf16x8_t pf = operand(pack_hi(p[0], p[1]), pack_hi(p[2], p[3]), pack_hi(p[4], p[5]), pack_hi(p[6], p[7]));
+    if constexpr (kMasked) {
+      // past the end: zero codes, and scales of 1 (garbage may be a NaN scale, which 0 * NaN would keep)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int n = t_end - (t0 + 16 * u + 4 * lg);  // tokens of this lane's four that are there
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int k = 0; k < VW; ++k) tv[u][i][k] = i < n ? tv[u][i][k] : 0u;
+        }
+        const uint32_t keep = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+        tvs[u] = (tvs[u] & keep) | (0x7f7f7f7fu & ~keep);
+      }
+    }
     // the scale of token i of a half is byte i of its dword, shifted under the exponent (the conversion
     // reads no other bit of it)
     float vsc[8];
-    uint32_t vw[8][VW];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t w = tvs[u];
-        uint32_t x = i == 3 ? w >> 1 : w << (23 - 8 * i);
-        bool in = true;
-        if constexpr (kMasked) {  // garbage past the end may be a NaN scale, which 0 * NaN would keep
-          in = t0 + 16 * u + 4 * lg + i < t_end;
-          x = in ? x : 0x3f800000u;
-        }
-        vsc[4 * u + i] = __uint_as_float(x);
-#pragma unroll
-        for (int k = 0; k < VW; ++k) vw[4 * u + i][k] = in ? tv[u][i][k] : 0u;
-      }
+    for (int j = 0; j < 8; ++j) {
+      vsc[j] = __uint_as_float((j & 3) == 3 ? tvs[j >> 2] >> 1 : tvs[j >> 2] << (23 - 8 * (j & 3)));
     }
-    auto byte_of = [&](auto which, int k) {
-      constexpr int kByte = decltype(which)::value;
-      uint32_t x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[j][k], vsc[j], kByte));
-      }
-      uint32_t lo[4], hi[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        lo[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
-        hi[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
-      }
-      const int e = 8 * k + 2 * kByte;
-      o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(lo[0], lo[1], lo[2], lo[3]), pf, o[e], 0, 0, 0);
-      o[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(hi[0], hi[1], hi[2], hi[3]), pf, o[e + 1], 0, 0, 0);
-    };
+    // One dword of codes at a time: all its elements converted, then, the codes' registers being free, the next tile's
+    // loads, then the products.
+    constexpr int kBytes = VE >= 8 ? 4 : 2;
 #pragma unroll
     for (int k = 0; k < VW; ++k) {
-      byte_of(std::integral_constant<int, 0>{}, k);
-      byte_of(std::integral_constant<int, 1>{}, k);
-      if constexpr (VE >= 8) {
-        byte_of(std::integral_constant<int, 2>{}, k);
-        byte_of(std::integral_constant<int, 3>{}, k);
+      uint32_t x[4][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t w = tv[j >> 2][j & 3][k];
+        x[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vsc[j], 0));
+        x[1][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vsc[j], 1));
+        if constexpr (kBytes == 4) {
+          x[2][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vsc[j], 2));
+          x[3][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vsc[j], 3));
+        }
+      }
+      if (k == VW - 1) next_v();
+#pragma unroll
+      for (int y = 0; y < kBytes; ++y) {
+        uint32_t lo[4], hi[4];  // elements 2 y and 2 y + 1 of two tokens each
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          lo[j] = __builtin_amdgcn_perm(x[y][2 * j + 1], x[y][2 * j], 0x05040100u);
+          hi[j] = __builtin_amdgcn_perm(x[y][2 * j + 1], x[y][2 * j], 0x07060302u);
+        }
+        const int e = 8 * k + 2 * y;
+        o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(lo[0], lo[1], lo[2], lo[3]), pf, o[e], 0, 0, 0);
+        o[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(hi[0], hi[1], hi[2], hi[3]), pf, o[e + 1], 0, 0, 0);
       }
     }
-    next_v();
   };
 
   // Loads stay one tile ahead of their use: the next tile's K is on its way from when this tile's scores are made, its
   // V from when the sums are, and its pages are known a tile earlier. Every load of the loop is unconditional.
-  int t0 = t_begin + wave * kTile;
   if (t0 < t_end) {
     auto none = [] {};
-    int pg[2], pn[2];
-    load_pages(t0, pg);
-    load_pages(t0 + kRound, pn);
-    issue_k(t0, pg);
-    issue_v(t0, pg);
     for (; t0 + kRound < t_end; t0 += kRound) {  // a tile with another behind it is whole
       const int t1 = t0 + kRound;
       compute(t0, std::false_type{}, [&] { issue_k(t1, pn); pg[0] = pn[0]; pg[1] = pn[1]; load_pages(t1 + kRound, pn); },
               [&] { issue_v(t1, pg); });
     }
-    if (t0 + kTile <= t_end) compute(t0, std::false_type{}, none, none);
-    else compute(t0, std::true_type{}, none, none);
+    compute(t0, std::true_type{}, none, none);
   }
 
-  // ---- the waves' states through LDS: (m, l) per head, then the sums, parts added up
+  // ---- the waves' states through LDS (not q's part of it, which other waves may still read): (m, l) per head, then the sums, parts added up
   l = over_groups<SumOp>(l);
   float* sm_ml = smem;                  // [wave][HB][2]
   float* sm_o = smem + kW * HB * 2;     // [wave][nh][D]
@@ -422,7 +495,7 @@ __global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
   }
   __syncthreads();
   const int part_floats = partial_floats(min(HB, a.G), D);
-  const auto mine = partial_rsrc(partials + (int64_t(blockIdx.x) * gridDim.y + blockIdx.y) * part_floats, part_floats);
+  const auto mine = partial_rsrc(partials + int64_t(blockIdx.x) * part_floats, part_floats);
   for (int i = threadIdx.x; i < nh * (D / 4); i += 64 * kW) {
     const int gg = i / (D / 4), d = (i - gg * (D / 4)) * 4;
     float M = -INFINITY;
@@ -442,7 +515,7 @@ __global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
       acc.w = fmaf(x.w, wt, acc.w);
     }
     if (si.n_split == 1) {
-      const float inv = si.len > 0 ? 1.0f / L : 0.0f;
+      const float inv = 1.0f / L;
       const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
       T* row = out + b * a.os0 + (h0 + gg) * a.os1 + d;
 #pragma unroll
@@ -464,7 +537,7 @@ __global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
-    int* counter = counters + int64_t(b) * gridDim.y + blockIdx.y;
+    int* counter = counters + int64_t(b) * a.cols + column;
     const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     *sm_last = before == si.n_split - 1;
     if (before == si.n_split - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -472,8 +545,8 @@ __global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
   __syncthreads();
   if (!*sm_last) return;  // uniform
   __syncthreads();        // sm_last has been read by every wave; its words are used again below
-  const auto row_parts = partial_rsrc(partials + (int64_t(si.first) * gridDim.y + blockIdx.y) * part_floats,
-                                      (int64_t(si.n_split - 1) * gridDim.y + 1) * part_floats);
+  const auto row_parts = partial_rsrc(partials + (int64_t(si.first) * a.cols + column) * part_floats,
+                                      (int64_t(si.n_split - 1) * a.cols + 1) * part_floats);
   // NG groups of threads take the splits in turn, kFold at a time, and are folded through LDS
   const int lanes = nh * (D / 4);                       // threads that hold one split's sums, 4 each
   const int ng = max(1, 64 * kW / lanes);               // 64 kW threads, lanes a multiple of 16
@@ -493,8 +566,8 @@ __global__ __launch_bounds__(64 * kW, FP4_MINW) void paged_decode_fp4_kernel(
 #pragma unroll
       for (int j = 0; j < kFold; ++j) {
         const int s = min(s0 + j * ng, si.n_split - 1);
-        const int at = (s * int(gridDim.y) * part_floats + gg * D + d) * 4;
-        const int at_ml = (s * int(gridDim.y) * part_floats + nh * D + gg * 2) * 4;
+        const int at = (s * a.cols * part_floats + gg * D + d) * 4;
+        const int at_ml = (s * a.cols * part_floats + nh * D + gg * 2) * 4;
         ml[j] = __builtin_amdgcn_raw_buffer_load_b64(row_parts, at_ml, 0, kSc1);
         x[j] = __builtin_amdgcn_raw_buffer_load_b128(row_parts, at, 0, kSc1);
       }
@@ -556,15 +629,6 @@ bool fp4_dim(int D) { return D == 64 || D == 128 || D == 256; }
 
 bool fp4_block(int bs) { return bs >= 16 && (bs & (bs - 1)) == 0; }
 
-#ifndef FP4_GROUPS8
-#define FP4_GROUPS8 256
-#endif
-#ifndef FP4_GROUPS4
-#define FP4_GROUPS4 512
-#endif
-#ifndef FP4_LIMIT8
-#define FP4_LIMIT8 256
-#endif
 struct Fp4Plan {
   int n_hchunks, cols, waves, target, slots, nh;
   size_t counter_bytes, partial_bytes;
@@ -577,8 +641,12 @@ Fp4Plan make_plan(int B, int H, int H_kv, int D, int dtype) {
   p.n_hchunks = (H / H_kv + heads - 1) / heads;
   p.cols = H_kv * p.n_hchunks;
   p.nh = H / H_kv < heads ? H / H_kv : heads;
-  p.waves = int64_t(B) * p.cols <= FP4_LIMIT8 ? 8 : 4;
-  const int groups = p.waves == 8 ? FP4_GROUPS8 : FP4_GROUPS4;
+  // One workgroup of 8 waves per CU, or two of 4: the latter where the rows times columns are more than half the
+  // CUs and at most all of them, too few splits per row for 256 workgroups to be dealt out evenly. us per layer, 8 and 4
+  // waves: 32 ragged rows (256 in all) 16.1 and 14.0, 16 of 4000-8000 (128) 27.3 and 25.9, 32 of 500 8.1 and 8.7, 32 of 8192 51.9
+  // and 53.6; outside, 8 of 512 (64) 7.1 and 7.6, 64 ragged rows (512) 21.5 and 22.4, one of 8000 10.2 and 10.3.
+  p.waves = int64_t(B) * p.cols > 128 && int64_t(B) * p.cols <= 256 ? 4 : 8;
+  const int groups = p.waves == 8 ? 256 : 512;
   p.target = groups / p.cols > 1 ? groups / p.cols : 1;
   p.slots = p.target + B;
   p.counter_bytes = (size_t(B) * p.cols * sizeof(int32_t) + 255) / 256 * 256;
@@ -595,8 +663,8 @@ int launch_d(const void* q, const void* k, const void* v, const int32_t* bt, con
     constexpr int kW = decltype(waves)::value;
     // the waves' states; the fold of the splits needs 6 floats per thread at most
     const size_t states = size_t(kW) * (kHeads<T> * 2 + p.nh * D), fold = size_t(64 * kW) * 6;
-    const size_t lds = (states > fold ? states : fold) * sizeof(float);
-    hipLaunchKernelGGL((paged_decode_fp4_kernel<T, D, kW>), dim3(p.slots, p.cols), dim3(64 * kW), lds, s,
+    const size_t lds = (states + D * 8 > fold ? states + D * 8 : fold) * sizeof(float);  // 32 D bytes of q
+    hipLaunchKernelGGL((paged_decode_fp4_kernel<T, D, kW>), dim3(unsigned(p.slots) * unsigned(p.cols)), dim3(64 * kW), lds, s,
                        static_cast<const T*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), bt, seqlen,
                        static_cast<T*>(out), counters, partials, a);
   };
@@ -654,7 +722,7 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
     return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: B * max_blocks * block_size must stay below 2^31 tokens");
   }
   const Fp4Plan p = make_plan(B, H, H_kv, D, dtype);
-  if (B > 65535 || H > 65535 || p.cols > 65535) {
+  if (int64_t(p.slots) * p.cols > 0x7fffffff / (64 * 8)) {  // threads of the grid in 32 bits
     return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: grid too large (B=%d, H=%d)", B, H);
   }
   const int64_t* st = strides;
@@ -673,7 +741,8 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
     return fail(MI_ERR_WORKSPACE, "mi_paged_decode_fp4: workspace must be 16-byte aligned");
   }
   Fp4DecodeArgs a;
-  a.n_hchunks = p.n_hchunks; a.target = p.target; a.slots = p.slots;
+  a.n_hchunks = p.n_hchunks; a.target = p.target; a.cols = p.cols;
+  a.cols_log2 = (p.cols & (p.cols - 1)) == 0 ? __builtin_ctz(unsigned(p.cols)) : -1;
   a.B = B; a.H = H; a.H_kv = H_kv; a.G = H / H_kv; a.max_blocks = max_blocks;
   a.bs_log2 = __builtin_ctz(unsigned(block_size));
   a.qs0 = st[0]; a.qs1 = st[1]; a.ks0 = st[2]; a.ks1 = st[3]; a.vs0 = st[4]; a.vs1 = st[5];

@@ -689,3 +689,24 @@ def test_server_runs_a_trace_on_a_4_bit_pool(cuda):
     assert all(len(r.tokens) == 6 for r in records) and server.blocks.n_free == 64
     with pytest.raises(ValueError, match="kv_bits must be 4 or 16"):
         ContinuousServer(model, n_blocks=8, kv_bits=8)
+
+
+def test_decode_of_lengths_past_24_bits(cuda):
+    """Rows of more than 2^24 tokens, where fp32 no longer counts tokens one by one: a mean (scale 0) over one and
+    over two such rows, with all weight of V on a few tokens at the rows' ends and at odd places."""
+    D, bs, n = 64, 512, (1 << 24) + 1_234_567
+    pool = Fp4PagedPool(1, -(-n // bs), bs, 1, D, dtype=torch.float32, device=cuda)
+    table = torch.arange(pool.n_blocks, dtype=torch.int32, device=cuda).flip(0).repeat(2, 1).contiguous()
+    lengths = [n, n - (1 << 23) + 17]
+    marks = sorted({0, 5, 777_777, 1 << 24, *(m - i for m in lengths for i in (1, 2, 300))})
+    slots = torch.tensor([int(table[0, t // bs]) * bs + t % bs for t in marks], device=cuda)
+    rows = torch.full((len(marks), 1, D), 4.0, device=cuda)
+    pool.write_slots(0, slots, torch.zeros_like(rows), rows)
+    for count in (1, 2):
+        seqlen = torch.tensor(lengths[:count], dtype=torch.int32, device=cuda)
+        out = paged_decode_fp4(torch.randn(count, 2, D, device=cuda), pool.keys[0], pool.values[0], table[:count], seqlen,
+                               scale=0.0)
+        for r in range(count):
+            want = 4.0 * sum(t < lengths[r] for t in marks) / lengths[r]
+            # fp32 sums of n ones over some hundred waves, a few thousand each: well inside 2^-18
+            assert (out[r].double() / want - 1).abs().max() <= 2.0 ** -18
