@@ -119,16 +119,37 @@ def test_write_slots_stores_the_oracles_bytes_and_read_slots_returns_them(dtype,
     pool.check_writes()
 
 
-@pytest.mark.parametrize("n", [0, 1, 2, 65])
-def test_write_of_few_and_no_tokens(n, cuda):
-    pool = Fp4PagedPool(1, 8, 16, 2, 128, dtype=torch.bfloat16, device=cuda)
+@pytest.mark.parametrize("n", [0, 1, 2, 65, 8191, 8197])
+def test_write_of_no_few_and_many_tokens(n, cuda):
+    pool = Fp4PagedPool(1, max(8, n // 8), 16, 2, 128, dtype=torch.bfloat16, device=cuda)
     k, v = torch.randn(n, 2, 128).bfloat16(), torch.randn(n, 2, 128).bfloat16()
     slots = torch.randperm(pool.n_slots)[:n]
     pool.write_slots(0, slots.cuda(), k.cuda(), v.cuda())
     got_k, got_v = pool.read_slots(0, slots.cuda())
     assert got_k.shape == k.shape
-    if n:
+    pool.check_writes()
+    if 0 < n < 100:
         assert torch.equal(got_k.cpu().double(), oracle.held(k)) and torch.equal(got_v.cpu().double(), oracle.held(v))
+
+
+def test_many_tokens_are_stored_as_the_same_tokens_one_call_at_a_time(cuda):
+    """Large calls work on two rows per lane: the same bytes as small ones, a bad slot among them skipped."""
+    n, H_kv, D = 9001, 3, 128
+    k, v = torch.randn(n, H_kv, D).half().cuda(), torch.randn(n, H_kv, D).half().cuda()
+    pools = [Fp4PagedPool(1, 600, 16, H_kv, D, dtype=torch.float16, device=cuda) for _ in range(2)]
+    slots = torch.randperm(9600, generator=torch.Generator().manual_seed(0))[:n].cuda()
+    slots[4321] = 9600
+    pools[0].write_slots(0, slots, k, v)
+    with pytest.raises(IndexError, match="token 4321 of"):
+        pools[0].check_writes()
+    for a in range(0, n, 500):
+        pools[1].write_slots(0, slots[a: a + 500], k[a: a + 500], v[a: a + 500])
+    assert torch.equal(pools[0].keys[0], pools[1].keys[0]) and torch.equal(pools[0].values[0], pools[1].values[0])
+    whole = pools[0].read_slots(0, slots)
+    for a in range(0, n, 500):
+        part = pools[0].read_slots(0, slots[a: a + 500])
+        assert all(torch.equal(x[a: a + 500], y) for x, y in zip(whole, part))
+    assert not whole[0][4321].any() and whole[0][4320].any()
 
 
 def test_out_of_range_slots_are_skipped_and_reported(cuda):
