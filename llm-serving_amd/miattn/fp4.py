@@ -33,7 +33,7 @@ from types import SimpleNamespace
 import torch
 
 from . import _lib
-from ._contract import Rule, enforce, is_pow2, same_device
+from ._contract import Rule, enforce, is_pow2
 from .decode import _INDEXING, _PLAN_INPUTS, _SEQLEN_WATCH, DecodeGeometry, _require_backend, _require_device_tensors
 from .paged import PagedPool
 
@@ -44,6 +44,7 @@ GROUP = 32
 _HEAD_DIMS = (64, 128, 256)
 _MIN_BLOCK = 16
 _ELEMENT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
+_SLOT_TYPES = (torch.int32, torch.int64)
 
 
 def page_bytes(block_size: int, head_dim: int) -> int:
@@ -65,10 +66,10 @@ _POOL = (
 _READ_SLOTS = (
     Rule(lambda a: a.slots.dim() != 1, ValueError,
          lambda a: f"slot_ids must be 1-D, got {tuple(a.slots.shape)}"),
-    Rule(lambda a: a.slots.dtype not in (torch.int32, torch.int64), ValueError,
+    Rule(lambda a: a.slots.dtype not in _SLOT_TYPES, ValueError,
          lambda a: f"slot_ids must be an integer tensor (int32 or int64), got {a.slots.dtype}"),
-    Rule(lambda a: not same_device(a.slots.device, a.pool.device), ValueError,
-         lambda a: f"slot_ids are on {a.slots.device} but the pool is on {a.pool.device}"),
+    Rule(lambda a: a.slots.device != a.pool._home, ValueError,
+         lambda a: f"slot_ids are on {a.slots.device} but the pool is on {a.pool._home}"),
 )
 
 
@@ -84,19 +85,39 @@ class Fp4PagedPool(PagedPool):
         shape = (self.n_blocks, self.n_kv_head, page_bytes(self.block_size, self.head_dim))
         return torch.zeros(shape, dtype=torch.uint8, device=self.device)
 
+    def __init__(self, *args, **kw) -> None:
+        super().__init__(*args, **kw)
+        self._home = self._write_error.device  # with its index
+        self._row = torch.Size((self.n_kv_head, self.head_dim))
+        self._sizes = (self.n_kv_head, self.head_dim, self.n_blocks, self.block_size)
+        row = self.n_kv_head * self.head_dim
+        self._dense = _lib.int64_array((row, self.head_dim, 1) * 2)  # strides of contiguous k and v
+        self._code = _lib.dtype_code(self.dtype)
+
+    def write_slots(self, layer: int, slot_ids: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+        """``pool_flat[slot_ids[i]] = k[i]`` and the same for ``v``, rounded to 4 bits (``PagedPool.write_slots``)."""
+        shape, dtype, home = k.shape, self.dtype, self._home
+        if (len(shape) != 3 or shape[1:] != self._row or v.shape != shape or slot_ids.shape != shape[:1]
+                or k.dtype != dtype or v.dtype != dtype or slot_ids.dtype not in _SLOT_TYPES
+                or k.device != home or v.device != home or slot_ids.device != home):
+            super().write_slots(layer, slot_ids, k, v)  # raises what is wrong, or converts k and v
+            return
+        self._scatter_hip(self._layer(layer), slot_ids, k, v)
+
     def _scatter_hip(self, layer: int, slot_ids, k, v) -> None:
-        if not (same_device(k.device, self.device) and same_device(v.device, self.device)):
-            raise RuntimeError(f"the pool is on {self.device} and takes k/v there; got {k.device}/{v.device}")
-        n = int(k.shape[0])
+        if k.device != self._home or v.device != self._home:
+            raise RuntimeError(f"the pool is on {self._home} and takes k/v there; got {k.device}/{v.device}")
+        n = k.shape[0]
         if n == 0:
             return
         slot_ids = slot_ids.contiguous()
-        with _lib.on_device(k.device):
+        strides = self._dense if k.is_contiguous() and v.is_contiguous() else \
+            _lib.int64_array((*k.stride(), *v.stride()))
+        with _lib.on_device(self._home):
             rc = _lib.lib.mi_kv_slot_write_fp4(
                 k.data_ptr(), v.data_ptr(), slot_ids.data_ptr(), 8 * slot_ids.element_size(),
-                self.keys[layer].data_ptr(), self.values[layer].data_ptr(), n, self.n_kv_head, self.head_dim,
-                self.n_blocks, self.block_size, _lib.int64_array((*k.stride(), *v.stride())),
-                _lib.dtype_code(self.dtype), self._write_error.data_ptr(), _lib.current_stream(k.device))
+                self.keys[layer].data_ptr(), self.values[layer].data_ptr(), n, *self._sizes, strides, self._code,
+                self._write_error.data_ptr(), _lib.current_stream(self._home))
         _lib.check(rc, "Fp4PagedPool.write_slots")
         if self.strict_writes:
             self.check_writes()
@@ -106,20 +127,19 @@ class Fp4PagedPool(PagedPool):
         head_dim)`` in the pool's dtype (exact in bf16 and fp32; in fp16 rounded, past its largest value that).
         A slot outside the pool reads as zeros and is reported by :meth:`check_writes`."""
         layer = self._layer(layer)
-        enforce(_READ_SLOTS, SimpleNamespace(pool=self, slots=slot_ids))
-        n = int(slot_ids.numel())
-        shape = (n, self.n_kv_head, self.head_dim)
-        k = torch.empty(shape, dtype=self.dtype, device=slot_ids.device)
+        if slot_ids.dim() != 1 or slot_ids.dtype not in _SLOT_TYPES or slot_ids.device != self._home:
+            enforce(_READ_SLOTS, SimpleNamespace(pool=self, slots=slot_ids))
+        n = slot_ids.shape[0]
+        k = torch.empty((n, *self._row), dtype=self.dtype, device=self._home)
         v = torch.empty_like(k)
         if n == 0:
             return k, v
         slot_ids = slot_ids.contiguous()
-        with _lib.on_device(slot_ids.device):
+        with _lib.on_device(self._home):
             rc = _lib.lib.mi_kv_slot_read_fp4(
                 self.keys[layer].data_ptr(), self.values[layer].data_ptr(), slot_ids.data_ptr(),
-                8 * slot_ids.element_size(), k.data_ptr(), v.data_ptr(), n, self.n_kv_head, self.head_dim,
-                self.n_blocks, self.block_size, _lib.dtype_code(self.dtype), self._write_error.data_ptr(),
-                _lib.current_stream(slot_ids.device))
+                8 * slot_ids.element_size(), k.data_ptr(), v.data_ptr(), n, *self._sizes, self._code,
+                self._write_error.data_ptr(), _lib.current_stream(self._home))
         _lib.check(rc, "Fp4PagedPool.read_slots")
         if self.strict_writes:
             self.check_writes()
@@ -129,16 +149,16 @@ class Fp4PagedPool(PagedPool):
                          q, k_out, v_out, eps, zero_centred_norm) -> int:
         B, H, D = q.shape
         tensors = (source, q_norm_w, k_norm_w, cos, sin, pos, slot_ids, *(t for t in (k_out, v_out) if t is not None))
-        if not all(same_device(t.device, self.device) for t in tensors):
-            raise RuntimeError(f"the pool is on {self.device} and takes every tensor of the epilogue there")
-        with _lib.on_device(source.device):
+        if any(t.device != self._home for t in tensors):
+            raise RuntimeError(f"the pool is on {self._home} and takes every tensor of the epilogue there")
+        with _lib.on_device(self._home):
             return _lib.lib.mi_qk_norm_rope_write_fp4(
                 source.data_ptr(), row_stride, n_parts, q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(),
                 sin.data_ptr(), cos.shape[0], rotary, pos.data_ptr(), slot_ids.data_ptr(),
                 8 * slot_ids.element_size(), q.data_ptr(), self.keys[layer].data_ptr(), self.values[layer].data_ptr(),
                 None if k_out is None else k_out.data_ptr(), None if v_out is None else v_out.data_ptr(),
-                B, H, self.n_kv_head, D, self.n_blocks, self.block_size, float(eps), int(bool(zero_centred_norm)),
-                _lib.dtype_code(self.dtype), self._write_error.data_ptr(), _lib.current_stream(source.device))
+                B, H, *self._sizes, float(eps), int(bool(zero_centred_norm)), self._code, self._write_error.data_ptr(),
+                _lib.current_stream(self._home))
 
     def decode_plan(self, q, block_table, seqlen, *, scale=None) -> "Fp4DecodePlan":
         return paged_decode_fp4_plan(q, self.keys, self.values, block_table, seqlen, scale=scale)
@@ -238,7 +258,7 @@ class Fp4DecodePlan:
     reference, ``seqlen`` updates in place seen; one workspace, so its runs stay ordered on one stream)."""
 
     __slots__ = ("n_layer", "geometry", "q_signature", "_k_ptrs", "_v_ptrs", "_pools", "_table", "_seqlen", "_ws",
-                 "_strides", "_frozen")
+                 "_strides", "_frozen", "_shape", "_stride", "_dtype", "_device")
 
     def __init__(self, q, k_caches, v_caches, block_table, seqlen, *, scale=None) -> None:
         _require_backend()
@@ -256,6 +276,7 @@ class Fp4DecodePlan:
         self.n_layer = len(ks)
         self.geometry = g
         self.q_signature = (tuple(q.shape), q.dtype, q.device, q.stride())
+        self._shape, self._stride, self._dtype, self._device = q.shape, q.stride(), q.dtype, q.device
         self._pools = (ks, vs)  # keeps the pool tensors alive
         self._k_ptrs = [k.data_ptr() for k in ks]
         self._v_ptrs = [v.data_ptr() for v in vs]
@@ -271,18 +292,17 @@ class Fp4DecodePlan:
         layer = int(layer)
         if not 0 <= layer < self.n_layer:
             raise IndexError(f"layer {layer} is outside the plan's {self.n_layer} layers")
-        signature = (tuple(q.shape), q.dtype, q.device, q.stride())
-        if signature != self.q_signature:
+        if q.shape != self._shape or q.dtype != self._dtype or q.device != self._device or q.stride() != self._stride:
             raise ValueError(
-                "paged_decode_fp4_plan.run: the query does not match the validated layout "
-                f"(built for shape/dtype/device/strides {self.q_signature}, got {signature}); "
-                "build a new plan for a new layout"
+                "paged_decode_fp4_plan.run: the query does not match the validated layout (built for "
+                f"shape/dtype/device/strides {self.q_signature}, got "
+                f"{(tuple(q.shape), q.dtype, q.device, q.stride())}); build a new plan for a new layout"
             )
-        with _lib.on_device(q.device):
+        with _lib.on_device(self._device):
             out = torch.empty_like(q)
             rc = _lib.lib.mi_paged_decode_fp4(
                 q.data_ptr(), self._k_ptrs[layer], self._v_ptrs[layer], self._table.data_ptr(),
-                self._seqlen.data_ptr(), out.data_ptr(), *self._frozen, _lib.current_stream(q.device))
+                self._seqlen.data_ptr(), out.data_ptr(), *self._frozen, _lib.current_stream(self._device))
         _lib.check(rc, "paged_decode_fp4_plan.run")
         return out
 

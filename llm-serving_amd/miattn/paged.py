@@ -317,9 +317,10 @@ class PagedPool:
         if len(src) != len(dst):
             raise ValueError(f"copy_blocks needs one destination per source, got {len(src)} / {len(dst)}")
         self._check_block_ids(src + dst, 0)
-        if len(set(dst)) != len(dst):
+        targets = set(dst)
+        if len(targets) != len(dst):
             raise ValueError("copy_blocks: a destination block is named twice")
-        both = set(src) & set(dst)
+        both = targets.intersection(src)
         if both:
             raise ValueError(f"copy_blocks: block {min(both)} is both a source and a destination")
         if not src:
@@ -332,7 +333,7 @@ class PagedPool:
             return
         _lib.require_library("PagedPool.copy_blocks on a HIP pool")
         pools = (ctypes.c_void_p * len(stores))(*[t.data_ptr() for t in stores])
-        page = stores[0][0].numel() * stores[0].element_size()
+        page = stores[0].stride(0) * stores[0].element_size()
         with _lib.on_device(self.keys[0].device):
             rc = _lib.lib.mi_copy_pages(pools, len(stores), page, self.n_blocks, (ctypes.c_int32 * len(src))(*src),
                                         (ctypes.c_int32 * len(dst))(*dst), len(src),
