@@ -305,7 +305,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
   // A negative scale is moved into q, so that the largest score is the largest product.
   const float flip = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
   const float c2 = a.scale_log2 * flip;
-  uint4* sm_q = reinterpret_cast<uint4*>(smem + kW * (HB * 2 + min(HB, a.G) * D));  // [KW][64 lanes]
+  uint4* sm_q = reinterpret_cast<uint4*>(smem + kW * (HB * 2 + min(HB, a.G) * (D + 16)));  // [KW][64 lanes]
 #pragma unroll
   for (int i = 0; i < QW; ++i) {
     const int kk = wave + i * kW;
@@ -472,10 +472,15 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
     compute(t0, std::true_type{}, none, none);
   }
 
-  // ---- the waves' states through LDS (not q's part of it, which other waves may still read): (m, l) per head, then the sums, parts added up
+  // ---- the waves' states through LDS (not q's part of it, which other waves may still read): (m, l) per head, then the
+  // sums, parts added up, four elements at a time. Piece x of a head is rows 4 lg + r of the products, elements
+  // 4 n .. 4 n + 3 of each, x = (r VE / 4 + n) 4 + lg: the lane groups of a column and, heads being 16 words apart
+  // modulo the banks, its heads write side by side.
   l = over_groups<SumOp>(l);
-  float* sm_ml = smem;                  // [wave][HB][2]
-  float* sm_o = smem + kW * HB * 2;     // [wave][nh][D]
+  constexpr int kHeadWords = D + 16;
+  auto element_of = [](int x) { return (4 * (x & 3) + (x >> 2) / (VE / 4)) * VE + (x >> 2) % (VE / 4) * 4; };
+  float* sm_ml = smem;                // [wave][HB][2]
+  float* sm_o = smem + kW * HB * 2;   // [wave][nh][kHeadWords]
   const int g = col / NC;
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
@@ -484,48 +489,61 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
   }
   if (part == 0 && g < nh) {
     if (lg == 0) *reinterpret_cast<float2*>(sm_ml + (wave * HB + g) * 2) = make_float2(m, l);
+    float* dst = sm_o + (wave * nh + g) * kHeadWords + lg * 4;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {  // rows 4 lg + r of the products: VE consecutive elements of D
-      float* dst = sm_o + (wave * nh + g) * D + (4 * lg + r) * VE;
+    for (int r = 0; r < 4; ++r) {
 #pragma unroll
       for (int i = 0; i < VE; i += 4) {
-        *reinterpret_cast<float4*>(dst + i) = make_float4(o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]);
+        *reinterpret_cast<float4*>(dst + (r * (VE / 4) + i / 4) * 16) = make_float4(o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]);
       }
     }
   }
   __syncthreads();
+  auto finish = [&](int gg, int x, const float4& acc, float L) {
+    const float inv = 1.0f / L;
+    const float y[4] = {fp4_saturate<T>(acc.x * inv), fp4_saturate<T>(acc.y * inv), fp4_saturate<T>(acc.z * inv),
+                        fp4_saturate<T>(acc.w * inv)};
+    T* row = out + b * a.os0 + (h0 + gg) * a.os1 + element_of(x);
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(row) = make_float4(y[0], y[1], y[2], y[3]);
+    } else {
+      const uint32_t w0 = uint32_t(from_f32<T>(y[0]).bits) | uint32_t(from_f32<T>(y[1]).bits) << 16;
+      const uint32_t w1 = uint32_t(from_f32<T>(y[2]).bits) | uint32_t(from_f32<T>(y[3]).bits) << 16;
+      *reinterpret_cast<uint2*>(row) = make_uint2(w0, w1);
+    }
+  };
   const int part_floats = partial_floats(min(HB, a.G), D);
   const auto mine = partial_rsrc(partials + int64_t(blockIdx.x) * part_floats, part_floats);
   for (int i = threadIdx.x; i < nh * (D / 4); i += 64 * kW) {
-    const int gg = i / (D / 4), d = (i - gg * (D / 4)) * 4;
+    const int gg = i / (D / 4), x = i - gg * (D / 4);
+    float2 ml[kW];
+    float4 v[kW];
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kW; ++w) M = fmaxf(M, sm_ml[(w * HB + gg) * 2]);
+    for (int w = 0; w < kW; ++w) {
+      ml[w] = *reinterpret_cast<const float2*>(sm_ml + (w * HB + gg) * 2);
+      v[w] = *reinterpret_cast<const float4*>(sm_o + (w * nh + gg) * kHeadWords + x * 4);
+      M = fmaxf(M, ml[w].x);
+    }
     float L = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kW; ++w) {
-      const float2 ml = *reinterpret_cast<const float2*>(sm_ml + (w * HB + gg) * 2);
-      const float wt = ml.x == -INFINITY ? 0.0f : fast_exp2((ml.x - M) * c2);
-      const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * nh + gg) * D + d);
-      L = fmaf(ml.y, wt, L);
-      acc.x = fmaf(x.x, wt, acc.x);
-      acc.y = fmaf(x.y, wt, acc.y);
-      acc.z = fmaf(x.z, wt, acc.z);
-      acc.w = fmaf(x.w, wt, acc.w);
+      const float wt = ml[w].x == -INFINITY ? 0.0f : fast_exp2((ml[w].x - M) * c2);
+      L = fmaf(ml[w].y, wt, L);
+      acc.x = fmaf(v[w].x, wt, acc.x);
+      acc.y = fmaf(v[w].y, wt, acc.y);
+      acc.z = fmaf(v[w].z, wt, acc.z);
+      acc.w = fmaf(v[w].w, wt, acc.w);
     }
     if (si.n_split == 1) {
-      const float inv = 1.0f / L;
-      const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-      T* row = out + b * a.os0 + (h0 + gg) * a.os1 + d;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) row[j] = from_f32<T>(fp4_saturate<T>(y[j]));
+      finish(gg, x, acc, L);
     } else {
       const u32x4_nt val = {__float_as_uint(acc.x), __float_as_uint(acc.y), __float_as_uint(acc.z), __float_as_uint(acc.w)};
-      __builtin_amdgcn_raw_buffer_store_b128(val, mine, (gg * D + d) * 4, 0, kSc1);
-      if (d == 0) {
-        const u32x2_t ml = {__float_as_uint(M == -INFINITY ? M : M * c2), __float_as_uint(L)};
-        __builtin_amdgcn_raw_buffer_store_b64(ml, mine, (nh * D + gg * 2) * 4, 0, kSc1);
+      __builtin_amdgcn_raw_buffer_store_b128(val, mine, (gg * D + x * 4) * 4, 0, kSc1);
+      if (x == 0) {
+        const u32x2_t mine_ml = {__float_as_uint(M == -INFINITY ? M : M * c2), __float_as_uint(L)};
+        __builtin_amdgcn_raw_buffer_store_b64(mine_ml, mine, (nh * D + gg * 2) * 4, 0, kSc1);
       }
     }
   }
@@ -557,7 +575,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
     const int grp = ng > 1 ? threadIdx.x / lanes : 0;
     const int i = ng > 1 ? threadIdx.x - grp * lanes : i0 + threadIdx.x;
     const bool mine_too = grp < ng && i < lanes;
-    const int gg = mine_too ? i / (D / 4) : 0, d = mine_too ? (i - gg * (D / 4)) * 4 : 0;
+    const int gg = mine_too ? i / (D / 4) : 0, x0 = mine_too ? i - gg * (D / 4) : 0;
     float M = -INFINITY, L = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int s0 = grp; s0 < si.n_split; s0 += kFold * ng) {
@@ -566,7 +584,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
 #pragma unroll
       for (int j = 0; j < kFold; ++j) {
         const int s = min(s0 + j * ng, si.n_split - 1);
-        const int at = (s * a.cols * part_floats + gg * D + d) * 4;
+        const int at = (s * a.cols * part_floats + gg * D + x0 * 4) * 4;
         const int at_ml = (s * a.cols * part_floats + nh * D + gg * 2) * 4;
         ml[j] = __builtin_amdgcn_raw_buffer_load_b64(row_parts, at_ml, 0, kSc1);
         x[j] = __builtin_amdgcn_raw_buffer_load_b128(row_parts, at, 0, kSc1);
@@ -613,13 +631,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
         acc.w = acc.w * w0 + x.w * w1;
       }
     }
-    if (mine_too) {
-      const float inv = 1.0f / L;
-      const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-      T* row = out + b * a.os0 + (h0 + gg) * a.os1 + d;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) row[j] = from_f32<T>(fp4_saturate<T>(y[j]));
-    }
+    if (mine_too) finish(gg, x0, acc, L);
   }
 }
 
@@ -662,7 +674,7 @@ int launch_d(const void* q, const void* k, const void* v, const int32_t* bt, con
   auto go = [&](auto waves) {
     constexpr int kW = decltype(waves)::value;
     // the waves' states; the fold of the splits needs 6 floats per thread at most
-    const size_t states = size_t(kW) * (kHeads<T> * 2 + p.nh * D), fold = size_t(64 * kW) * 6;
+    const size_t states = size_t(kW) * (kHeads<T> * 2 + p.nh * (D + 16)), fold = size_t(64 * kW) * 6;
     const size_t lds = (states + D * 8 > fold ? states + D * 8 : fold) * sizeof(float);  // 32 D bytes of q
     hipLaunchKernelGGL((paged_decode_fp4_kernel<T, D, kW>), dim3(unsigned(p.slots) * unsigned(p.cols)), dim3(64 * kW), lds, s,
                        static_cast<const T*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), bt, seqlen,
