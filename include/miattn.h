@@ -354,7 +354,8 @@ int mi_prefill_wait_limit(int polls);
  * mi_qk_norm_rope_write_fp4: mi_qk_norm_rope_write over such a pool, with the same arguments (n_blocks and block_size
  *   in place of n_slots) and the same idle and refused rows. The norm and the rotation are fp32 and
  *   rounded to `dtype` once (mi_qk_norm_rope_write rounds after every op); the pool holds the 4-bit form of
- *   the rounded k (what mi_kv_slot_write_fp4 of k_out would store). q_out, k_out and v_out 16-byte aligned. */
+ *   the rounded k (what mi_kv_slot_write_fp4 of k_out would store). q_out, k_out and v_out 16-byte aligned.
+ *   B = 0 does nothing. */
 int64_t mi_fp4_page_bytes(int block_size, int D);
 int mi_kv_slot_write_fp4(const void* k, const void* v, const void* slot_ids, int slot_bits, void* k_pool,
                          void* v_pool, int64_t n_tokens, int H_kv, int D, int64_t n_blocks, int block_size,
@@ -372,8 +373,11 @@ int mi_qk_norm_rope_write_fp4(const void* qkv, int64_t row_stride, int qkv_parts
  * (clamped to [0, max_blocks * block_size]; zeros for none), fp32 sums, rounded to `dtype` once.
  * strides = {q_s0, q_s1, k_s0, k_s1, v_s0, v_s1, o_s0, o_s1, bt_s0}: q and out (B, H, D) in elements with D
  * contiguous, the pools' block and head strides in bytes, the table's row stride; every row, head and page
- * 16-byte aligned. B * max_blocks * block_size below 2^31. Block ids are trusted. Workspace:
- * mi_paged_decode_fp4_workspace_size() bytes, 16-byte aligned; calls that share one must be ordered. */
+ * 16-byte aligned. B * max_blocks * block_size within 2^30. Block ids are trusted. One launch; a row cut into
+ * splits is folded by the last of its workgroups to finish, in the splits' order (the result does not depend
+ * on who was last). Workspace: mi_paged_decode_fp4_workspace_size() bytes, 16-byte aligned, zeroed once before its
+ * first call (it starts with those workgroups' counters, which every call leaves zero); calls that share one
+ * must be ordered. */
 size_t mi_paged_decode_fp4_workspace_size(int B, int H, int H_kv, int D, int block_size, int max_blocks, int dtype);
 int mi_paged_decode_fp4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                         const int32_t* seqlen, void* out, int B, int H, int H_kv, int D, int block_size,

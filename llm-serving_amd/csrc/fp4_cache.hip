@@ -412,6 +412,7 @@ extern "C" int mi_qk_norm_rope_write_fp4(const void* qkv, int64_t row_stride, in
   if (norm_mode != 0 && norm_mode != 1) {
     return fail(MI_ERR_INVALID, "mi_qk_norm_rope_write_fp4: norm_mode %d is not 0 or 1", norm_mode);
   }
+  if (B == 0) return MI_OK;
   if (qkv == nullptr || q_norm_w == nullptr || k_norm_w == nullptr || cos_tab == nullptr || sin_tab == nullptr ||
       pos == nullptr || slot_ids == nullptr || q_out == nullptr || k_pool == nullptr || v_pool == nullptr) {
     return fail(MI_ERR_INVALID, "mi_qk_norm_rope_write_fp4: NULL pointer argument");
@@ -419,7 +420,6 @@ extern "C" int mi_qk_norm_rope_write_fp4(const void* qkv, int64_t row_stride, in
   if (!aligned16({k_pool, v_pool, q_out, k_out, v_out})) {
     return fail(MI_ERR_UNSUPPORTED, "mi_qk_norm_rope_write_fp4: the pools and outputs must be 16-byte aligned");
   }
-  if (B == 0) return MI_OK;
   const EpilogueArgs a{qkv, row_stride, qkv_parts, int64_t(B) * row_stride, q_norm_w, k_norm_w, cos_tab, sin_tab, n_pos,
                        rotary_dim, pos, slot_ids, q_out, k_out, v_out, B, H, H_kv, eps, norm_mode, error_word};
   const int in_size = qkv_parts > 0 ? 4 : esize_of(dtype);

@@ -730,8 +730,9 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
       out == nullptr) {
     return fail(MI_ERR_INVALID, "mi_paged_decode_fp4: NULL tensor pointer");
   }
-  if ((long long)max_blocks * block_size * B > 2147483647LL) {
-    return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: B * max_blocks * block_size must stay below 2^31 tokens");
+  // token counts and their rounding up to whole rounds stay in 32 bits
+  if ((long long)max_blocks * block_size * B > (1LL << 30)) {
+    return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: B * max_blocks * block_size must stay within 2^30 tokens");
   }
   const Fp4Plan p = make_plan(B, H, H_kv, D, dtype);
   if (int64_t(p.slots) * p.cols > 0x7fffffff / (64 * 8)) {  // threads of the grid in 32 bits

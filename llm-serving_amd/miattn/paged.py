@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from array import array
 from types import SimpleNamespace
 
 import numpy as np
@@ -332,7 +333,7 @@ class PagedPool:
                 store[b] = store[a]
             return
         _lib.require_library("PagedPool.copy_blocks on a HIP pool")
-        pools = (ctypes.c_void_p * len(stores))(*[t.data_ptr() for t in stores])
+        pools = (ctypes.c_void_p * len(stores)).from_buffer(array("Q", map(torch.Tensor.data_ptr, stores)))
         page = stores[0].stride(0) * stores[0].element_size()
         with _lib.on_device(self.keys[0].device):
             rc = _lib.lib.mi_copy_pages(pools, len(stores), page, self.n_blocks, (ctypes.c_int32 * len(src))(*src),

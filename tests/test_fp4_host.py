@@ -119,6 +119,21 @@ def test_c_entries_refuse_bad_sizes_before_any_launch():
     assert decode(width=0) == _lib.MI_ERR_INVALID and decode(strides=None) == _lib.MI_ERR_INVALID
     assert decode() == _lib.MI_ERR_INVALID and "NULL" in _lib.last_error()
     assert decode(B=0) == _lib.MI_OK
+    # sizes and the workspace are looked at before any pointer is used
+    dense = _lib.int64_array([256, 64, 1088, 544, 1088, 544, 256, 64, 2, 0])
+
+    def placed(width=2, strides=dense, q=4096, workspace=4096, size=1 << 30):
+        return lib.mi_paged_decode_fp4(q, 4096, 4096, 4096, 4096, 4096, 1, 4, 2, 64, 16, width, strides, 1.0, 2, workspace,
+                                       size, None)
+
+    need = lib.mi_paged_decode_fp4_workspace_size(1, 4, 2, 64, 16, 2, 2)
+    assert need > 0 and lib.mi_paged_decode_fp4_workspace_size(1, 3, 2, 64, 16, 2, 2) == 0
+    assert placed(workspace=None) == _lib.MI_ERR_WORKSPACE and placed(workspace=4100) == _lib.MI_ERR_WORKSPACE
+    assert placed(size=need - 1) == _lib.MI_ERR_WORKSPACE
+    assert placed(width=(1 << 26) + 1) == _lib.MI_ERR_UNSUPPORTED and "2^30" in _lib.last_error()
+    assert placed(q=4104) == _lib.MI_ERR_UNSUPPORTED and "aligned" in _lib.last_error()
+    assert placed(strides=_lib.int64_array([256, 60, 1088, 544, 1088, 544, 256, 64, 2, 0])) == _lib.MI_ERR_UNSUPPORTED
+    assert placed(strides=_lib.int64_array([256, 64, 1080, 544, 1088, 544, 256, 64, 2, 0])) == _lib.MI_ERR_UNSUPPORTED
 
     def epilogue(B=1, H=4, H_kv=2, D=64, bs=16, rotary=64, row=512, n_pos=8, mode=0, parts=0):
         return lib.mi_qk_norm_rope_write_fp4(None, row, parts, None, None, None, None, n_pos, rotary, None, None, 64, None,
@@ -128,6 +143,7 @@ def test_c_entries_refuse_bad_sizes_before_any_launch():
     assert epilogue(mode=2) == _lib.MI_ERR_INVALID and epilogue(parts=-1) == _lib.MI_ERR_INVALID
     assert epilogue(rotary=128) == _lib.MI_ERR_UNSUPPORTED and epilogue(H=5) == _lib.MI_ERR_INVALID
     assert epilogue() == _lib.MI_ERR_INVALID and "NULL" in _lib.last_error()
+    assert epilogue(B=0) == _lib.MI_OK
 
 
 def test_c_page_copy_refuses_ids_outside_the_pool():

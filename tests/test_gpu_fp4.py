@@ -289,6 +289,8 @@ def test_epilogue_idle_and_refused_rows_write_nothing_and_return_zeros(cuda):
     assert torch.equal(k[[0, 5]].cpu().double(), oracle.held(k_out[[0, 5]]))
     with pytest.raises(IndexError, match="token [124] of"):
         pool.check_writes()
+    none = pool.write_qk_norm_rope(0, slots[:0].cuda(), qkv[:0].cuda(), *args, pos[:0].cuda(), 1e-6)
+    assert none.shape == (0, H, D)
     idle = torch.full((B,), -1, device=cuda)
     assert not pool.write_qk_norm_rope(0, idle, qkv.cuda(), *args, pos.cuda(), 1e-6).any()
     pool.check_writes()  # idle seats report nothing
