@@ -64,6 +64,38 @@ __device__ __forceinline__ uint32_t fp4_encode(const float (&x)[8], int scale_by
 
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+
+// The same for eight 16-bit elements as they are in memory: the largest |x| as 16-bit integers, two at a time, and the
+// conversions that read 16-bit pairs (a third of the instructions; a write of 4311 tokens at H_kv 8 / D 128 7.2 -> 6.9 us).
+template <typename T>
+__device__ __forceinline__ uint32_t fp4_group_max16(const uint4& w) {
+  auto bits = [](uint32_t x) { return __builtin_bit_cast(u16x2_t, x & 0x7fff7fffu); };
+  const u16x2_t a = __builtin_elementwise_max(bits(w.x), bits(w.y)), b = __builtin_elementwise_max(bits(w.z), bits(w.w));
+  const u16x2_t c = __builtin_elementwise_max(a, b);
+  uint32_t m = max_u32(c.x, c.y);
+  m = max_u32(m, uint32_t(__builtin_amdgcn_update_dpp(0, int(m), kDppQuadXor1, 0xf, 0xf, false)));
+  m = max_u32(m, uint32_t(__builtin_amdgcn_update_dpp(0, int(m), kDppQuadXor2, 0xf, 0xf, false)));
+  return __float_as_uint(to_f32(T{uint16_t(m)}));  // infinity and NaN stay what they are
+}
+template <typename T>
+__device__ __forceinline__ uint32_t fp4_encode16(const uint4& x, int scale_byte) {
+  const float s = fp4_scale(uint32_t(scale_byte));
+  uint32_t w = 0;
+  if constexpr (std::is_same<T, bf16_t>::value) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x.x), s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x.y), s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x.z), s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x.w), s, 3);
+  } else {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(f16x2_t, x.x), s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(f16x2_t, x.y), s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(f16x2_t, x.z), s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(f16x2_t, x.w), s, 3);
+  }
+  return scale_byte == 255 ? 0u : w;
+}
 
 // The eight values of a code dword.
 __device__ __forceinline__ void fp4_decode(uint32_t w, float scale, float (&x)[8]) {

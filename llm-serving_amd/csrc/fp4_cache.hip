@@ -32,6 +32,32 @@ __device__ __forceinline__ Fp4Place fp4_place(const Fp4Pool& p, int64_t slot, in
           page + ((int64_t(D / 2)) << p.bs_log2) + (int64_t(c >> 2) << p.bs_log2) + at};
 }
 
+// Eight elements as they are loaded: 16-bit types stay packed.
+template <typename T, bool kVec>
+struct Raw8 {
+  float x[8];
+  __device__ __forceinline__ void load(const T* p, int64_t stride) { load8<T, kVec, true>(p, stride, x); }
+  __device__ __forceinline__ int byte() const { return fp4_scale_byte(fp4_group_max(x)); }
+  __device__ __forceinline__ uint32_t code(int b) const { return fp4_encode(x, b); }
+};
+template <typename T>
+struct Packed8 {
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p, int64_t) { w = load16_nt(p); }
+  __device__ __forceinline__ int byte() const { return fp4_scale_byte(fp4_group_max16<T>(w)); }
+  __device__ __forceinline__ uint32_t code(int b) const { return fp4_encode16<T>(w, b); }
+};
+
+template <typename T, bool kVec>
+using Loaded8 = std::conditional_t<kVec && sizeof(T) == 2, Packed8<T>, Raw8<T, kVec>>;
+
+template <typename R>
+__device__ __forceinline__ void fp4_put_raw(uint8_t* pool, const Fp4Place& at, int c, const R& x) {
+  const int byte = x.byte();
+  *reinterpret_cast<uint32_t*>(pool + at.code) = x.code(byte);
+  if ((c & 3) == 0) pool[at.scale] = uint8_t(byte);
+}
+
 template <int D>
 __device__ __forceinline__ void fp4_put(uint8_t* pool, const Fp4Place& at, int c, const float (&x)[8]) {
   const int byte = fp4_scale_byte(fp4_group_max(x));
@@ -58,13 +84,13 @@ __global__ __launch_bounds__(256) void fp4_write_kernel(const T* __restrict__ k,
   const int head = int(i - grp * uint32_t(H_kv));
   const int64_t first = int64_t(grp) * (TPW * kRows) + lane / LPR;
   if (first >= n_tokens) return;  // whole quads leave together
-  float x[kRows][8], y[kRows][8];
+  Loaded8<T, kVec> x[kRows], y[kRows];
   int64_t slot[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int64_t token = first + r * TPW < n_tokens ? first + r * TPW : first;  // past the end: not stored
-    load8<T, kVec, true>(k + token * ks0 + head * ks1 + c * 8 * ks2, ks2, x[r]);
-    load8<T, kVec, true>(v + token * vs0 + head * vs1 + c * 8 * vs2, vs2, y[r]);
+    x[r].load(k + token * ks0 + head * ks1 + c * 8 * ks2, ks2);
+    y[r].load(v + token * vs0 + head * vs1 + c * 8 * vs2, vs2);
     slot[r] = int64_t(slots[token]);
   }
 #pragma unroll
@@ -76,8 +102,8 @@ __global__ __launch_bounds__(256) void fp4_write_kernel(const T* __restrict__ k,
       continue;
     }
     const Fp4Place at = fp4_place<D>(pool, slot[r], head, c);
-    fp4_put<D>(pool.k, at, c, x[r]);
-    fp4_put<D>(pool.v, at, c, y[r]);
+    fp4_put_raw(pool.k, at, c, x[r]);
+    fp4_put_raw(pool.v, at, c, y[r]);
   }
 }
 
