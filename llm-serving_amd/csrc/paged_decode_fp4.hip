@@ -25,7 +25,18 @@
 //     overflows), so the accumulators are rarely rescaled; sums are fp32.
 // Rows are cut into splits of whole rounds (one tile per wave of the workgroup), planned on the device from the row
 // lengths so that the splits of all rows fill the chip however ragged the batch is; the waves of a
-// workgroup take a split's tiles in turn and are merged through LDS, splits of one row by a second small launch.
+// workgroup take a split's tiles in turn and are merged through LDS; the last workgroup of a row to finish
+// folds its splits.
+//
+// Measured (H 16 / H_kv 8 / D 128 bf16, us per layer in a graph; an empty launch is 1.8 there): one row of 300 tokens 5.5, 8
+// of 512 6.8, 32 of 128-2048 14.0, 32 of 8192 52-54 (285 MB: 5.4 TB/s, about 6.1 between the launch's ramp and its
+// end; a large copy reaches 5.15), one of 100003 26-27. A 16-bit cache reads 3.8 times the bytes (32 of 8192: 162 us).
+// Bound by memory in the long cases; in the short ones by round trips (row lengths, page ids, K and V: 4 us with the
+// launch) and, per round of 8 tiles on a CU, 0.75 us of vector instructions (about 200 a tile and wave: 64 conversions, 32
+// exchanges, 8 exponentials at a quarter of the rate). Tried and left: a workgroup for all KV heads at once, so that
+// whole pages are swept (32 of 8192 53.3 against 51.0, more splits to fold elsewhere); 16 waves per workgroup
+// (as 8 in long rows, 1 us slower in short ones); two register sets, loads two tiles ahead (half the waves, 8 of
+// 512 8.0 against 6.8).
 #include <type_traits>
 
 #include "fp4.h"
@@ -565,11 +576,12 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
   __syncthreads();        // sm_last has been read by every wave; its words are used again below
   const auto row_parts = partial_rsrc(partials + (int64_t(si.first) * a.cols + column) * part_floats,
                                       (int64_t(si.n_split - 1) * a.cols + 1) * part_floats);
-  // NG groups of threads take the splits in turn, kFold at a time, and are folded through LDS
+  // ng groups of threads take the splits in turn and are folded through LDS, in the groups' order
   const int lanes = nh * (D / 4);                       // threads that hold one split's sums, 4 each
   const int ng = max(1, 64 * kW / lanes);               // 64 kW threads, lanes a multiple of 16
   float* sm_f = smem;                                   // [group][lanes] sums, then [group][lanes] (m, l)
   float* sm_g = smem + ng * lanes * 4;
+  // splits loaded at once by a group (2, 1 or 8: within 2% either way, 1 up to 10% slower with many splits)
   constexpr int kFold = 4;
   for (int i0 = 0; i0 < lanes; i0 += 64 * kW) {  // more than one pass where a column has more sums than threads
     const int grp = ng > 1 ? threadIdx.x / lanes : 0;
