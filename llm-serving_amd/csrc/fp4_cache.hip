@@ -65,6 +65,16 @@ __device__ __forceinline__ void fp4_put(uint8_t* pool, const Fp4Place& at, int c
   if ((c & 3) == 0) pool[at.scale] = uint8_t(byte);
 }
 
+// 1 / sqrt(x), rounded once for a normal x: the instruction's result (within an ulp) and one Newton step on its exact residual
+// 1 - x r^2.
+__device__ __forceinline__ float exact_rsqrt(float x) {
+  const float r = __builtin_amdgcn_rsqf(x);
+  const float h = x * r;
+  const float e = fmaf(-fmaf(x, r, -h), r, fmaf(-h, r, 1.0f));
+  const float y = fmaf(0.5f * r, e, r);
+  return x >= 0x1p-100f && x <= 0x1p100f ? y : r;  // the others: zero, infinity, NaN, or a residual out of range
+}
+
 __device__ __forceinline__ void report(int32_t* err, int64_t row) {
   if (err != nullptr) atomicCAS(err, 0, int32_t(row + 1));
 }
@@ -224,10 +234,16 @@ __global__ __launch_bounds__(256) void fp4_epilogue_kernel(EpilogueArgs a, Fp4Po
       load8<T, kVec, true>(static_cast<const T*>(a.qkv) + src + int64_t(head) * D, 1, x);
     }
     if (head < a.H + a.H_kv) {  // uniform over a head's lanes
-      float ss = 0.0f;
+      // Each operation rounded by itself and the squares added in the order of a tensor reduction (fours in turn from
+      // D 128 on, then pairs): the result is the one that fp32 tensor operations give, so a k next to a border of
+      // its 4-bit levels falls to the same side as theirs.
+#pragma clang fp contract(off)
+      float sq[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
-      const float r = 1.0f / sqrtf(group_allreduce<LPR, SumOp>(ss) * (1.0f / D) + a.eps);
+      for (int j = 0; j < 8; ++j) sq[j] = x[j] * x[j];
+      const float low = D == 64 ? (sq[0] + sq[1]) + (sq[2] + sq[3]) : ((sq[0] + sq[1]) + sq[2]) + sq[3];
+      const float high = D == 64 ? (sq[4] + sq[5]) + (sq[6] + sq[7]) : ((sq[4] + sq[5]) + sq[6]) + sq[7];
+      const float r = exact_rsqrt(group_allreduce<LPR, SumOp>(low + high) * (1.0f / D) + a.eps);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float w = head < a.H ? wq[j] : wk[j];
@@ -236,7 +252,8 @@ __global__ __launch_bounds__(256) void fp4_epilogue_kernel(EpilogueArgs a, Fp4Po
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float p = half == 64 ? dpp<kDppRowRor8>(x[j]) : half == 32 ? swap4(x[j]) : swap16(x[j]);
-        if (e0 < a.rotary) x[j] = e0 < half ? x[j] * cs[j] - p * sn[j] : x[j] * cs[j] + p * sn[j];
+        const float own = x[j] * cs[j], other = p * sn[j];
+        if (e0 < a.rotary) x[j] = e0 < half ? own - other : own + other;
         x[j] = to_f32(from_f32<T>(x[j]));
       }
     }

@@ -75,7 +75,9 @@ _READ_SLOTS = (
 
 class Fp4PagedPool(PagedPool):
     """Physical KV blocks in 4 bits: uint8 ``(n_blocks, n_kv_head, page_bytes)`` K and V per layer (the
-    module docstring has the format). ``dtype`` is what writes take, reads return and queries are."""
+    module docstring has the format). ``dtype`` is what writes take, reads return and queries are.
+    ``write_qk_norm_rope`` keeps norm and rotation in fp32 and rounds q and k to ``dtype`` once (the 16-bit
+    pool's rounds after every op); the pool holds the 4-bit form of that k, as a write of ``k_out`` would."""
 
     def _check_storage(self) -> None:
         enforce(_POOL, self)

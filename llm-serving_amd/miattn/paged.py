@@ -333,6 +333,8 @@ class PagedPool:
                 store[b] = store[a]
             return
         _lib.require_library("PagedPool.copy_blocks on a HIP pool")
+        if not all(map(torch.Tensor.is_contiguous, stores)):
+            raise ValueError("copy_blocks needs contiguous keys and values")
         pools = (ctypes.c_void_p * len(stores)).from_buffer(array("Q", map(torch.Tensor.data_ptr, stores)))
         page = stores[0].stride(0) * stores[0].element_size()
         with _lib.on_device(self.keys[0].device):

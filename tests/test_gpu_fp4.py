@@ -534,6 +534,38 @@ def test_captured_step_replays_with_new_tokens_and_lengths(lengths, cuda):
         _within(out, eager_q, pool, table, seqlen)
 
 
+def test_captured_one_shot_call_brings_its_own_zeroed_workspace(cuda):
+    """Two graphs of the plain call (rows that are cut into splits), replayed several times in turn and at once on
+    two streams, with eager calls between: every replay equals the eager call."""
+    cases = [_pool_case([2500, 4000, 0, 31], 8, 4, 128, 16, torch.bfloat16, seed=s) for s in (3, 4)]
+    graphs, outs = [], []
+    for pool, q, table, seqlen in cases:
+        paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen)  # the lengths are known to be in range
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(6):
+        for j, (pool, q, table, seqlen) in enumerate(cases):
+            q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(10 * i + j)))
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream if i % 2 else torch.cuda.current_stream()):
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, (pool, q, table, seqlen) in zip(outs, cases):
+            assert torch.equal(out, paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen))
+
+
+def test_copy_blocks_refuses_pools_that_are_not_contiguous(cuda):
+    pool = PagedPool(1, 8, 16, 2, 64, dtype=torch.bfloat16, device=cuda)
+    pool.keys[0] = torch.zeros(8, 16, 4, 64, dtype=torch.bfloat16, device=cuda)[:, :, :2]
+    with pytest.raises(ValueError, match="contiguous"):
+        pool.copy_blocks([0], [1])
+
+
 def test_calls_on_two_streams_and_repeated_calls_give_the_same_bits(cuda):
     """The same call twice gives the same bits, and two plans may run at once on two streams."""
     cases = [_pool_case([2500, 400, 31], 16, 8, 128, 16, torch.bfloat16, seed=s) for s in (1, 2)]
