@@ -260,7 +260,7 @@ class Fp4DecodePlan:
     reference, ``seqlen`` updates in place seen; one workspace, so its runs stay ordered on one stream)."""
 
     __slots__ = ("n_layer", "geometry", "q_signature", "_k_ptrs", "_v_ptrs", "_pools", "_table", "_seqlen", "_ws",
-                 "_strides", "_frozen", "_shape", "_stride", "_dtype", "_device")
+                 "_strides", "_frozen", "_shape", "_stride", "_dtype", "_device", "_index", "_table_ptr", "_seqlen_ptr")
 
     def __init__(self, q, k_caches, v_caches, block_table, seqlen, *, scale=None) -> None:
         _require_backend()
@@ -282,7 +282,9 @@ class Fp4DecodePlan:
         self._pools = (ks, vs)  # keeps the pool tensors alive
         self._k_ptrs = [k.data_ptr() for k in ks]
         self._v_ptrs = [v.data_ptr() for v in vs]
-        self._table, self._seqlen = block_table, seqlen
+        self._table, self._seqlen = block_table, seqlen  # kept alive; read in place at every run
+        self._table_ptr, self._seqlen_ptr = block_table.data_ptr(), seqlen.data_ptr()
+        self._index = q.device.index
         self._strides = _strides(q, ks[0], vs[0], q, block_table)
         n_ws = _workspace_bytes(g, q.dtype)
         self._ws = torch.zeros(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
@@ -300,12 +302,18 @@ class Fp4DecodePlan:
                 f"shape/dtype/device/strides {self.q_signature}, got "
                 f"{(tuple(q.shape), q.dtype, q.device, q.stride())}); build a new plan for a new layout"
             )
-        with _lib.on_device(self._device):
-            out = torch.empty_like(q)
-            rc = _lib.lib.mi_paged_decode_fp4(
-                q.data_ptr(), self._k_ptrs[layer], self._v_ptrs[layer], self._table.data_ptr(),
-                self._seqlen.data_ptr(), out.data_ptr(), *self._frozen, _lib.current_stream(self._device))
-        _lib.check(rc, "paged_decode_fp4_plan.run")
+        if self._index != _lib._current_device():
+            with torch.cuda.device(self._index):
+                return self._launch(layer, q)
+        return self._launch(layer, q)
+
+    def _launch(self, layer: int, q) -> torch.Tensor:
+        out = torch.empty_like(q)
+        rc = _lib.lib.mi_paged_decode_fp4(q.data_ptr(), self._k_ptrs[layer], self._v_ptrs[layer], self._table_ptr,
+                                          self._seqlen_ptr, out.data_ptr(), *self._frozen,
+                                          _lib.current_stream(self._device))
+        if rc:
+            _lib.check(rc, "paged_decode_fp4_plan.run")
         return out
 
     def fused_supported(self, dtype: torch.dtype, rotary_dim: int, zero_centred_norm: bool = False) -> bool:
