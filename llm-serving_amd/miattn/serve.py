@@ -140,7 +140,8 @@ class BlockFreeList:
             for b in table:
                 times[b] = times.get(b, 0) + 1
         free = set(self._free)
-        if len(times) + len(free) != self._n_blocks or any(b in free for b in times) or \
+        if len(times) + len(free) != self._n_blocks or \
+                any(b in free or not 0 <= b < self._n_blocks for b in times) or \
                 any(n != self._holders.get(b, 1) for b, n in times.items()):
             raise ValueError("compact needs the table of every live request: these tables hold other blocks than "
                              "were handed out")

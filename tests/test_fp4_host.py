@@ -262,4 +262,7 @@ def test_compact_refuses_tables_that_are_not_all_of_them():
         blocks.compact([a, b, [7]])
     with pytest.raises(ValueError, match="every live request"):
         blocks.compact([a, b, list(a)])  # not shared, yet in two tables
+    for outside in (-1, 8):
+        with pytest.raises(ValueError, match="every live request"):
+            blocks.compact([a, [b[0], outside]])  # as many blocks as are held, one of them not the pool's
     assert blocks.compact([a, b]) == ([], [])
