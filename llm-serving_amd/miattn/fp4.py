@@ -150,7 +150,8 @@ class Fp4PagedPool(PagedPool):
     def _launch_epilogue(self, layer, source, row_stride, n_parts, q_norm_w, k_norm_w, cos, sin, rotary, pos, slot_ids,
                          q, k_out, v_out, eps, zero_centred_norm) -> int:
         B, H, D = q.shape
-        tensors = (source, q_norm_w, k_norm_w, cos, sin, pos, slot_ids, *(t for t in (k_out, v_out) if t is not None))
+        tensors = (source, q_norm_w, k_norm_w, cos, sin, pos, slot_ids, q)
+        tensors += tuple(t for t in (k_out, v_out) if t is not None)
         if any(t.device != self._home for t in tensors):
             raise RuntimeError(f"the pool is on {self._home} and takes every tensor of the epilogue there")
         with _lib.on_device(self._home):

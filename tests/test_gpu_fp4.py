@@ -240,6 +240,25 @@ def test_epilogue_rounds_once_and_stores_what_a_write_of_its_k_would(dtype, B, H
     assert torch.equal(q, q2) and torch.equal(third.keys[0], pool.keys[0]) and torch.equal(third.values[0], pool.values[0])
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("B,H,H_kv,D,rotary,zero_centred", [
+    (3, 16, 8, 128, 128, False), (700, 8, 2, 256, 64, True), (700, 16, 16, 64, 64, False), (7, 24, 2, 128, 64, False)])
+def test_epilogue_gives_the_bits_of_fp32_tensor_operations(dtype, B, H, H_kv, D, rotary, zero_centred, cuda):
+    """So a k next to a border between two 4-bit levels is stored as the level that those operations give."""
+    dt, eps = DTYPES[dtype], 1e-6
+    qkv, qw, kw, cos, sin, pos = (t.cuda() for t in _epilogue_case(B, H, H_kv, D, rotary, dt, seed=7 * B + D))
+    pool = Fp4PagedPool(1, -(-B // 16), 16, H_kv, D, dtype=dt, device=cuda, n_head=H, strict_writes=True)
+    k_out = torch.empty(B, H_kv, D, dtype=dt, device=cuda)
+    q = pool.write_qk_norm_rope(0, torch.arange(B, device=cuda), qkv, qw, kw, cos, sin, pos, eps, k_out=k_out,
+                                rotary_dim=rotary, zero_centred_norm=zero_centred)
+    heads = qkv.view(B, H + 2 * H_kv, D)
+    c, s = cos[pos].float().unsqueeze(1), sin[pos].float().unsqueeze(1)
+    for got, x, w in ((q, heads[:, :H].float(), qw.float()), (k_out, heads[:, H: H + H_kv].float(), kw.float())):
+        y = x * torch.rsqrt(x.pow(2).mean(-1, True) + eps) * (1 + w if zero_centred else w)
+        a, b, rest = y[..., : rotary // 2], y[..., rotary // 2: rotary], y[..., rotary:]
+        assert torch.equal(got, torch.cat([a * c - b * s, a * s + b * c, rest], -1).to(dt))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("parts", [1, 2, 3, 9])
 def test_epilogue_of_partial_sums_is_that_of_their_rounded_sum(dtype, parts, cuda):
