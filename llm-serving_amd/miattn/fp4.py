@@ -258,7 +258,8 @@ def paged_decode_fp4(q, k_cache, v_cache, block_table, seqlen, *, scale: float |
 class Fp4DecodePlan:
     """Checked-once launch state for the decode calls of one container over a 4-bit pool: the counterpart of
     :class:`~miattn.decode.PagedDecodePlan`, with the same contract (pools, table and ``seqlen`` by
-    reference, ``seqlen`` updates in place seen; one workspace, so its runs stay ordered on one stream)."""
+    reference, ``seqlen`` updates in place seen; one workspace, so its runs stay ordered on one stream). Built
+    outside a capture: the workspace is cleared once, here, and the host waits for that."""
 
     __slots__ = ("n_layer", "geometry", "q_signature", "_k_ptrs", "_v_ptrs", "_pools", "_table", "_seqlen", "_ws",
                  "_strides", "_frozen", "_shape", "_stride", "_dtype", "_device", "_index", "_table_ptr", "_seqlen_ptr")
@@ -288,7 +289,12 @@ class Fp4DecodePlan:
         self._index = q.device.index
         self._strides = _strides(q, ks[0], vs[0], q, block_table)
         n_ws = _workspace_bytes(g, q.dtype)
-        self._ws = torch.zeros(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
+        with _lib.on_device(q.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("paged_decode_fp4_plan clears its workspace once, which a capture would only record: "
+                                   "build the plan before the capture")
+            self._ws = torch.zeros(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
+            torch.cuda.current_stream().synchronize()  # runs may be on any stream
         self._frozen = (*g.dims(), self._strides, float(1.0 / math.sqrt(g.head_dim) if scale is None else scale),
                         _lib.dtype_code(q.dtype), None if self._ws is None else self._ws.data_ptr(), n_ws)
 

@@ -578,6 +578,35 @@ def test_captured_one_shot_call_brings_its_own_zeroed_workspace(cuda):
             assert torch.equal(out, paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen))
 
 
+def test_a_plan_built_on_a_busy_stream_runs_on_another(cuda):
+    """Its workspace, cleared at the build, is clear for the first run, whichever stream that is on."""
+    pool, q, table, seqlen = _pool_case([4000, 31], 8, 4, 128, 16, torch.bfloat16, seed=5)
+    want = paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen)  # the lengths are known to be in range
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        junk = torch.full((1 << 20,), 0x55, dtype=torch.uint8, device=cuda)  # small enough to share the plan's blocks
+        del junk
+        torch.cuda._sleep(20_000_000)
+        plan = paged_decode_fp4_plan(q, pool.keys, pool.values, table, seqlen)
+    for _ in range(3):
+        assert torch.equal(plan.run(0, q), want)
+
+
+def test_a_plan_is_not_built_inside_a_capture(cuda):
+    pool, q, table, seqlen = _pool_case([40], 8, 4, 128, 16, torch.bfloat16, seed=5)
+    want = paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            paged_decode_fp4_plan(q, pool.keys, pool.values, table, seqlen)
+        out = paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(out, want)
+
+
 def test_copy_blocks_refuses_pools_that_are_not_contiguous(cuda):
     pool = PagedPool(1, 8, 16, 2, 64, dtype=torch.bfloat16, device=cuda)
     pool.keys[0] = torch.zeros(8, 16, 4, 64, dtype=torch.bfloat16, device=cuda)[:, :, :2]
