@@ -101,16 +101,21 @@ struct Fp4Split {
   int b, split, n_split, first, len, begin, end;
 };
 // This workgroup's (row, split) and its tokens, derived by every wave from the row lengths, 64 rows at a time. Tokens
-// per split: total / target in whole rounds; as long as the splits of the first 64 rows (one per row at least,
-// an empty row's writes its zeros) are more than target the chunk grows, up to kFitSteps times. A row's tokens
-// are then shared out evenly over its splits, again in whole rounds.
-// A merge of splits costs 2-3 us (a partial's way to memory, the count's there and back, the partials' way back), a round of
-// tiles 0.75 (D 256: about 2), so rows of up to kWhole tokens stay whole and no split is shorter than kLeast. Measured,
-// us per layer, H 16 / H_kv 8 / D 128: 4 rows of 600 whole 6.9, cut at 512 8.8; one of 1000 8.5 either way; one of 8000 with
-// kLeast 512 10.2, 768 10.7; D 256, 16 rows of 128-2048: kLeast 256 11.7, 512 14.2.
+// per split: the share, total / target in whole rounds, or kLeast if that is more; as long as the splits of the first 64 rows
+// (one per row at least, an empty row's writes its zeros) are more than target the share grows, up to kFitSteps times. A
+// row's tokens are then shared out evenly over its splits, again in whole rounds.
+// A merge of splits costs about 2 us (a partial's way to memory, the count's there and back, the partials' way back) and more
+// with their number, a round of tiles 0.75 (D 256: about 2) where others hide its loads, up to 2 where nothing does. So
+// no split is shorter than kLeast, or half of it in rows of up to kShortRow, and rows of up to kWhole tokens stay whole,
+// kWholeAlone where the share says that the chip is far from full. Measured, us per layer, H 16 / H_kv 8 / D 128: 4 rows of
+// 600 whole 6.9, cut at 256 8.3; one of 1000 whole 8.8, cut at 512 8.5, at 256 7.7; 4 of 1000 9.1 and 8.3 (256); 4 of 2048
+// cut at 512 9.4, at 256 9.7; one of 8000 at 512 10.2, at 768 10.7. D 256, 8 / 2 heads: one of 500 whole 9.6, cut at 128
+// 7.6; 16 rows of 128-2048 cut at 256 10.0, at 128 10.9, at 128 only up to 1024 tokens 10.0.
 constexpr int kFitSteps = 8;
 template <int D> constexpr int kLeast = D == 256 ? 256 : 512;
 template <int D> constexpr int kWhole = D == 256 ? 512 : 1024;
+template <int D> constexpr int kWholeAlone = D == 256 ? 256 : 768;
+constexpr int kShortRow = 1024;
 template <int kRound, int D>
 __device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, const Fp4DecodeArgs& a, int w,
                                            Fp4Split& si) {
@@ -123,18 +128,18 @@ __device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, c
     total += __builtin_amdgcn_readlane(wave_inclusive_scan(row < a.B ? clamp_len(seqlen[row], capacity) : 0), 63);
   }
   // total / target rounded up to whole rounds: the share of one split
-  int chunk = (int((uint32_t(total) + uint32_t(a.target) * kRound - 1u) / (uint32_t(a.target) * kRound))) * kRound;
-  chunk = chunk > kLeast<D> ? chunk : kLeast<D>;
+  int share = (int((uint32_t(total) + uint32_t(a.target) * kRound - 1u) / (uint32_t(a.target) * kRound))) * kRound;
   auto count = [&](int len, int row) {
+    const int chunk = len > kShortRow ? max(share, kLeast<D>) : max(share, kLeast<D> / 2);
     const int n = ceil_div(len, chunk);
-    return row < a.B ? (len > kWhole<D> ? n : 1) : 0;
+    return row < a.B ? (len > (share > kLeast<D> / 2 ? kWhole<D> : kWholeAlone<D>) ? n : 1) : 0;
   };
   int n = count(len_first, lane), incl = wave_inclusive_scan(n);
   if (2 * a.B <= a.target) {
-    const int step = (chunk / 16 + kRound) / kRound * kRound;
+    const int step = (share / 16 + kRound) / kRound * kRound;
 #pragma unroll 1
     for (int i = 0; i < kFitSteps && __builtin_amdgcn_readlane(incl, 63) > a.target; ++i) {
-      chunk += step;
+      share += step;
       n = count(len_first, lane);
       incl = wave_inclusive_scan(n);
     }
@@ -581,8 +586,9 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
   const int ng = max(1, 64 * kW / lanes);               // 64 kW threads, lanes a multiple of 16
   float* sm_f = smem;                                   // [group][lanes] sums, then [group][lanes] (m, l)
   float* sm_g = smem + ng * lanes * 4;
-  // splits loaded at once by a group (2, 1 or 8: within 2% either way, 1 up to 10% slower with many splits)
-  constexpr int kFold = 4;
+  // splits loaded at once by a group: 2, 1 or 8 are within 2% of 4 either way, 1 up to 10% slower with many splits; with the
+  // few groups of D 256 in 4 waves 8 are faster (one row of 8000 13.0 -> 12.1 us)
+  constexpr int kFold = D == 256 && kW == 4 ? 8 : 4;
   for (int i0 = 0; i0 < lanes; i0 += 64 * kW) {  // more than one pass where a column has more sums than threads
     const int grp = ng > 1 ? threadIdx.x / lanes : 0;
     const int i = ng > 1 ? threadIdx.x - grp * lanes : i0 + threadIdx.x;
@@ -669,7 +675,10 @@ Fp4Plan make_plan(int B, int H, int H_kv, int D, int dtype) {
   // CUs and at most all of them, too few splits per row for 256 workgroups to be dealt out evenly. us per layer, 8 and 4
   // waves: 32 ragged rows (256 in all) 16.1 and 14.0, 16 of 4000-8000 (128) 27.3 and 25.9, 32 of 500 8.1 and 8.7, 32 of 8192 51.9
   // and 53.6; outside, 8 of 512 (64) 7.1 and 7.6, 64 ragged rows (512) 21.5 and 22.4, one of 8000 10.2 and 10.3.
-  p.waves = int64_t(B) * p.cols > 128 && int64_t(B) * p.cols <= 256 ? 4 : 8;
+  // At D 256 a round of 8 waves is two tiles per SIMD, so up to 32 rows times columns, which leave CUs idle, take 4 as well:
+  // 16 ragged rows of 2 columns 10.9 and 10.0, 8 of 512 (32) 10.0 and 8.6; 32 ragged rows (64) 13.1 and 13.5.
+  const int64_t items = int64_t(B) * p.cols;
+  p.waves = (D == 256 && items <= 32) || (items > 128 && items <= 256) ? 4 : 8;
   const int groups = p.waves == 8 ? 256 : 512;
   p.target = groups / p.cols > 1 ? groups / p.cols : 1;
   p.slots = p.target + B;

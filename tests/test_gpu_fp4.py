@@ -374,6 +374,15 @@ def test_decode_of_every_head_group(H, H_kv, dtype, D, cuda):
     _within(paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen), q, pool, table, seqlen)
 
 
+@pytest.mark.parametrize("n", [255, 256, 257, 383, 385, 511, 512, 513, 767, 768, 769, 1023, 1024, 1025, 1537, 2049, 3000])
+@pytest.mark.parametrize("H,H_kv,D,dtype", [(16, 8, 128, "bf16"), (8, 2, 256, "fp16"), (16, 1, 256, "bf16"), (4, 4, 64, "fp32")])
+def test_decode_around_the_lengths_where_rows_are_cut(n, H, H_kv, D, dtype, cuda):
+    """One row alone, and beside others that share the chip with it."""
+    for others in ([], [2300, 130, 0, 900]):
+        pool, q, table, seqlen = _pool_case([n, *others], H, H_kv, D, 16, DTYPES[dtype], seed=n)
+        _within(paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen), q, pool, table, seqlen)
+
+
 @pytest.mark.parametrize("bs", [16, 32, 64, 128, 512])
 def test_decode_of_every_page_size(bs, cuda):
     pool, q, table, seqlen = _pool_case([1, bs - 1, bs, bs + 1, 3 * bs + 5], 8, 4, 128, bs, torch.bfloat16, seed=bs)
