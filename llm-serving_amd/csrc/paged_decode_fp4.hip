@@ -17,10 +17,13 @@
 //     tokens; converted pairs lie along D and are exchanged between two tokens by v_perm_b32 (one
 //     instruction per pair), so a register holds one element of two tokens. The 8 tokens are those whose scores
 //     the same lane holds of S, so P needs no exchange between lanes;
-//   * exactness: q of a 16-bit type in one bf16 operand (bf16) or a high and a low one (fp16), fp32 in three. p in
-//     fp32 is cut into a high and a low bf16 part, 16 bits together (three parts, 24 bits, for fp32
-//     outputs), so no precision is lost against fp32 products. The parts are columns of the same product
-//     that would be empty otherwise: NC = 2 columns per query head (4 for fp32), 8 (4) heads at a time;
+//   * exactness: q of a 16-bit type in one bf16 operand (bf16) or a high and a low one (fp16), fp32 in three, all exact.
+//     p is in fp32; for fp32 outputs it is cut into three bf16 parts, its 24 bits. For 16-bit outputs it is the nearest bf16
+//     and the nearest one to what that leaves: off by at most 2^-17 of p, either way, so the errors of a row's tokens average
+//     out (cut instead, up to 2^-14 and always towards zero, one output in 27 (fp16, 16 ragged rows at D 256) or 160
+//     (bf16, 32 at D 128) is not its type's nearest value to the 64-bit result; so, one in 82 or 420; fp32 tensor operations 580
+//     and 3400). A third part would be exact, for 16 more instructions a tile and half the heads a pass. The parts are columns of the same product that would be empty
+//     otherwise: NC = 2 columns per query head (4 for fp32), 8 (4) heads at a time;
 //   * the running maximum is raised only when a tile's is past it by 2^8 (p stays below 2^8, nothing
 //     overflows), so the accumulators are rarely rescaled; sums are fp32.
 // Rows are cut into splits of whole rounds (one tile per wave of the workgroup), planned on the device from the row
@@ -69,6 +72,10 @@ __device__ __forceinline__ float hi_bf16(float x) { return __uint_as_float(__flo
 // the high halves of two floats as a bf16 pair (cut, not rounded)
 __device__ __forceinline__ uint32_t pack_hi(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+// two floats rounded to the nearest bf16, as a pair
+__device__ __forceinline__ uint32_t pack_near(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)lo, (__bf16)hi});
 }
 __device__ __forceinline__ bf16x8_t operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __builtin_bit_cast(bf16x8_t, make_uint4(a, b, c, d));
@@ -349,7 +356,8 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
   for (int i = 0; i < VE; ++i) o[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, mc = 0.0f, l = 0.0f;  // the running maximum (of q . k), times c2, and the sum of p
   const float raise = fminf(kRaise / c2, 3.0e38f);
-  const uint32_t cut1 = part >= 1 ? 0xffff0000u : 0u, cut2 = part >= 2 ? 0xffff0000u : 0u;
+  // of p, what the parts before this column's hold: by pairs with two parts, by value with three
+  const uint32_t cut1 = part >= 1 ? (NC == 4 ? 0xffff0000u : 0xffffffffu) : 0u, cut2 = part >= 2 ? 0xffff0000u : 0u;
 
   // One tile: the scores from K, the running maximum, the sums from V; `next` issues the loads that come into K's, then
   // into V's registers.
@@ -414,15 +422,25 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
         float x = fast_exp2(fmaf(s[u][i], c2, -mc));
         if constexpr (kMasked) x = t0 + 16 * u + 4 * lg + i < t_end ? x : 0.0f;
         l += x;
-        x -= __uint_as_float(__float_as_uint(x) & cut1);
         if constexpr (NC == 4) {
+          x -= __uint_as_float(__float_as_uint(x) & cut1);
           x -= __uint_as_float(__float_as_uint(x) & cut2);
           if (part == 3) x = 0.0f;
         }
         p[4 * u + i] = x;
       }
     }
-    const bf16x8_t pf = operand(pack_hi(p[0], p[1]), pack_hi(p[2], p[3]), pack_hi(p[4], p[5]), pack_hi(p[6], p[7]));
+    uint32_t pw[4];  // this column's part of two p each
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (NC == 4) {
+        pw[j] = pack_hi(p[2 * j], p[2 * j + 1]);
+      } else {
+        const uint32_t near = pack_near(p[2 * j], p[2 * j + 1]) & cut1;  // part 0 takes nothing away
+        pw[j] = pack_near(p[2 * j] - __uint_as_float(near << 16), p[2 * j + 1] - __uint_as_float(near & 0xffff0000u));
+      }
+    }
+    const bf16x8_t pf = operand(pw[0], pw[1], pw[2], pw[3]);
     if constexpr (kMasked) {
       // past the end: zero codes, and scales of 1 (garbage may be a NaN scale, which 0 * NaN would keep)
 #pragma unroll

@@ -822,3 +822,21 @@ def test_decode_of_lengths_past_24_bits(cuda):
             want = 4.0 * sum(t < lengths[r] for t in marks) / lengths[r]
             # fp32 sums of n ones over some hundred waves, a few thousand each: well inside 2^-18
             assert (out[r].double() / want - 1).abs().max() <= 2.0 ** -18
+
+
+def test_decode_gives_nearly_always_the_nearest_value_of_its_type(cuda):
+    """Weights and V of one sign, so that what the weights are off by does not cancel in the output. Each p is off by at
+    most 2^-17, to either side: over some hundred tokens 2^-20 of an output, and the fp32 sums and scores 2^-19 at most
+    (n = 600 terms of 2^-24 in a random walk, scores of a few units): 2^-18.4 together. An output of fp16 has steps of
+    2^-11 of its value at least, so at most 2^-7.4 of them, 0.6%, round to the other side of a border. (Weights cut to 16 bits
+    are 2^-17 too small on average, one output in 100.)"""
+    lengths = torch.randint(300, 600, (32,), generator=torch.Generator().manual_seed(1)).tolist()
+    pool, q, table, seqlen = _pool_case(lengths, 16, 8, 128, 16, torch.float16, seed=21)
+    for r, n in enumerate(lengths):
+        ids = table[r, : -(-n // 16)].tolist()
+        k, v = pool.read_slots(0, pool.slot_ids(ids, 0, n))
+        pool.write_prefill(0, ids, 0, k, v.abs())
+    out = paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen)
+    want, _, _ = oracle.paged_attention(q, pool.keys[0], pool.values[0], table, seqlen)
+    off = (out.cpu() != want.to(torch.float16))
+    assert off.double().mean() <= 2.0 ** -7.4, f"{int(off.sum())} of {off.numel()}"
