@@ -24,8 +24,9 @@
 //     (bf16, 32 at D 128) is not its type's nearest value to the 64-bit result; so, one in 82 or 420; fp32 tensor operations 580
 //     and 3400). A third part would be exact, for 16 more instructions a tile and half the heads a pass. The parts are columns of the same product that would be empty
 //     otherwise: NC = 2 columns per query head (4 for fp32), 8 (4) heads at a time;
-//   * the running maximum is raised only when a tile's is past it by 2^8 (p stays below 2^8, nothing
-//     overflows), so the accumulators are rarely rescaled; sums are fp32.
+//   * the running maximum is raised only when a tile's is past it by 2^8, so the accumulators are rarely rescaled. p is
+//     taken against a reference 2^8 above that maximum: never more than 1, as against the row's own largest, so the fp32 sums of
+//     p v overflow only where those do (the format holds values to 1.5 * 2^127). Terms below 2^-118 of the largest are lost.
 // Rows are cut into splits of whole rounds (one tile per wave of the workgroup), planned on the device from the row
 // lengths so that the splits of all rows fill the chip however ragged the batch is; the waves of a
 // workgroup take a split's tiles in turn and are merged through LDS; the last workgroup of a row to finish
@@ -54,7 +55,7 @@ struct Fp4DecodeArgs {
 };
 
 constexpr int kTile = 32;       // tokens per wave and step
-constexpr float kRaise = 8.0f;  // log2 units a tile's maximum may be past the running one
+constexpr float kRaise = 8.0f;  // log2 units a tile's maximum may be past the running one, and p's reference above that
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -178,7 +179,7 @@ __device__ __forceinline__ bool plan_split(const int32_t* __restrict__ seqlen, c
   }
 }
 
-// One split's partial of one column: sums of nh heads, then (m, l) of each; whole 16 bytes.
+// One split's partial of one column: sums of nh heads, then (reference, l) of each; whole 16 bytes.
 __host__ __device__ constexpr int partial_floats(int nh, int D) { return nh * D + (2 * nh + 3) / 4 * 4; }
 
 // Device-scope 16- and 8-byte accesses of the partials: written through to, and read from, the level that all XCDs share,
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
   constexpr int VE = D / 16;                // V elements per lane and token
   constexpr int VW = VE >= 8 ? VE / 8 : 1;  // dwords they take (D 64: half of one)
   constexpr int NC = kCols<T>, HB = kHeads<T>;
-  extern __shared__ __align__(16) float smem[];  // per wave: (m, l) of HB heads, then nh x D sums
+  extern __shared__ __align__(16) float smem[];  // per wave: (reference, l) of HB heads, then nh x D sums
 
   Fp4Split si;
   // Columns (KV head and chunk of its query heads) are the fast index, so the workgroups that have a split come first and
@@ -354,7 +355,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
   f32x4_t o[VE];
 #pragma unroll
   for (int i = 0; i < VE; ++i) o[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = -INFINITY, mc = 0.0f, l = 0.0f;  // the running maximum (of q . k), times c2, and the sum of p
+  float m = -INFINITY, mc = 0.0f, l = 0.0f;  // the running maximum (of q . k), p's reference in log2 units, the sum of p
   const float raise = fminf(kRaise / c2, 3.0e38f);
   // of p, what the parts before this column's hold: by pairs with two parts, by value with three
   const uint32_t cut1 = part >= 1 ? (NC == 4 ? 0xffff0000u : 0xffffffffu) : 0u, cut2 = part >= 2 ? 0xffff0000u : 0u;
@@ -407,9 +408,10 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
     most = over_groups<MaxOp>(most);
     if (__any(!(most - m <= raise))) {  // also the first tile
       const float up = fmaxf(m, most);
-      const float alpha = m == -INFINITY ? 0.0f : fast_exp2((m - up) * c2);
+      const float ref = up == -INFINITY ? 0.0f : fmaf(up, c2, kRaise);
+      const float alpha = m == -INFINITY ? 0.0f : fast_exp2(mc - ref);
       m = up;
-      mc = up == -INFINITY ? 0.0f : up * c2;
+      mc = ref;
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < VE; ++i) o[i] *= alpha;
@@ -506,7 +508,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
     compute(t0, std::true_type{}, none, none);
   }
 
-  // ---- the waves' states through LDS (not q's part of it, which other waves may still read): (m, l) per head, then the
+  // ---- the waves' states through LDS (not q's part of it, which other waves may still read): (reference, l) per head, then the
   // sums, parts added up, four elements at a time. Piece x of a head is rows 4 lg + r of the products, elements
   // 4 n .. 4 n + 3 of each, x = (r VE / 4 + n) 4 + lg: the lane groups of a column and, heads being 16 words apart
   // modulo the banks, its heads write side by side.
@@ -522,7 +524,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
     for (int r = 0; r < 4; ++r) o[i][r] = over_parts<NC>(o[i][r]);
   }
   if (part == 0 && g < nh) {
-    if (lg == 0) *reinterpret_cast<float2*>(sm_ml + (wave * HB + g) * 2) = make_float2(m, l);
+    if (lg == 0) *reinterpret_cast<float2*>(sm_ml + (wave * HB + g) * 2) = make_float2(m == -INFINITY ? m : mc, l);
     float* dst = sm_o + (wave * nh + g) * kHeadWords + lg * 4;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -563,7 +565,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kW; ++w) {
-      const float wt = ml[w].x == -INFINITY ? 0.0f : fast_exp2((ml[w].x - M) * c2);
+      const float wt = ml[w].x == -INFINITY ? 0.0f : fast_exp2(ml[w].x - M);
       L = fmaf(ml[w].y, wt, L);
       acc.x = fmaf(v[w].x, wt, acc.x);
       acc.y = fmaf(v[w].y, wt, acc.y);
@@ -576,7 +578,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
       const u32x4_nt val = {__float_as_uint(acc.x), __float_as_uint(acc.y), __float_as_uint(acc.z), __float_as_uint(acc.w)};
       __builtin_amdgcn_raw_buffer_store_b128(val, mine, (gg * D + x * 4) * 4, 0, kSc1);
       if (x == 0) {
-        const u32x2_t mine_ml = {__float_as_uint(M == -INFINITY ? M : M * c2), __float_as_uint(L)};
+        const u32x2_t mine_ml = {__float_as_uint(M), __float_as_uint(L)};
         __builtin_amdgcn_raw_buffer_store_b64(mine_ml, mine, (nh * D + gg * 2) * 4, 0, kSc1);
       }
     }
@@ -602,7 +604,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
   // ng groups of threads take the splits in turn and are folded through LDS, in the groups' order
   const int lanes = nh * (D / 4);                       // threads that hold one split's sums, 4 each
   const int ng = max(1, 64 * kW / lanes);               // 64 kW threads, lanes a multiple of 16
-  float* sm_f = smem;                                   // [group][lanes] sums, then [group][lanes] (m, l)
+  float* sm_f = smem;                                   // [group][lanes] sums, then [group][lanes] (reference, l)
   float* sm_g = smem + ng * lanes * 4;
   // splits loaded at once by a group: 2, 1 or 8 are within 2% of 4 either way, 1 up to 10% slower with many splits; with the
   // few groups of D 256 in 4 waves 8 are faster (one row of 8000 13.0 -> 12.1 us)

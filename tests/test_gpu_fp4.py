@@ -840,3 +840,25 @@ def test_decode_gives_nearly_always_the_nearest_value_of_its_type(cuda):
     want, _, _ = oracle.paged_attention(q, pool.keys[0], pool.values[0], table, seqlen)
     off = (out.cpu() != want.to(torch.float16))
     assert off.double().mean() <= 2.0 ** -7.4, f"{int(off.sum())} of {off.numel()}"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n", [320, 5000])
+def test_decode_of_the_largest_values_stays_finite(n, D, dtype, cuda):
+    """Tokens whose scores lie a little above those before them, with V near the format's largest (1.5 * 2^127): weights of
+    the row's own largest or less, the products stay in fp32, and the result is V's size."""
+    H, H_kv, dt = 4, 2, DTYPES[dtype]
+    pool, _, table, seqlen = _pool_case([n], H, H_kv, D, 16, dt, seed=13)
+    q = torch.ones(1, H, D, dtype=dt, device=cuda)
+    k, v = torch.zeros(n, H_kv, D, dtype=dt), torch.randn(n, H_kv, D).to(dt)
+    for t, size in ((300, 1.5), (n - 1, -0.75)):
+        k[t], v[t] = 1.0, size * 2.0 ** 126
+    v[300, 1] = 1.5 * 2.0 ** 127
+    pool.write_prefill(0, table[0][: -(-n // 16)].tolist(), 0, k.cuda(), v.cuda())
+    # 7.5 binary orders above the scores of 0, and 100
+    for above in (7.5, 100.0):
+        scale = above * math.log(2.0) / D
+        out = paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen, scale=scale)
+        assert out.isfinite().all() and out.abs().max() > 2.0 ** 120
+        _within(out, q, pool, table, seqlen, scale=scale)
