@@ -372,11 +372,12 @@ int mi_qk_norm_rope_write_fp4(const void* qkv, int64_t row_stride, int qkv_parts
 /* mi_paged_decode over a 4-bit pool: out[b, h] = softmax(scale * q[b, h] K^T) V over the first seqlen[b] tokens
  * (clamped to [0, max_blocks * block_size]; zeros for none), fp32 sums, rounded to `dtype` once.
  * strides = {q_s0, q_s1, k_s0, k_s1, v_s0, v_s1, o_s0, o_s1, bt_s0}: q and out (B, H, D) in elements with D
- * contiguous, the pools' block and head strides in bytes, the table's row stride; every row, head and page
- * 16-byte aligned. B * max_blocks * block_size within 2^30. Block ids are trusted. One launch; a row cut into
- * splits is folded by the last of its workgroups to finish, in the splits' order (the result does not depend
- * on who was last). Workspace: mi_paged_decode_fp4_workspace_size() bytes, 16-byte aligned, zeroed once before its
- * first call (it starts with those workgroups' counters, which every call leaves zero); calls that share one
+ * contiguous, the pools' block and head strides in bytes, the table's row stride; every row, head and page 16-byte
+ * aligned; mi_fp4_page_bytes below 2^31, B * max_blocks * block_size within 2^30 (else MI_ERR_UNSUPPORTED). Block
+ * ids are trusted. One launch; a row cut into splits is folded by the last of its workgroups to finish, in the
+ * splits' order (the result does not depend on who was last). Workspace: mi_paged_decode_fp4_workspace_size()
+ * bytes, 16-byte aligned, zeroed once before its first call (it starts with those workgroups' counters, which
+ * every call leaves zero); calls that share one
  * must be ordered. */
 size_t mi_paged_decode_fp4_workspace_size(int B, int H, int H_kv, int D, int block_size, int max_blocks, int dtype);
 int mi_paged_decode_fp4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,

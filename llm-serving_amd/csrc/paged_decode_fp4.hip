@@ -679,6 +679,9 @@ bool fp4_dim(int D) { return D == 64 || D == 128 || D == 256; }
 
 bool fp4_block(int bs) { return bs >= 16 && (bs & (bs - 1)) == 0; }
 
+// The kernel's offsets inside a page of one KV head are 32 bits.
+bool fp4_page_fits(int bs, int D) { return fp4_page_bytes(bs, D) <= 0x7fffffff; }
+
 struct Fp4Plan {
   int n_hchunks, cols, waves, target, slots, nh;
   size_t counter_bytes, partial_bytes;
@@ -741,8 +744,8 @@ int launch_t(int D, const void* q, const void* k, const void* v, const int32_t* 
 extern "C" size_t mi_paged_decode_fp4_workspace_size(int B, int H, int H_kv, int D, int block_size, int max_blocks,
                                                      int dtype) {
   using namespace miattn;
-  if (B < 1 || H < 1 || H_kv < 1 || H % H_kv != 0 || !fp4_dim(D) || !fp4_block(block_size) || max_blocks < 1 ||
-      esize_of(dtype) == 0) {
+  if (B < 1 || H < 1 || H_kv < 1 || H % H_kv != 0 || !fp4_dim(D) || !fp4_block(block_size) ||
+      !fp4_page_fits(block_size, D) || max_blocks < 1 || esize_of(dtype) == 0) {
     return 0;
   }
   return make_plan(B, H, H_kv, D, dtype).bytes();
@@ -763,6 +766,10 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
   if (!fp4_block(block_size)) {
     return fail(MI_ERR_UNSUPPORTED,
                 "mi_paged_decode_fp4: the 4-bit cache needs a power-of-two block_size of at least 16, got %d", block_size);
+  }
+  if (!fp4_page_fits(block_size, D)) {
+    return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: a page of one KV head must stay below 2^31 bytes, got block_size %d",
+                block_size);
   }
   if (max_blocks < 1) return fail(MI_ERR_INVALID, "mi_paged_decode_fp4: max_blocks must be >= 1");
   if (strides == nullptr) return fail(MI_ERR_INVALID, "mi_paged_decode_fp4: strides is NULL");

@@ -22,7 +22,8 @@ by token (element ``2i`` in the low half of byte ``i``), then ``head_dim / 32`` 
 ``e + 127`` (255: NaN).
 
 Limits: HIP devices only (a 4-bit pool on the host is refused); ``head_dim`` 64, 128 or 256;
-``block_size`` a power of two of at least 16; fp16, bf16 or fp32 on the 16/32-bit side.
+``block_size`` a power of two of at least 16; fp16, bf16 or fp32 on the 16/32-bit side. The attention takes pages
+below 2^31 bytes per KV head (``block_size`` below 2^24 at ``head_dim`` 256, 2^25 at 128, 2^26 at 64).
 """
 
 from __future__ import annotations
@@ -44,6 +45,8 @@ __all__ = ["GROUP", "Fp4PagedPool", "Fp4DecodePlan", "page_bytes", "paged_decode
 GROUP = 32
 _HEAD_DIMS = (64, 128, 256)
 _MIN_BLOCK = 16
+#: the attention's offsets inside a page of one KV head are 32 bits
+_MOST_PAGE_BYTES = 2**31 - 1
 _ELEMENT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 _SLOT_TYPES = (torch.int32, torch.int64)
 
@@ -191,6 +194,8 @@ _LAYOUT = (
     Rule(lambda a: _block_size(a.k, a.q.shape[2]) < _MIN_BLOCK, ValueError,
          lambda a: f"pages of {a.k.shape[2]} bytes at head_dim {a.q.shape[2]} hold no power of two block_size of at "
                    f"least {_MIN_BLOCK} tokens ({page_bytes(1, a.q.shape[2])} bytes each)"),
+    Rule(lambda a: a.k.shape[2] > _MOST_PAGE_BYTES, ValueError,
+         lambda a: f"the 4-bit decode reads pages below 2^31 bytes per KV head, got {a.k.shape[2]}"),
 )
 
 _PAGES = (

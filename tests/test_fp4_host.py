@@ -266,3 +266,25 @@ def test_compact_refuses_tables_that_are_not_all_of_them():
         with pytest.raises(ValueError, match="every live request"):
             blocks.compact([a, [b[0], outside]])  # as many blocks as are held, one of them not the pool's
     assert blocks.compact([a, b]) == ([], [])
+
+
+@pytest.mark.parametrize("D,most", [(64, 1 << 25), (128, 1 << 24), (256, 1 << 23)])
+def test_decode_refuses_pages_past_its_32_bit_offsets(D, most):
+    """Offsets inside a page of one KV head are 32 bits: the largest block sizes that fit are taken, the next is refused
+    before anything is read."""
+    lib, dense = _lib.lib, _lib.int64_array([512, 256, 1 << 34, 1 << 33, 1 << 34, 1 << 33, 512, 256, 1])
+    assert lib.mi_fp4_page_bytes(most, D) < 1 << 31 <= lib.mi_fp4_page_bytes(2 * most, D)
+    assert lib.mi_paged_decode_fp4_workspace_size(1, 4, 2, D, most, 1, 2) > 0
+    assert lib.mi_paged_decode_fp4_workspace_size(1, 4, 2, D, 2 * most, 1, 2) == 0
+
+    def call(bs):  # without a workspace, so a call of sizes that are taken ends there
+        return lib.mi_paged_decode_fp4(4096, 4096, 4096, 4096, 4096, 4096, 1, 4, 2, D, bs, 1, dense, 1.0, 2, None, 0, None)
+
+    assert call(most) == _lib.MI_ERR_WORKSPACE
+    assert call(2 * most) == _lib.MI_ERR_UNSUPPORTED and "2^31" in _lib.last_error()
+    q, table, seqlen = torch.zeros(1, 4, D), torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    page = torch.zeros(1, dtype=torch.uint8).expand(1, 2, fp4_mod.page_bytes(2 * most, D))  # no memory behind it
+    with pytest.raises(ValueError, match="below 2\\^31 bytes"):
+        fp4_mod._check(q, page, page, table, seqlen)
+    page = page[..., : fp4_mod.page_bytes(most, D)]
+    assert fp4_mod._check(q, page, page, table, seqlen).page == most
