@@ -779,7 +779,8 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
     return fail(MI_ERR_INVALID, "mi_paged_decode_fp4: NULL tensor pointer");
   }
   // token counts and their rounding up to whole rounds stay in 32 bits
-  if ((long long)max_blocks * block_size * B > (1LL << 30)) {
+  const int64_t row_tokens = int64_t(max_blocks) * block_size;  // below 2^57
+  if (row_tokens > (1LL << 30) || row_tokens * B > (1LL << 30)) {
     return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: B * max_blocks * block_size must stay within 2^30 tokens");
   }
   const Fp4Plan p = make_plan(B, H, H_kv, D, dtype);

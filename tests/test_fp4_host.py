@@ -288,3 +288,12 @@ def test_decode_refuses_pages_past_its_32_bit_offsets(D, most):
         fp4_mod._check(q, page, page, table, seqlen)
     page = page[..., : fp4_mod.page_bytes(most, D)]
     assert fp4_mod._check(q, page, page, table, seqlen).page == most
+
+
+def test_decode_counts_tokens_past_64_bits():
+    """B * max_blocks * block_size = 2^64: refused, not taken for 0."""
+    dense = _lib.int64_array([256, 64, 1 << 34, 1 << 33, 1 << 34, 1 << 33, 256, 64, 1])
+    for B, width in ((1 << 20, 1 << 19), (1, 1 << 19), (1 << 20, 1)):
+        rc = _lib.lib.mi_paged_decode_fp4(4096, 4096, 4096, 4096, 4096, 4096, B, 4, 2, 64, 1 << 25, width, dense, 1.0, 2,
+                                          None, 0, None)
+        assert rc == _lib.MI_ERR_UNSUPPORTED and "2^30" in _lib.last_error(), (B, width)
