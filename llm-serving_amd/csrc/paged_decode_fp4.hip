@@ -791,8 +791,11 @@ extern "C" int mi_paged_decode_fp4(const void* q, const void* k_cache, const voi
   const int es = esize_of(dtype);
   bool ok = true;
   for (const void* p : {q, k_cache, v_cache, static_cast<const void*>(out)}) ok = ok && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  for (int i : {0, 1, 6, 7}) ok = ok && (st[i] * es) % 16 == 0;
-  for (int i : {2, 3, 4, 5}) ok = ok && st[i] % 16 == 0;
+  // the stride of a dimension of one is never used
+  for (int i : {0, 6}) ok = ok && (B == 1 || (st[i] * es) % 16 == 0);
+  for (int i : {1, 7}) ok = ok && (H == 1 || (st[i] * es) % 16 == 0);
+  for (int i : {2, 4}) ok = ok && st[i] % 16 == 0;
+  for (int i : {3, 5}) ok = ok && (H_kv == 1 || st[i] % 16 == 0);
   if (!ok) {
     return fail(MI_ERR_UNSUPPORTED, "mi_paged_decode_fp4: q, out, k_cache and v_cache need 16-byte aligned rows and heads");
   }

@@ -201,9 +201,14 @@ _LAYOUT = (
 _PAGES = (
     Rule(lambda a: a.k.stride(2) != 1 or a.v.stride(2) != 1, ValueError,
          lambda a: f"the 4-bit decode reads contiguous pages; got strides {a.k.stride()} / {a.v.stride()}"),
-    Rule(lambda a: (a.k.data_ptr() | a.v.data_ptr()) % 16 != 0 or any(s % 16 for s in a.k.stride()[:2] + a.v.stride()[:2]),
+    Rule(lambda a: (a.k.data_ptr() | a.v.data_ptr()) % 16 != 0 or any(_odd_stride(t, i) for t in (a.k, a.v) for i in (0, 1)),
          ValueError, lambda a: "the 4-bit decode needs 16-byte aligned pages"),
 )
+
+
+def _odd_stride(pages, dim: int) -> bool:
+    """Whether a step along ``dim`` leaves the 16-byte grid (no launch steps along the heads of a single one)."""
+    return pages.stride(dim) % 16 != 0 and (dim == 0 or pages.shape[dim] > 1)
 
 
 def _block_size(k_cache, head_dim: int) -> int:

@@ -297,3 +297,18 @@ def test_decode_counts_tokens_past_64_bits():
         rc = _lib.lib.mi_paged_decode_fp4(4096, 4096, 4096, 4096, 4096, 4096, B, 4, 2, 64, 1 << 25, width, dense, 1.0, 2,
                                           None, 0, None)
         assert rc == _lib.MI_ERR_UNSUPPORTED and "2^30" in _lib.last_error(), (B, width)
+
+
+def test_decode_looks_at_the_strides_it_uses_only():
+    page = 1088
+    for H, H_kv, B, strides, taken in (
+            (4, 2, 1, [1028, 128, 2 * page, page, 2 * page, page, 1028, 128, 1], True),
+            (4, 2, 2, [1028, 128, 2 * page, page, 2 * page, page, 1028, 128, 1], False),
+            (1, 1, 2, [128, 3, page, 7, page, 9, 128, 5, 1], True),
+            (2, 1, 2, [256, 3, page, 7, page, 9, 256, 5, 1], False),
+            (4, 2, 1, [512, 128, 2 * page, 8, 2 * page, page, 512, 128, 1], False),
+            (4, 2, 1, [512, 128, 8, page, 2 * page, page, 512, 128, 1], False)):
+        rc = _lib.lib.mi_paged_decode_fp4(4096, 4096, 4096, 4096, 4096, 4096, B, H, H_kv, 128, 16, 1,
+                                          _lib.int64_array(strides), 1.0, 2, None, 0, None)
+        # without a workspace, so a call whose strides are taken ends there
+        assert rc == (_lib.MI_ERR_WORKSPACE if taken else _lib.MI_ERR_UNSUPPORTED), (H, H_kv, B, strides)

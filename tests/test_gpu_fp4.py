@@ -862,3 +862,23 @@ def test_decode_of_the_largest_values_stays_finite(n, D, dtype, cuda):
         out = paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen, scale=scale)
         assert out.isfinite().all() and out.abs().max() > 2.0 ** 120
         _within(out, q, pool, table, seqlen, scale=scale)
+
+
+def test_decode_of_one_row_or_head_whose_stride_is_odd(cuda):
+    """A dimension of one has whatever stride its tensor was cut with: a row of a packed projection whose rows are no
+    multiple of 16 bytes, one head, one KV head."""
+    pool, q, table, seqlen = _pool_case([100, 40, 0], 8, 4, 128, 16, torch.bfloat16, seed=2)
+    packed = torch.zeros(3, 8 * 128 + 4, dtype=torch.bfloat16, device=cuda)
+    packed[:, :1024] = q.view(3, -1)
+    row = packed[:, :1024].view(3, 8, 128)[:1]
+    assert row.stride() == (1028, 128, 1) and row.contiguous().stride() == row.stride()
+    want = paged_decode_fp4(q[:1].clone(), pool.keys[0], pool.values[0], table[:1], seqlen[:1])
+    assert torch.equal(paged_decode_fp4(row, pool.keys[0], pool.values[0], table[:1], seqlen[:1]), want)
+    plan = paged_decode_fp4_plan(row, pool.keys, pool.values, table[:1], seqlen[:1])
+    assert torch.equal(plan.run(0, row), want)
+    single, q1, table1, seqlen1 = _pool_case([100, 40], 1, 1, 128, 16, torch.bfloat16, seed=3)
+    want = paged_decode_fp4(q1, single.keys[0], single.values[0], table1, seqlen1)
+    odd = q1.as_strided(q1.shape, (128, 3, 1))
+    pages = [s.as_strided(s.shape, (s.stride(0), 7, 1)) for s in (single.keys[0], single.values[0])]
+    assert torch.equal(paged_decode_fp4(odd, *pages, table1, seqlen1), want)
+    assert torch.equal(paged_decode_fp4_plan(odd, pages[:1], pages[1:], table1, seqlen1).run(0, odd), want)
