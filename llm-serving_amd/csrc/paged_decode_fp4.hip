@@ -194,7 +194,7 @@ template <typename T, int D, int kW>
 __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
     const T* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const int32_t* __restrict__ block_table, const int32_t* __restrict__ seqlen, T* __restrict__ out,
-    int32_t* __restrict__ counters, float* __restrict__ partials, Fp4DecodeArgs a) {
+    unsigned* __restrict__ counters, float* __restrict__ partials, Fp4DecodeArgs a) {
   constexpr int kRound = kW * kTile;
   constexpr int KW = D / 32;                // code dwords of K per lane and 16 tokens
   constexpr int KS = D == 256 ? 2 : 1;      // scales of those
@@ -591,10 +591,10 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
-    int* counter = counters + int64_t(b) * a.cols + column;
-    const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *sm_last = before == si.n_split - 1;
-    if (before == si.n_split - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // It counts modulo n_split, so it is 0 again by itself: launches of the same row lengths that overlapped on one
+    // workspace by mistake leave it at 0 too (counted up and then cleared, it stayed off for every later launch).
+    const unsigned last = unsigned(si.n_split - 1);
+    *sm_last = atomicInc(counters + int64_t(b) * a.cols + column, last) == last;
   }
   __syncthreads();
   if (!*sm_last) return;  // uniform
@@ -705,7 +705,7 @@ Fp4Plan make_plan(int B, int H, int H_kv, int D, int dtype) {
   const int groups = p.waves == 8 ? 256 : 512;
   p.target = groups / p.cols > 1 ? groups / p.cols : 1;
   p.slots = p.target + B;
-  p.counter_bytes = (size_t(B) * p.cols * sizeof(int32_t) + 255) / 256 * 256;
+  p.counter_bytes = (size_t(B) * p.cols * sizeof(unsigned) + 255) / 256 * 256;
   p.partial_bytes = size_t(p.slots) * p.cols * partial_floats(p.nh, D) * sizeof(float);
   return p;
 }
@@ -713,7 +713,7 @@ Fp4Plan make_plan(int B, int H, int H_kv, int D, int dtype) {
 template <typename T, int D>
 int launch_d(const void* q, const void* k, const void* v, const int32_t* bt, const int32_t* seqlen, void* out,
              void* workspace, const Fp4DecodeArgs& a, const Fp4Plan& p, hipStream_t s) {
-  int32_t* counters = static_cast<int32_t*>(workspace);
+  unsigned* counters = static_cast<unsigned*>(workspace);
   float* partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.counter_bytes);
   auto go = [&](auto waves) {
     constexpr int kW = decltype(waves)::value;

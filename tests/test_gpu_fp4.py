@@ -882,3 +882,26 @@ def test_decode_of_one_row_or_head_whose_stride_is_odd(cuda):
     pages = [s.as_strided(s.shape, (s.stride(0), 7, 1)) for s in (single.keys[0], single.values[0])]
     assert torch.equal(paged_decode_fp4(odd, *pages, table1, seqlen1), want)
     assert torch.equal(paged_decode_fp4_plan(odd, pages[:1], pages[1:], table1, seqlen1).run(0, odd), want)
+
+
+def test_runs_that_overlapped_by_mistake_leave_the_plan_right(cuda):
+    """Two graphs of one plan's runs replayed at once, against its contract: those outputs are unspecified, but the runs
+    after them, in order again, are right."""
+    pool, q, table, seqlen = _pool_case([6000, 2500, 31, 4000], 4, 2, 128, 16, torch.bfloat16, seed=4)
+    plan = paged_decode_fp4_plan(q, pool.keys, pool.values, table, seqlen)
+    others = [torch.randn(q.shape, device=cuda).bfloat16() for _ in range(2)]  # no split's partial is left from the run before
+    want = [plan.run(0, x).clone() for x in others]
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            for _ in range(50):
+                plan.run(0, q)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(others, want):
+            assert torch.equal(plan.run(0, x), y)
