@@ -151,6 +151,10 @@ class Fp4PagedPool(PagedPool):
             self.check_writes()
         return k, v
 
+    def _refusal(self, token: int) -> str:
+        return (f"token {token} of a write or read had a slot (or position) outside the pool's {self.n_slots} slots "
+                f"({self.n_blocks} blocks x {self.block_size}): a write left it out, a read returned zeros for it")
+
     def _launch_epilogue(self, layer, source, row_stride, n_parts, q_norm_w, k_norm_w, cos, sin, rotary, pos, slot_ids,
                          q, k_out, v_out, eps, zero_centred_norm) -> int:
         B, H, D = q.shape

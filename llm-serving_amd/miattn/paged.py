@@ -286,8 +286,11 @@ class PagedPool:
         first_bad = int(self._write_error.item())
         if first_bad:
             self._write_error.zero_()
-            raise IndexError(f"token {first_bad - 1} of a write had a slot outside the pool's {self.n_slots} "
-                             f"slots ({self.n_blocks} blocks x {self.block_size}) and was not written")
+            raise IndexError(self._refusal(first_bad - 1))
+
+    def _refusal(self, token: int) -> str:
+        return (f"token {token} of a write had a slot outside the pool's {self.n_slots} "
+                f"slots ({self.n_blocks} blocks x {self.block_size}) and was not written")
 
     def write_prefill_slots(self, layer: int, slot_ids: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """The prefill name of :meth:`write_slots` (reference ``model/paged.py:241-250``)."""

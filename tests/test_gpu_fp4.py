@@ -905,3 +905,10 @@ def test_runs_that_overlapped_by_mistake_leave_the_plan_right(cuda):
         torch.cuda.synchronize()
         for x, y in zip(others, want):
             assert torch.equal(plan.run(0, x), y)
+
+
+def test_a_refused_read_is_not_reported_as_a_write(cuda):
+    pool = Fp4PagedPool(1, 2, 16, 2, 64, dtype=torch.bfloat16, device=cuda)
+    pool.read_slots(0, torch.tensor([3, 32], device=cuda))
+    with pytest.raises(IndexError, match="token 1 of a write or read .* a read returned zeros"):
+        pool.check_writes()
