@@ -348,7 +348,8 @@ int mi_prefill_wait_limit(int polls);
  * nearest level, ties to the even code, past 6 to 6. A group with a value that is not finite has the
  * byte 255 and reads back as NaN. Slots, slot_bits and error_word as for mi_kv_slot_write.
  * mi_kv_slot_write_fp4: k, v (n_tokens, H_kv, D) in `dtype` with element strides src_strides = {k_s0, k_s1,
- *   k_s2, v_s0, v_s1, v_s2}; distinct slots are the caller's contract.
+ *   k_s2, v_s0, v_s1, v_s2}; distinct slots are the caller's contract (a slot named twice may get one row's codes
+ *   under the other's scales).
  * mi_kv_slot_read_fp4: k, v (n_tokens, H_kv, D) contiguous in `dtype` receive the rows at the slots (repeats
  *   allowed); past fp16's largest value that value; zeros for a slot outside the pool, which is reported.
  * mi_qk_norm_rope_write_fp4: mi_qk_norm_rope_write over such a pool, with the same arguments (n_blocks and block_size
@@ -370,7 +371,8 @@ int mi_qk_norm_rope_write_fp4(const void* qkv, int64_t row_stride, int qkv_parts
                               int64_t n_blocks, int block_size, float eps, int norm_mode, int dtype,
                               int32_t* error_word, void* stream);
 /* mi_paged_decode over a 4-bit pool: out[b, h] = softmax(scale * q[b, h] K^T) V over the first seqlen[b] tokens
- * (clamped to [0, max_blocks * block_size]; zeros for none), fp32 sums, rounded to `dtype` once.
+ * (clamped to [0, max_blocks * block_size]; zeros for none), fp32 sums, rounded to `dtype` once, past fp16's largest
+ * value to that.
  * strides = {q_s0, q_s1, k_s0, k_s1, v_s0, v_s1, o_s0, o_s1, bt_s0}: q and out (B, H, D) in elements with D
  * contiguous, the pools' block and head strides in bytes, the table's row stride; every row, head and page 16-byte
  * aligned; mi_fp4_page_bytes below 2^31, B * max_blocks * block_size within 2^30 (else MI_ERR_UNSUPPORTED). Block

@@ -101,7 +101,8 @@ class Fp4PagedPool(PagedPool):
         self._code = _lib.dtype_code(self.dtype)
 
     def write_slots(self, layer: int, slot_ids: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
-        """``pool_flat[slot_ids[i]] = k[i]`` and the same for ``v``, rounded to 4 bits (``PagedPool.write_slots``)."""
+        """``pool_flat[slot_ids[i]] = k[i]`` and the same for ``v``, rounded to 4 bits (``PagedPool.write_slots``).
+        Distinct slots: a slot named twice may end up with one row's codes under the other's scales."""
         shape, dtype, home = k.shape, self.dtype, self._home
         if (len(shape) != 3 or shape[1:] != self._row or v.shape != shape or slot_ids.shape != shape[:1]
                 or k.dtype != dtype or v.dtype != dtype or slot_ids.dtype not in _SLOT_TYPES
@@ -244,7 +245,9 @@ def paged_decode_fp4(q, k_cache, v_cache, block_table, seqlen, *, scale: float |
     """Decode one query token per row against a 4-bit paged pool: ``softmax(scale q K^T) V`` over each
     row's first ``seqlen`` tokens, zeros for a row of none. ``q`` ``(B, H, D)`` fp16, bf16 or fp32;
     ``k_cache``/``v_cache`` uint8 ``(n_blocks, H_kv, page_bytes)``; ``block_table`` ``(B, width)`` int32 (ids trusted,
-    as in ``paged_decode``); ``seqlen`` ``(B,)`` int32 or int64. Sums are fp32, the output is rounded once."""
+    as in ``paged_decode``); ``seqlen`` ``(B,)`` int32 or int64. Sums are fp32, the output is rounded once; in fp16 what is past
+    its largest value (pages may hold more, written from bf16 or fp32; an fp32 sum's infinity too) comes out as that, as
+    ``Fp4PagedPool.read_slots`` returns it."""
     _require_backend()
     _require_device_tensors((("q", q), ("k_cache", k_cache), ("v_cache", v_cache),
                              ("block_table", block_table), ("seqlen", seqlen)))

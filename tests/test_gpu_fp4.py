@@ -912,3 +912,16 @@ def test_a_refused_read_is_not_reported_as_a_write(cuda):
     pool.read_slots(0, torch.tensor([3, 32], device=cuda))
     with pytest.raises(IndexError, match="token 1 of a write or read .* a read returned zeros"):
         pool.check_writes()
+
+
+def test_fp16_decode_of_values_past_its_range(cuda):
+    """Pages written from bf16 hold more than fp16 does: such outputs come out as fp16's largest value, the others as ever."""
+    pool, _, table, seqlen = _pool_case([40], 4, 2, 64, 16, torch.bfloat16, seed=6)
+    k, v = torch.zeros(40, 2, 64), torch.randn(40, 2, 64)
+    v[:, 0, :32], v[:, 1, 32:] = 2.0 ** 20, -2.0 ** 100
+    pool.write_prefill(0, table[0][:3].tolist(), 0, k.bfloat16().cuda(), v.bfloat16().cuda())
+    q = torch.randn(1, 4, 64).half().cuda()
+    out = paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen)
+    want, weight, _ = oracle.paged_attention(q, pool.keys[0], pool.values[0], table, seqlen)
+    _assert_within(out, want.clamp(-65504, 65504), _half_step(want.abs(), q.dtype) + 2.0 ** -13 * weight)
+    assert (out[0, :2, :32] == 65504).all() and (out[0, 2:, 32:] == -65504).all()
