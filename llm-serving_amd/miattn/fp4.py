@@ -93,7 +93,8 @@ class Fp4PagedPool(PagedPool):
 
     def __init__(self, *args, **kw) -> None:
         super().__init__(*args, **kw)
-        self._home = self._write_error.device  # with its index
+        # with its index: "cuda" alone would name whichever device is current at a later call
+        self.device = self._home = self._write_error.device
         self._row = torch.Size((self.n_kv_head, self.head_dim))
         self._sizes = (self.n_kv_head, self.head_dim, self.n_blocks, self.block_size)
         row = self.n_kv_head * self.head_dim

@@ -925,3 +925,13 @@ def test_fp16_decode_of_values_past_its_range(cuda):
     want, weight, _ = oracle.paged_attention(q, pool.keys[0], pool.values[0], table, seqlen)
     _assert_within(out, want.clamp(-65504, 65504), _half_step(want.abs(), q.dtype) + 2.0 ** -13 * weight)
     assert (out[0, :2, :32] == 65504).all() and (out[0, 2:, 32:] == -65504).all()
+
+
+def test_a_pool_stays_on_the_device_it_was_built_on(cuda):
+    """Built on "cuda", it names the device that was current then: tensors that its calls make later (q of the epilogue, slot
+    maps) belong to that one, whichever is current."""
+    pool = Fp4PagedPool(1, 2, 16, 2, 64, dtype=torch.bfloat16, device="cuda", n_head=4)
+    assert pool.device == pool.keys[0].device and pool.device.index is not None
+    assert pool.slot_ids([1, 0], 0, 20).device == pool.device
+    kv = PagedKV(pool, [[0, 1]], [3], rope_len=30, n_head=4)
+    assert kv.device == pool.device and kv.pos.device == pool.device
