@@ -87,9 +87,8 @@ class Fp4PagedPool(PagedPool):
         enforce(_POOL, self)
         _lib.require_library("Fp4PagedPool")
 
-    def _layer_store(self) -> torch.Tensor:
-        shape = (self.n_blocks, self.n_kv_head, page_bytes(self.block_size, self.head_dim))
-        return torch.zeros(shape, dtype=torch.uint8, device=self.device)
+    def _store_layout(self) -> tuple[tuple[int, ...], torch.dtype]:
+        return (self.n_blocks, self.n_kv_head, page_bytes(self.block_size, self.head_dim)), torch.uint8
 
     def __init__(self, *args, **kw) -> None:
         super().__init__(*args, **kw)

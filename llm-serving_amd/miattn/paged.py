@@ -28,6 +28,7 @@ from __future__ import annotations
 import ctypes
 import os
 from array import array
+from operator import is_
 from types import SimpleNamespace
 
 import numpy as np
@@ -93,13 +94,18 @@ class PagedPool:
         # device word: 1 + index of the first token a HIP write skipped, 0 when none
         self._write_error = torch.zeros(1, dtype=torch.int32, device=self.device) if self._on_device else None
         self._slot_memo: tuple[tuple, torch.Tensor] | None = None
+        self._copy_stores: tuple[list[torch.Tensor], array] = ([], array("Q"))  # that copy_blocks has looked over
 
     def _check_storage(self) -> None:
         """What a pool of another storage requires of its sizes, dtype and device."""
 
+    def _store_layout(self) -> tuple[tuple[int, ...], torch.dtype]:
+        """Shape and dtype of a layer's K or V store, blocks first."""
+        return (self.n_blocks, self.block_size, self.n_kv_head, self.head_dim), self.dtype
+
     def _layer_store(self) -> torch.Tensor:
-        shape = (self.n_blocks, self.block_size, self.n_kv_head, self.head_dim)
-        return torch.zeros(shape, dtype=self.dtype, device=self.device)
+        shape, dtype = self._store_layout()
+        return torch.zeros(shape, dtype=dtype, device=self.device)
 
     # ------------------------------------------------------------------ tables and slots
     def _layer(self, layer) -> int:
@@ -336,15 +342,28 @@ class PagedPool:
                 store[b] = store[a]
             return
         _lib.require_library("PagedPool.copy_blocks on a HIP pool")
-        if not all(map(torch.Tensor.is_contiguous, stores)):
-            raise ValueError("copy_blocks needs contiguous keys and values")
-        pools = (ctypes.c_void_p * len(stores)).from_buffer(array("Q", map(torch.Tensor.data_ptr, stores)))
+        addresses = array("Q", map(torch.Tensor.data_ptr, stores))
+        known, at = self._copy_stores
+        if len(known) != len(stores) or not all(map(is_, stores, known)) or at != addresses:
+            self._check_copy_stores(stores)
+            self._copy_stores = (stores, addresses)
+        pools = (ctypes.c_void_p * len(stores)).from_buffer(addresses)
         page = stores[0].stride(0) * stores[0].element_size()
         with _lib.on_device(self.keys[0].device):
             rc = _lib.lib.mi_copy_pages(pools, len(stores), page, self.n_blocks, (ctypes.c_int32 * len(src))(*src),
                                         (ctypes.c_int32 * len(dst))(*dst), len(src),
                                         _lib.current_stream(self.keys[0].device))
         _lib.check(rc, "PagedPool.copy_blocks")
+
+    def _check_copy_stores(self, stores) -> None:
+        """The page copy takes addresses: what ``keys`` and ``values`` hold has to be the pool's layout, on one device."""
+        shape, dtype = self._store_layout()
+        for t in stores:
+            if tuple(t.shape) != shape or t.dtype != dtype or t.device != stores[0].device:
+                raise ValueError(f"copy_blocks needs keys and values of shape {shape} and {dtype} on one device, got "
+                                 f"{tuple(t.shape)} {t.dtype} on {t.device}")
+            if not t.is_contiguous():
+                raise ValueError("copy_blocks needs contiguous keys and values")
 
     def decode_plan(self, q, block_table, seqlen, *, scale=None):
         """The decode plan of this pool's layers (``paged_decode_plan`` over ``keys`` and ``values``)."""

@@ -312,3 +312,21 @@ def test_decode_looks_at_the_strides_it_uses_only():
                                           _lib.int64_array(strides), 1.0, 2, None, 0, None)
         # without a workspace, so a call whose strides are taken ends there
         assert rc == (_lib.MI_ERR_WORKSPACE if taken else _lib.MI_ERR_UNSUPPORTED), (H, H_kv, B, strides)
+
+
+def test_page_copies_on_a_device_refuse_stores_that_are_not_the_pools():
+    """The device's copy takes addresses, so a store put in the pool's place has to have its layout. The stores here are on
+    the host: the checks come before anything is launched."""
+    for i, wrong in ((0, lambda t: t[:4].clone()), (1, lambda t: t.double()), (2, lambda t: t.flatten(2)),
+                     (3, lambda t: t.to("meta"))):
+        pool = PagedPool(2, 8, 4, 2, 8)
+        pool._on_device = True
+        stores = pool.keys if i < 2 else pool.values
+        stores[i % 2] = wrong(stores[i % 2])
+        with pytest.raises(ValueError, match="keys and values of shape \\(8, 4, 2, 8\\)"):
+            pool.copy_blocks([0], [5])
+    pool = PagedPool(2, 8, 4, 2, 8)
+    pool._on_device = True
+    pool.keys[1] = torch.zeros(8, 4, 4, 8)[:, :, :2]
+    with pytest.raises(ValueError, match="contiguous"):
+        pool.copy_blocks([0], [5])

@@ -935,3 +935,28 @@ def test_a_pool_stays_on_the_device_it_was_built_on(cuda):
     assert pool.slot_ids([1, 0], 0, 20).device == pool.device
     kv = PagedKV(pool, [[0, 1]], [3], rope_len=30, n_head=4)
     assert kv.device == pool.device and kv.pos.device == pool.device
+
+
+def test_copy_blocks_looks_at_stores_put_in_place_of_the_pools(cuda):
+    """Stores of the pool's own layout may take the place of its own at any time, others are refused each time."""
+    pool = PagedPool(2, 8, 16, 2, 64, dtype=torch.bfloat16, device=cuda)
+    for store in pool.keys + pool.values:
+        store.copy_(torch.randn_like(store))
+    for _ in range(3):
+        pool.copy_blocks([0, 1], [5, 6])
+        assert all(torch.equal(s[:2], s[5:7]) for s in pool.keys + pool.values)
+        kept, pool.keys[1] = pool.keys[1], torch.randn_like(pool.keys[1])
+        pool.copy_blocks([2], [7])
+        assert all(torch.equal(s[2], s[7]) for s in pool.keys + pool.values) and not torch.equal(kept[7], pool.keys[1][7])
+        good, pool.values[0] = pool.values[0], pool.values[0][:4].clone()
+        with pytest.raises(ValueError, match="keys and values of shape"):
+            pool.copy_blocks([0], [7])
+        pool.values[0] = good
+        moved = torch.randn_like(good)
+        pool.values[0].data = moved  # the same tensor, elsewhere
+        pool.copy_blocks([3], [4])
+        assert torch.equal(moved[3], moved[4])
+        pool.values[0].data = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16, device=cuda)
+        with pytest.raises(ValueError, match="keys and values of shape"):
+            pool.copy_blocks([0], [7])
+        pool.values[0].data = moved
