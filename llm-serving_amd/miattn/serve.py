@@ -116,7 +116,7 @@ class BlockFreeList:
         many blocks as ``blocks``); its full blocks are shared with ``blocks``, the partly filled one and
         those to come are its own. ``src``/``dst`` (one pair, or none at a block boundary) go to
         ``PagedPool.copy_blocks`` before either request writes its next token."""
-        length = int(length)
+        blocks, length = list(blocks), int(length)
         full, part = divmod(length, self.block_size)
         if length < 0 or full + (part > 0) > len(blocks):
             raise ValueError(f"a table of {len(blocks)} blocks of {self.block_size} does not hold {length} tokens")

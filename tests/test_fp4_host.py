@@ -330,3 +330,14 @@ def test_page_copies_on_a_device_refuse_stores_that_are_not_the_pools():
     pool.keys[1] = torch.zeros(8, 4, 4, 8)[:, :, :2]
     with pytest.raises(ValueError, match="contiguous"):
         pool.copy_blocks([0], [5])
+
+
+def test_fork_takes_any_sequence_of_blocks():
+    """A table kept as a tuple forks as a list does, and no block is taken or shared by a call that fails."""
+    blocks = BlockFreeList(10, 16)
+    a = tuple(blocks.take(3))
+    table, src, dst = blocks.fork(a, 37)
+    assert table[:2] == list(a[:2]) and src == [a[2]] and dst == [table[2]] and blocks.n_free == 6
+    blocks.give_back(list(a))
+    blocks.give_back(table)
+    assert blocks.n_free == 10
