@@ -134,7 +134,10 @@ class BlockFreeList:
         """Move the blocks in use to the lowest ids: ``(src, dst)`` for ``PagedPool.copy_blocks``, with
         ``tables`` (every live request's) rewritten in place; afterwards ids from the number of blocks in
         use on are free. The copy has to run, and device tables to be uploaded again, before the next
-        launch that reads or writes a moved block. Raises when ``tables`` are not what is held."""
+        launch that reads or writes a moved block. Raises, with nothing changed, when ``tables`` are not what is held
+        or cannot be rewritten."""
+        if any(not hasattr(table, "__setitem__") for table in tables):
+            raise TypeError("compact rewrites the tables in place and needs lists")
         times: dict[int, int] = {}
         for table in tables:
             for b in table:

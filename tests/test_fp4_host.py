@@ -341,3 +341,14 @@ def test_fork_takes_any_sequence_of_blocks():
     blocks.give_back(list(a))
     blocks.give_back(table)
     assert blocks.n_free == 10
+
+
+def test_compact_changes_nothing_when_a_table_cannot_be_rewritten():
+    blocks = BlockFreeList(8, 16)
+    gone, a, b = blocks.take(2), blocks.take(2), blocks.take(2)
+    blocks.give_back(gone)
+    with pytest.raises(TypeError, match="needs lists"):
+        blocks.compact([a, tuple(b)])
+    assert a == [2, 3] and b == [4, 5] and blocks.n_free == 4
+    src, dst = blocks.compact([a, b])
+    assert src == [4, 5] and dst == [0, 1] and a == [2, 3] and b == [0, 1]
