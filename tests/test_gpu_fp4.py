@@ -17,7 +17,7 @@ import math
 import pytest
 import torch
 
-from miattn import Fp4PagedPool, PackedPrefill, PagedKV, PagedPool, paged_decode_fp4, paged_decode_fp4_plan
+from miattn import Fp4PagedPool, PackedPrefill, PagedKV, PagedPool, _lib, paged_decode_fp4, paged_decode_fp4_plan
 from miattn.fp4 import page_bytes
 from miattn.qwen3 import GraphDecoder, Qwen3, Qwen3Config, random_weights
 from miattn.rows import Parts
@@ -960,3 +960,123 @@ def test_copy_blocks_looks_at_stores_put_in_place_of_the_pools(cuda):
         with pytest.raises(ValueError, match="keys and values of shape"):
             pool.copy_blocks([0], [7])
         pool.values[0].data = moved
+
+
+# ------------------------------------------------------------------ every kernel variant, and its borders
+def _waves(B, H, H_kv, D, bs, width, dtype):
+    """Waves per workgroup that a decode of these sizes takes, from its workspace: counters of each row and column (a KV head
+    and up to 8 of its query heads, 4 in fp32), then a partial per column for each of target + B splits."""
+    heads = 4 if dtype == torch.float32 else 8
+    group = H // H_kv
+    cols, nh = H_kv * -(-group // heads), min(group, heads)
+    partial = 4 * (nh * D + -(-2 * nh // 4) * 4)
+    size = _lib.lib.mi_paged_decode_fp4_workspace_size(B, H, H_kv, D, bs, width, _lib.dtype_code(dtype))
+    target, rest = divmod(size - -(-B * cols * 4 // 256) * 256, partial * cols)
+    assert rest == 0
+    return {max(1, 256 // cols): 8, max(1, 512 // cols): 4}[target - B]
+
+
+def _lengths_with(B, special, seed, most=150):
+    """``special`` (row -> length) among rows of 0 to ``most`` tokens."""
+    lengths = torch.randint(0, most, (B,), generator=torch.Generator().manual_seed(seed)).tolist()
+    for row, n in special.items():
+        lengths[row % B] = n
+    return lengths
+
+
+LONG = {0: 1100, 2: 2500, 3: 0, 5: 1, 7: 700, -1: 1500}
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("B,H,H_kv,D,waves", [
+    (16, 16, 8, 128, 8), (17, 16, 8, 128, 4), (32, 16, 8, 128, 4), (33, 16, 8, 128, 8),
+    (128, 2, 1, 128, 8), (129, 2, 1, 128, 4), (256, 2, 1, 128, 4), (257, 2, 1, 128, 8),
+    (8, 16, 16, 64, 8), (16, 16, 16, 64, 4), (257, 1, 1, 64, 8),
+    (16, 4, 2, 256, 4), (17, 4, 2, 256, 8), (33, 4, 1, 256, 8), (64, 4, 2, 256, 8), (65, 4, 2, 256, 4), (129, 4, 2, 256, 8)])
+def test_decode_in_every_variant_with_rows_that_are_cut(B, H, H_kv, D, waves, dtype, cuda):
+    """Both workgroup sizes of every type and head_dim, at the borders between them, with rows of several splits, whole ones and
+    empty ones; the same plan twice, so that a counter left behind would show."""
+    dt = DTYPES[dtype]
+    pool, q, table, seqlen = _pool_case(_lengths_with(B, LONG, B + D), H, H_kv, D, 16, dt, seed=B)
+    assert _waves(B, H, H_kv, D, 16, table.shape[1], dt) == waves
+    plan = paged_decode_fp4_plan(q, pool.keys, pool.values, table, seqlen)
+    out = plan.run(0, q)
+    _within(out, q, pool, table, seqlen)
+    assert torch.equal(plan.run(0, q), out)
+    assert torch.equal(paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen), out)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,H,H_kv", [(17, 16, 1), (20, 16, 1), (34, 8, 1), (17, 14, 1)])
+def test_decode_of_eight_wide_heads_per_column(B, H, H_kv, dtype, cuda):
+    """head_dim 256 in workgroups of 8 waves with 7 or 8 query heads per column: their states take more than 64 KiB of LDS."""
+    dt = DTYPES[dtype]
+    pool, q, table, seqlen = _pool_case(_lengths_with(B, LONG, B), H, H_kv, 256, 16, dt, seed=B)
+    assert _waves(B, H, H_kv, 256, 16, table.shape[1], dt) == 8
+    _within(paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen), q, pool, table, seqlen)
+
+
+@pytest.mark.parametrize("H,H_kv,D,dtype", [(2, 1, 128, "bf16"), (4, 2, 64, "fp16"), (2, 1, 256, "fp32")])
+@pytest.mark.parametrize("B", [65, 130, 200])
+def test_decode_of_long_rows_past_the_first_64(B, H, H_kv, D, dtype, cuda):
+    """The plan counts splits 64 rows at a time: long rows on both sides of such a border and last, run twice, then with the
+    lengths of the rows turned round."""
+    special = {62: 2100, 63: 5000, 64: 3000, 65: 2000, 66: 0, 128: 2200, 129: 4100, B - 1: 6000}
+    pool, q, table, seqlen = _pool_case(_lengths_with(B, {r: n for r, n in special.items() if r < B}, B, 40), H, H_kv, D, 16,
+                                        DTYPES[dtype], seed=B)
+    plan = paged_decode_fp4_plan(q, pool.keys, pool.values, table, seqlen)
+    for _ in range(2):
+        out = plan.run(0, q)
+        _within(out, q, pool, table, seqlen)
+        assert torch.equal(plan.run(0, q), out)
+        order = torch.arange(B - 1, -1, -1, device=cuda)
+        table.copy_(table[order])
+        seqlen.copy_(seqlen[order])
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("H_kv,D", [(2, 64), (3, 128), (1, 256)])
+@pytest.mark.parametrize("layout", ["contiguous", "permuted", "strided", "misaligned"])
+def test_large_calls_store_and_read_what_small_ones_do(dtype, H_kv, D, layout, cuda):
+    """One call on either side of the size from which a lane works on two rows, against calls of 500 tokens, whose bytes the
+    oracle's are compared with above."""
+    dt, border = DTYPES[dtype], -(-4096 * 64 // (H_kv * (D // 8)))
+    for n in (border - 1, border, border + 5):
+        g = torch.Generator(device=cuda).manual_seed(n)
+        rows = [torch.randn(n, H_kv, D, generator=g, device=cuda).to(dt) for _ in range(2)]
+        rows[0][n // 2, 0, 5], rows[1][n - 1, -1, -1] = math.nan, math.inf
+
+        def placed(x):
+            if layout == "permuted":
+                return x.permute(1, 0, 2).contiguous().permute(1, 0, 2)
+            if layout == "strided":
+                return torch.stack([x, x], -1)[..., 0]
+            if layout == "misaligned":
+                return torch.cat([x.new_zeros(1), x.flatten()])[1:].view(x.shape)
+            return x
+
+        pools = [Fp4PagedPool(1, n // 16 + 2, 16, H_kv, D, dtype=dt, device=cuda) for _ in range(2)]
+        slots = torch.randperm(pools[0].n_slots, generator=g, device=cuda)[:n]
+        slots = slots.int() if layout == "permuted" else slots
+        pools[0].write_slots(0, slots, *map(placed, rows))
+        for a in range(0, n, 500):
+            pools[1].write_slots(0, slots[a: a + 500], *(x[a: a + 500] for x in rows))
+        assert torch.equal(pools[0].keys[0], pools[1].keys[0]) and torch.equal(pools[0].values[0], pools[1].values[0])
+        whole = pools[0].read_slots(0, slots)
+        for a in range(0, n, 500):
+            part = pools[0].read_slots(0, slots[a: a + 500])
+            assert all(torch.equal(x[a: a + 500].nan_to_num(7.0), y.nan_to_num(7.0)) for x, y in zip(whole, part))
+        assert whole[0][n // 2, 0, :32].isnan().all() and int(whole[0].isnan().sum()) == 32
+        for pool in pools:
+            pool.check_writes()
+
+
+def test_decode_of_a_query_shared_by_rows_and_of_a_misaligned_one(cuda):
+    pool, q, table, seqlen = _pool_case([100, 40, 0], 8, 4, 128, 16, torch.bfloat16, seed=2)
+    shared = q[:1].expand(3, 8, 128)
+    want = paged_decode_fp4(shared.contiguous(), pool.keys[0], pool.values[0], table, seqlen)
+    assert torch.equal(paged_decode_fp4(shared, pool.keys[0], pool.values[0], table, seqlen), want)
+    flat = torch.zeros(2 * 3 * 1024 + 1, dtype=torch.bfloat16, device=cuda)
+    odd = flat[1:].view(3, 2, 8, 128)[:, 1]  # rows apart, and no address a multiple of 16 bytes
+    odd.copy_(shared)
+    assert torch.equal(paged_decode_fp4(odd, pool.keys[0], pool.values[0], table, seqlen), want)
