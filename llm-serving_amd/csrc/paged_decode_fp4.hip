@@ -32,12 +32,13 @@
 // workgroup take a split's tiles in turn and are merged through LDS; the last workgroup of a row to finish
 // folds its splits.
 //
-// Measured (H 16 / H_kv 8 / D 128 bf16, us per layer in a graph; an empty launch is 1.8 there): one row of 300 tokens 5.5, 8
-// of 512 6.8, 32 of 128-2048 14.0, 32 of 8192 52-54 (285 MB: 5.4 TB/s, about 6.1 between the launch's ramp and its
-// end; a large copy reaches 5.15), one of 100003 26-27. A 16-bit cache reads 3.8 times the bytes (32 of 8192: 162 us).
-// Bound by memory in the long cases; in the short ones by round trips (row lengths, page ids, K and V: 4 us with the
-// launch) and, per round of 8 tiles on a CU, 0.75 us of vector instructions (about 200 a tile and wave: 64 conversions, 32
-// exchanges, 8 exponentials at a quarter of the rate). Tried and left: a workgroup for all KV heads at once, so that
+// Measured (H 16 / H_kv 8 / D 128 bf16, us per layer in a graph; an empty launch is 1.8 there): one row of 300 tokens 5.6, 8
+// of 512 6.9, 32 of 128-2048 14.2, 32 of 8192 54 (285 MB: 5.3 TB/s; a large copy reaches 5.15), one of 100003 27.6. fp32:
+// 5.8, 15.4 and 61 for the first, third and fourth; D 64 (H 16 / H_kv 16): 5.0 for one of 300, 60 for 32 of 8192. A 16-bit cache
+// reads 3.8 times the bytes (32 of 8192: 162 us). Bound by memory in the long cases; in the short ones by dependent round
+// trips (row lengths with the page ids beside them, then K and V; rows behind a split one load the page ids in between) and, per
+// round of 8 tiles on a CU, 0.75 us of vector instructions (220 a tile and wave: 64 conversions, 32 exchanges, 8
+// exponentials at a quarter of the rate). Tried and left: a workgroup for all KV heads at once, so that
 // whole pages are swept (32 of 8192 53.3 against 51.0, more splits to fold elsewhere); 16 waves per workgroup
 // (as 8 in long rows, 1 us slower in short ones); two register sets, loads two tiles ahead (half the waves, 8 of
 // 512 8.0 against 6.8).
@@ -118,7 +119,9 @@ struct Fp4Split {
 // kWholeAlone where the share says that the chip is far from full. Measured, us per layer, H 16 / H_kv 8 / D 128: 4 rows of
 // 600 whole 6.9, cut at 256 8.3; one of 1000 whole 8.8, cut at 512 8.5, at 256 7.7; 4 of 1000 9.1 and 8.3 (256); 4 of 2048
 // cut at 512 9.4, at 256 9.7; one of 8000 at 512 10.2, at 768 10.7. D 256, 8 / 2 heads: one of 500 whole 9.6, cut at 128
-// 7.6; 16 rows of 128-2048 cut at 256 10.0, at 128 10.9, at 128 only up to 1024 tokens 10.0.
+// 7.6; 16 rows of 128-2048 cut at 256 10.0, at 128 10.9, at 128 only up to 1024 tokens 10.0. D 64, 16 / 16 heads, takes D 128's
+// figures: with D 256's instead one row of 600 is 7.2 for 6.3 and 4 of 600 7.6 for 6.6, the longer ones equal; at twice D 128's 16
+// rows of 128-2048 are 16.7 for 12.9, 4 of 1000 8.0 for 8.3, one of 8000 11.1 for 11.7.
 constexpr int kFitSteps = 8;
 template <int D> constexpr int kLeast = D == 256 ? 256 : 512;
 template <int D> constexpr int kWhole = D == 256 ? 512 : 1024;
@@ -695,11 +698,16 @@ Fp4Plan make_plan(int B, int H, int H_kv, int D, int dtype) {
   p.cols = H_kv * p.n_hchunks;
   p.nh = H / H_kv < heads ? H / H_kv : heads;
   // One workgroup of 8 waves per CU, or two of 4: the latter where the rows times columns are more than half the
-  // CUs and at most all of them, too few splits per row for 256 workgroups to be dealt out evenly. us per layer, 8 and 4
-  // waves: 32 ragged rows (256 in all) 16.1 and 14.0, 16 of 4000-8000 (128) 27.3 and 25.9, 32 of 500 8.1 and 8.7, 32 of 8192 51.9
-  // and 53.6; outside, 8 of 512 (64) 7.1 and 7.6, 64 ragged rows (512) 21.5 and 22.4, one of 8000 10.2 and 10.3.
+  // CUs and at most all of them, too few splits per row for 256 workgroups to be dealt out evenly. The host knows the number of
+  // rows but not their lengths, so this gives some of the even batches' time for more of the ragged ones'. us per layer
+  // with 8 and 4 waves, D 128, 32 rows (256 in all): ragged 128-2048 16.8 and 14.6, 4000-8000 56.5 and 47.3; all of 500 8.1 and
+  // 8.5, of 2000 16.9 and 18.8, of 8192 52.2 and 54.4. 17 rows (136): ragged 13.2 and 12.8, of 500 7.4 and 8.1, of 8192 44.6
+  // and 37.3. D 64, 16 rows (256): ragged 13.5 and 12.9, of 500 6.5 and 7.0, of 8192 40.2 and 41.8. D 256, 100 rows (200): ragged
+  // 29.3 and 21.8, of 4000 58.6 and 55.9. Outside: 16 rows (128) of 4000-8000 28.9 and 27.8, 8 of 512 (64) 7.4 and 7.9, 64 ragged
+  // ones (512) 22.6 and 23.4, one of 8000 equal.
   // At D 256 a round of 8 waves is two tiles per SIMD, so up to 32 rows times columns, which leave CUs idle, take 4 as well:
-  // 16 ragged rows of 2 columns 10.9 and 10.0, 8 of 512 (32) 10.0 and 8.6; 32 ragged rows (64) 13.1 and 13.5.
+  // 16 rows of 2 columns (32), ragged 11.3 and 10.2, of 512 10.5 and 8.9, but of 4000 14.6 and 17.1; 8 of 512 (16) 10.2 and 8.7,
+  // one of 500 9.9 and 7.9; 32 ragged ones (64) 13.2 and 13.5.
   const int64_t items = int64_t(B) * p.cols;
   p.waves = (D == 256 && items <= 32) || (items > 128 && items <= 256) ? 4 : 8;
   const int groups = p.waves == 8 ? 256 : 512;
