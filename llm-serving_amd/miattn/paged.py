@@ -359,11 +359,13 @@ class PagedPool:
         """The page copy takes addresses: what ``keys`` and ``values`` hold has to be the pool's layout, on one device."""
         shape, dtype = self._store_layout()
         for t in stores:
-            if tuple(t.shape) != shape or t.dtype != dtype or t.device != stores[0].device:
-                raise ValueError(f"copy_blocks needs keys and values of shape {shape} and {dtype} on one device, got "
-                                 f"{tuple(t.shape)} {t.dtype} on {t.device}")
+            if tuple(t.shape) != shape or t.dtype != dtype:
+                raise ValueError(f"copy_blocks needs keys and values of shape {shape} and {dtype}, got {tuple(t.shape)} {t.dtype}")
             if not t.is_contiguous():
                 raise ValueError("copy_blocks needs contiguous keys and values")
+        for t in stores:
+            if not t.is_cuda or t.device != stores[0].device:
+                raise ValueError(f"copy_blocks on a HIP pool needs every store on its device, got one on {t.device}")
 
     def decode_plan(self, q, block_table, seqlen, *, scale=None):
         """The decode plan of this pool's layers (``paged_decode_plan`` over ``keys`` and ``values``)."""

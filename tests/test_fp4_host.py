@@ -317,8 +317,7 @@ def test_decode_looks_at_the_strides_it_uses_only():
 def test_page_copies_on_a_device_refuse_stores_that_are_not_the_pools():
     """The device's copy takes addresses, so a store put in the pool's place has to have its layout. The stores here are on
     the host: the checks come before anything is launched."""
-    for i, wrong in ((0, lambda t: t[:4].clone()), (1, lambda t: t.double()), (2, lambda t: t.flatten(2)),
-                     (3, lambda t: t.to("meta"))):
+    for i, wrong in ((0, lambda t: t[:4].clone()), (1, lambda t: t.double()), (2, lambda t: t.flatten(2))):
         pool = PagedPool(2, 8, 4, 2, 8)
         pool._on_device = True
         stores = pool.keys if i < 2 else pool.values
@@ -352,3 +351,11 @@ def test_compact_changes_nothing_when_a_table_cannot_be_rewritten():
     assert a == [2, 3] and b == [4, 5] and blocks.n_free == 4
     src, dst = blocks.compact([a, b])
     assert src == [4, 5] and dst == [0, 1] and a == [2, 3] and b == [0, 1]
+
+
+def test_page_copies_on_a_device_refuse_stores_on_the_host():
+    """The pool's own layout, but host memory: its addresses are nothing a device may read."""
+    pool = PagedPool(2, 8, 4, 2, 8)
+    pool._on_device = True
+    with pytest.raises(ValueError, match="every store on its device, got one on cpu"):
+        pool.copy_blocks([0], [5])
