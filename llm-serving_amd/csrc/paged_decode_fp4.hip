@@ -18,12 +18,13 @@
 //     instruction per pair), so a register holds one element of two tokens. The 8 tokens are those whose scores
 //     the same lane holds of S, so P needs no exchange between lanes;
 //   * exactness: q of a 16-bit type in one bf16 operand (bf16) or a high and a low one (fp16), fp32 in three, all exact.
-//     p is in fp32; for fp32 outputs it is cut into three bf16 parts, its 24 bits. For 16-bit outputs it is the nearest bf16
-//     and the nearest one to what that leaves: off by at most 2^-17 of p, either way, so the errors of a row's tokens average
-//     out (cut instead, up to 2^-14 and always towards zero, one output in 27 (fp16, 16 ragged rows at D 256) or 160
-//     (bf16, 32 at D 128) is not its type's nearest value to the 64-bit result; so, one in 82 or 420; fp32 tensor operations 580
-//     and 3400). A third part would be exact, for 16 more instructions a tile and half the heads a pass. The parts are columns of the same product that would be empty
-//     otherwise: NC = 2 columns per query head (4 for fp32), 8 (4) heads at a time;
+//     p is in fp32; for fp32 outputs it is cut into three bf16 parts, its 24 bits. For 16-bit outputs it is the nearest
+//     bf16 and the nearest one to what that leaves: off by at most 2^-17 of p, to either side, so the errors of a row's tokens
+//     average out. One output in 82 (fp16, 16 ragged rows at D 256) or 420 (bf16, 32 at D 128) is not its type's nearest
+//     value to the 64-bit result; one in 27 or 160 with the second part cut (2^-14, always towards zero), one in 580 or 3400
+//     with fp32 tensor operations. A third part would be exact, for 16 more instructions a tile and half the heads a pass.
+//     The parts are columns of the same product that would be empty otherwise: NC = 2 columns per query head (4 for
+//     fp32), 8 (4) heads at a time;
 //   * the running maximum is raised only when a tile's is past it by 2^8, so the accumulators are rarely rescaled. p is
 //     taken against a reference 2^8 above that maximum: never more than 1, as against the row's own largest, so the fp32 sums of
 //     p v overflow only where those do (the format holds values to 1.5 * 2^127). Terms below 2^-118 of the largest are lost.
