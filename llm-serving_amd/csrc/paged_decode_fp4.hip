@@ -25,9 +25,11 @@
 //     with fp32 tensor operations. A third part would be exact, for 16 more instructions a tile and half the heads a pass.
 //     The parts are columns of the same product that would be empty otherwise: NC = 2 columns per query head (4 for
 //     fp32), 8 (4) heads at a time;
-//   * the running maximum is raised only when a tile's is past it by 2^8, so the accumulators are rarely rescaled. p is
-//     taken against a reference 2^8 above that maximum: never more than 1, as against the row's own largest, so the fp32 sums of
-//     p v overflow only where those do (the format holds values to 1.5 * 2^127). Terms below 2^-118 of the largest are lost.
+//   * the running maximum is raised only when a tile's is past it by 2^4, so the accumulators are rarely rescaled. p is
+//     taken against a reference 2^4 above that maximum: never more than 1, as against the row's own largest, so the fp32 sums of
+//     p v overflow only where those do (the format holds values to 1.5 * 2^127). Terms below 2^-122 of the largest are lost. The
+//     reference shifts the exponents, and with 2^8 their fp32 rounding was coarser (fp32 outputs, 4 rows of 500 at D 256, off by
+//     2.1e-7 of their norm against 1.5e-7; fp32 tensor operations 4.4e-7); with 2^2, 2^4 and 2^8 the times are the same.
 // Rows are cut into splits of whole rounds (one tile per wave of the workgroup), planned on the device from the row
 // lengths so that the splits of all rows fill the chip however ragged the batch is; the waves of a
 // workgroup take a split's tiles in turn and are merged through LDS; the last workgroup of a row to finish
@@ -57,7 +59,7 @@ struct Fp4DecodeArgs {
 };
 
 constexpr int kTile = 32;       // tokens per wave and step
-constexpr float kRaise = 8.0f;  // log2 units a tile's maximum may be past the running one, and p's reference above that
+constexpr float kRaise = 4.0f;  // log2 units a tile's maximum may be past the running one, and p's reference above that
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));

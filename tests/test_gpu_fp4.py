@@ -1080,3 +1080,23 @@ def test_decode_of_a_query_shared_by_rows_and_of_a_misaligned_one(cuda):
     odd = flat[1:].view(3, 2, 8, 128)[:, 1]  # rows apart, and no address a multiple of 16 bytes
     odd.copy_(shared)
     assert torch.equal(paged_decode_fp4(odd, pool.keys[0], pool.values[0], table, seqlen), want)
+
+
+def test_fp32_decode_rounds_its_exponents_finely(cuda):
+    """Rows of two tokens whose scores are 0 and c q (one element of q, so the score is exact), V 0 and 1: the output is
+    1 / (1 + 2^-cq), off by what its weights are. The exponents lie above -8 (4 for the reference, 4 at most for the score):
+    rounded by 2^-22 at most, times ln 2, over sqrt(3) in the mean square, 9.5e-8; the exponential's ulp 2^-23 / sqrt(3) = 6.9e-8; the
+    sum, the reciprocal and the product 2^-24 / sqrt(3) each. Together 1.33e-7."""
+    B, H, D = 64, 16, 64
+    pool, _, table, seqlen = _pool_case([2] * B, H, 1, D, 16, torch.float32, seed=1, garbage=False)
+    k, v = torch.zeros(2, 1, D, device=cuda), torch.zeros(2, 1, D, device=cuda)
+    k[1, 0, 0], v[1] = 1.0, 1.0
+    for ids in table[:, :1].tolist():
+        pool.write_prefill(0, ids, 0, k, v)
+    q = torch.zeros(B, H, D, device=cuda)
+    q[..., 0] = -3.9 * torch.rand(B, H, generator=torch.Generator().manual_seed(2)).cuda()
+    scale = math.log(2.0)
+    c = float(torch.tensor(scale) * torch.tensor(1.4426950408889634))  # the scale in fp32, as the exponents' unit
+    got = paged_decode_fp4(q, pool.keys[0], pool.values[0], table, seqlen, scale=scale)
+    want = 1.0 / (1.0 + 2.0 ** (-c * q[..., :1].double()))
+    assert (got.double() / want - 1).pow(2).mean().sqrt() <= 1.33e-7
