@@ -28,6 +28,9 @@
  *   mi_kv_slot_read_fp4,   4 bits              and the block-table decode over a 4-bit cache (no
  *   mi_qk_norm_rope_write_fp4, mi_paged_decode_fp4   reference counterpart)
  *   mi_copy_pages      page copies             forks and compactions of a paged cache (none either)
+ *   mi_paged_decode_window, mi_varlen_prefill_window  the two attentions under a sliding window with sinks (none either)
+ *   mi_paged_decode_weigh, mi_prompt_weights, mi_cache_evict  accounts of where attention goes, and rows of a paged
+ *                                              cache cut to a budget by them (none either)
  *
  * Conventions shared by every entry point:
  *   - every pointer except the `host_*` arguments is a device pointer;
@@ -395,6 +398,81 @@ int mi_paged_decode_fp4(const void* q, const void* k_cache, const void* v_cache,
  * an unspecified mix. */
 int mi_copy_pages(void* const* host_pools, int n_pools, int64_t page_bytes, int64_t n_blocks,
                   const int32_t* host_src, const int32_t* host_dst, int n_moves, void* stream);
+
+/* ------------------------------------------------------------------ sliding windows with sinks
+ * mi_paged_decode / mi_paged_decode_fused where row b sees its first `sinks` tokens and its last `window` ones (the
+ * query's own among them; all where it has no more than that): window >= 1, sinks >= 0. The
+ * other tokens and their table entries are not read (an entry of blocks that hold none of the seen tokens
+ * may name any block or none). The rest as for those, workspace size included. */
+int mi_paged_decode_window(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                           const int32_t* seqlen, void* out, int B, int H, int H_kv, int D, int block_size,
+                           int max_blocks, const int64_t* strides, float scale, int dtype, int window, int sinks,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int mi_paged_decode_fused_window(const void* qkv, int64_t row_stride, int qkv_parts, const void* q_norm_w,
+                                 const void* k_norm_w, const void* cos_tab, const void* sin_tab, int64_t n_pos,
+                                 int rotary_dim, const int64_t* pos, const void* slot_ids, int slot_bits,
+                                 void* k_cache, void* v_cache, const int32_t* block_table, const int32_t* seqlen,
+                                 void* out, int B, int H, int H_kv, int D, int block_size, int max_blocks,
+                                 int64_t n_slots, const int64_t* strides, float scale, float eps, int norm_mode,
+                                 int dtype, int window, int sinks, void* workspace, size_t workspace_bytes,
+                                 int32_t* error_word, void* stream);
+/* mi_varlen_prefill, causal, where query i of a segment sees key j <= i if i - j < window or j < sinks. Key tiles that
+ * no query of a tile sees are not read; head_dim 64, 128 or 256, at most 255 heads, scale > 0. A value of V
+ * that is not finite reaches the queries of its 64-key tile that do not see it too, as 0 * inf in the plain product
+ * does (a score that is not finite does not). schedule: mi_varlen_schedule_window's words (laid out as the duo
+ * schedule, with a layout word of their own), with the same window and sinks; workspace:
+ * mi_varlen_workspace_size of them. */
+int mi_varlen_schedule_window(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int D, int window, int sinks,
+                              int32_t* host_schedule, int capacity);
+int mi_varlen_prefill_window(const void* q, const void* k, const void* v, void* out, const int32_t* cu_seqlens,
+                             int n_seqs, int total_tokens, int max_seqlen, const int32_t* schedule, int n_work,
+                             int n_merge, int n_partials, int layout, int H, int H_kv, int D, float scale, int window,
+                             int sinks, int dtype, void* workspace, size_t workspace_bytes, int32_t* error_word,
+                             void* stream);
+
+/* ------------------------------------------------------------------ accounts of attention, and eviction by them
+ * mi_paged_decode_weigh: mi_paged_decode that also adds each token's attention weights to an account:
+ *   weights[b, kv, t] += sum over the query heads h of KV head kv of softmax(scale * q[b, h] K^T)[t],  t < seqlen[b],
+ *   weights fp32, element b * weights_s0 + kv * weights_s1 + t, at least max_blocks * block_size tokens wide.
+ *   Entries from seqlen[b] on stay as they are. head_dim 32, 64, 128 or 256. The workspace (16-byte aligned) has
+ *   mi_paged_decode_weigh_workspace_size() bytes, 4 per (token of the tables, query head) more than
+ *   mi_paged_decode's.
+ * mi_prompt_weights: the account of packed prompts (q (total, H, D), k (total, H_kv, D) contiguous, fp16 or bf16,
+ *   head_dim 64, 128 or 256, scale > 0): out[s, kv, j] = the weights that the last `observe` queries of segment s
+ *   give key j under causal attention, summed over the query heads of kv; zeros from the segment's length up to `width`
+ *   (at least the longest segment). out fp32, element s * out_s0 + kv * out_s1 + j. schedule: a
+ *   device copy of mi_prompt_weights_schedule's words (host only; NULL sizes it), host_header their first four.
+ *   Workspace: mi_prompt_weights_workspace_size() of that header.
+ * mi_cache_evict: rows longer than `budget` tokens cut to it, for every layer, row and KV head: the first `sinks` tokens,
+ *   the last `recent` and the heaviest of the others by `weights` (NaN above every number, the lowest index
+ *   of equal ones) are kept in their order, K and V rows and account; the account's entries from budget on up to the
+ *   old length become 0, and seqlen[b] = min(seqlen[b], budget). Pools: n_layers addresses of K and
+ *   of V, each (n_blocks, block_size, H_kv, row_bytes) contiguous, 16-byte aligned, row_bytes a power of two of
+ *   16 to 1024. weights: fp32, strides {layer, row, KV head} in elements, max_blocks * block_size wide.
+ *   to_table == block_table: in place. Another to_table (row stride to_stride, to_blocks wide): every row, those within
+ *   the budget too, is written to its blocks there, and the blocks of block_table are left as they are; it
+ *   may name no block that block_table's rows hold. No block may be in two rows of the table written to. A row whose tables
+ *   name a block outside the pool where a kept token lies loses those tokens' rows (nothing is read or
+ *   written outside) and puts 1 + its index into *error_word (may be NULL). Workspace:
+ *   mi_cache_evict_workspace_size() bytes, 16-byte aligned; calls that share one must be ordered. */
+size_t mi_paged_decode_weigh_workspace_size(int B, int H, int H_kv, int D, int block_size, int max_blocks, int dtype);
+int mi_paged_decode_weigh(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                          const int32_t* seqlen, void* out, int B, int H, int H_kv, int D, int block_size,
+                          int max_blocks, const int64_t* strides, float scale, int dtype, float* weights,
+                          int64_t weights_s0, int64_t weights_s1, void* workspace, size_t workspace_bytes,
+                          void* stream);
+int mi_prompt_weights_schedule(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int observe,
+                               int32_t* host_schedule, int capacity);
+size_t mi_prompt_weights_workspace_size(const int32_t* host_schedule, int H_kv);
+int mi_prompt_weights(const void* q, const void* k, const int32_t* schedule, const int32_t* host_header, int H, int H_kv,
+                      int D, float scale, int dtype, float* out, int64_t out_s0, int64_t out_s1, int width,
+                      void* workspace, size_t workspace_bytes, void* stream);
+size_t mi_cache_evict_workspace_size(int n_layers, int B, int H_kv, int budget);
+int mi_cache_evict(void* const* host_k_pools, void* const* host_v_pools, int n_layers, int64_t n_blocks, int block_size,
+                   int H_kv, int row_bytes, const int32_t* block_table, int64_t bt_stride, int max_blocks,
+                   const int32_t* to_table, int64_t to_stride, int to_blocks, int32_t* seqlen, float* weights,
+                   const int64_t* weight_strides, int B, int budget, int recent, int sinks, void* workspace,
+                   size_t workspace_bytes, int32_t* error_word, void* stream);
 
 #ifdef __cplusplus
 }

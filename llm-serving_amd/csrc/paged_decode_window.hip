@@ -1,0 +1,53 @@
+// The paged decode under a sliding window with sinks (kernels: paged_decode.h): row b sees its first `sinks`
+// tokens and its last `window` ones. Same bytes per visible token as the plain form and nothing for the others; the splits
+// are planned over the visible tokens, so a batch of rows far longer than the window is cut evenly.
+#include "paged_decode.h"
+
+namespace miattn {
+namespace {
+
+int windowed(Windowed& w, int window, int sinks) {
+  if (window < 1 || sinks < 0) {
+    return fail(MI_ERR_INVALID, "mi_paged_decode_window: window must be >= 1 and sinks >= 0, got %d and %d", window, sinks);
+  }
+  w.most = int(std::min<int64_t>(int64_t(window) + sinks, INT32_MAX));
+  w.sinks = sinks;
+  return MI_OK;
+}
+
+}  // namespace
+}  // namespace miattn
+
+extern "C" int mi_paged_decode_window(const void* q, const void* k_cache, const void* v_cache,
+                                      const int32_t* block_table, const int32_t* seqlen, void* out, int B, int H,
+                                      int H_kv, int D, int block_size, int max_blocks, const int64_t* strides,
+                                      float scale, int dtype, int window, int sinks, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  using namespace miattn;
+  Windowed w{};
+  const int rc = windowed(w, window, sinks);
+  if (rc != MI_OK) return rc;
+  return paged_decode_entry(q, k_cache, v_cache, block_table, seqlen, out, B, H, H_kv, D, block_size, max_blocks,
+                            strides, scale, dtype, workspace, workspace_bytes, stream, w);
+}
+
+extern "C" int mi_paged_decode_fused_window(const void* qkv, int64_t row_stride, int qkv_parts, const void* q_norm_w,
+                                            const void* k_norm_w, const void* cos_tab, const void* sin_tab,
+                                            int64_t n_pos, int rotary_dim, const int64_t* pos, const void* slot_ids,
+                                            int slot_bits, void* k_cache, void* v_cache, const int32_t* block_table,
+                                            const int32_t* seqlen, void* out, int B, int H, int H_kv, int D,
+                                            int block_size, int max_blocks, int64_t n_slots, const int64_t* strides,
+                                            float scale, float eps, int norm_mode, int dtype, int window, int sinks,
+                                            void* workspace, size_t workspace_bytes, int32_t* error_word,
+                                            void* stream) {
+  using namespace miattn;
+  Windowed w{};
+  int rc = windowed(w, window, sinks);
+  if (rc != MI_OK) return rc;
+  FusedArgs fa{};
+  rc = fused_args(fa, qkv, row_stride, qkv_parts, q_norm_w, k_norm_w, cos_tab, sin_tab, n_pos, rotary_dim, pos,
+                  slot_ids, slot_bits, B, H, H_kv, D, n_slots, eps, norm_mode, dtype, error_word);
+  if (rc != MI_OK) return rc;
+  return paged_decode_entry(nullptr, k_cache, v_cache, block_table, seqlen, out, B, H, H_kv, D, block_size, max_blocks,
+                            strides, scale, dtype, workspace, workspace_bytes, stream, w, &fa);
+}

@@ -1027,11 +1027,29 @@ struct Duo {
 // s_waitcnt lgkmcnt(0) alone (vmcnt and expcnt left at their maximum).
 __device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14)); }
 
-template <typename T, int D>
+// Windowed form (kWin): query i sees key j <= i where i - j < window or j < sinks. Of an item's key tiles those
+// that hold neither a sink nor a key within its first row's window are left out: the others are
+// numbered 0 .. n - 1, tile t < ts being tile t of the segment (sinks) and a later one tile t + jump, and
+// every step below goes by those numbers. So an item of a long segment costs what the window does.
+struct Band {
+  int ts, jump, n;
+};
+__host__ __device__ __forceinline__ Band band_of(int row0, int q_end, int window, int sinks, int BK) {
+  const int first = row0 - window + 1;
+  const int tw = first > 0 ? first / BK : 0;  // first tile of the window
+  const int s = ((sinks < q_end ? sinks : q_end) + BK - 1) / BK;
+  Band b;
+  b.ts = s < tw ? s : tw;
+  b.jump = tw - b.ts;
+  b.n = (q_end + BK - 1) / BK - b.jump;
+  return b;
+}
+
+template <typename T, int D, bool kWin = false>
 __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefill_duo_kernel(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     T* __restrict__ out, const int32_t* __restrict__ sched, float* __restrict__ partials, int H, int H_kv,
-    int G, float scale_log2, int causal, int32_t* __restrict__ err, int spin_max) {
+    int G, float scale_log2, int causal, int32_t* __restrict__ err, int spin_max, int window, int sinks) {
   using W = Duo<D>;
   constexpr int KS = D / 16;  // MFMA k-steps over D for S^T
   constexpr int DB = D / 32;  // 32-row blocks of D for O^T
@@ -1072,6 +1090,7 @@ __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefil
 
   struct Item {
     int seq0, L, row0, split, n_split, slot, h, t_first, t_end;
+    int ts, jump;  // windowed form
   };
   // an item's words are loaded (scalar) while the previous item runs, decoded when needed
   // (item 0's came with the table entry)
@@ -1090,7 +1109,13 @@ __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefil
     it.h = int(uint32_t(iw[3]) >> 24);
     it.slot = iw[3] & 0xffffff;
     const int q_end = min(it.L, it.row0 + BQ);
-    const int n_all = causal ? (q_end + BK - 1) / BK : (it.L + BK - 1) / BK;
+    int n_all = causal ? (q_end + BK - 1) / BK : (it.L + BK - 1) / BK;
+    if constexpr (kWin) {
+      const Band band = band_of(it.row0, q_end, window, sinks, BK);
+      it.ts = band.ts;
+      it.jump = band.jump;
+      n_all = band.n;
+    }
     it.t_first = it.split * n_all / it.n_split;
     it.t_end = (it.split + 1) * n_all / it.n_split;
     return it;
@@ -1123,8 +1148,14 @@ __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefil
     dma_off[p] = int(r * kv_row_b) + (((lane % W::NCH) ^ W::sw(r)) << 4);
   }
   const int dma_step = int((seg_index(LP) - seg_index(0)) * W::RPS * kv_row_b);
-  auto issue = [&](const char* seg, const Item& it, int t, uint8_t* dst) {
-    const int rows = t < it.t_end ? min(it.L - t * BK, BK) : 0;
+  // the segment's tile that an item's tile t is
+  auto tile_of = [&](const Item& it, int t) {
+    if constexpr (kWin) return t < it.ts ? t : t + it.jump;
+    return t;
+  };
+  auto issue = [&](const char* seg, const Item& it, int tv, uint8_t* dst) {
+    const int t = tile_of(it, tv);
+    const int rows = tv < it.t_end ? min(it.L - t * BK, BK) : 0;
     // the tile's byte offset as a 32 x 32 -> 64-bit unsigned product (t >= 0, and a tile's
     // bytes fit 32 bits, as its range below does): the signed 64-bit product took five
     // more scalar instructions per issue (29.6 against 29.8 us at head_dim 128, 37.1
@@ -1305,9 +1336,10 @@ __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefil
     auto step = [&](int sidx, uint8_t* kb_next, uint8_t* kb_free, const uint8_t* vb_prev, uint8_t* vb_free,
                     auto pv_c) {
       constexpr bool kPV = decltype(pv_c)::value;
-      const int t = it.t_first + sidx;
-      issue(kseg, it, t + 2, kb_free);
-      if constexpr (kPV) issue(vseg, it, t, vb_free);  // V(t0) came with the item's Q
+      const int tv = it.t_first + sidx;
+      issue(kseg, it, tv + 2, kb_free);
+      if constexpr (kPV) issue(vseg, it, tv, vb_free);  // V(t0) came with the item's Q
+      const int t = tile_of(it, tv);
       // Higher wave priority from here to the end-of-step wait: when the two waves sharing a
       // SIMD (one per workgroup) both have work, the one in its MFMA/softmax section issues
       // first, which keeps the matrix pipe fed (3-4% faster than equal priorities).
@@ -1344,7 +1376,8 @@ __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefil
       floatx16 sc = cur;
       // workgroup-uniform: only a tile that reaches past the segment end or the diagonal
       // needs the mask
-      if ((t + 1) * BK > L || (causal && (t + 1) * BK - 1 > it.row0)) {
+      if ((t + 1) * BK > L || (causal && (t + 1) * BK - 1 > it.row0) ||
+          (kWin && t * BK + window <= it.row0 + BQ - 1 && (t + 1) * BK > sinks)) {
         // at head_dim 256 the lane's query row and key group are rebuilt here from the lane
         // id: held through the item loop they were spilled, and the scratch reload's wait
         // (loads retire in order) also waited for the step's K/V loads just issued
@@ -1355,9 +1388,21 @@ __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefil
         } else {
           lim = (causal ? min(L, qi + 1) : L) - (t * BK + kh * 32) - g * 4;
         }
+        if constexpr (kWin) {
+          const int ml = __lane_id();
+          const int at = t * BK + kh * 32 + (ml >> 5) * 4;
+          // key offsets in [sink_end, lo) are neither sinks nor within the row's window
+          const int lo = it.row0 + qb * 32 + (ml & 31) - window + 1 - at, sink_end = sinks - at;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if ((e >> 2) * 8 + (e & 3) >= lim) sc[e] = -INFINITY;
+          for (int e = 0; e < 16; ++e) {
+            const int off = (e >> 2) * 8 + (e & 3);
+            if (off >= lim || (off < lo && off >= sink_end)) sc[e] = -INFINITY;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if ((e >> 2) * 8 + (e & 3) >= lim) sc[e] = -INFINITY;
+          }
         }
       }
       float mloc = sc[0];
@@ -2280,7 +2325,8 @@ __global__ __launch_bounds__(256) void varlen_prefill_merge_kernel(
 }
 
 // Schedule layout word: kernel kind << 20 | head_dim << 8 | query rows per tile.
-enum Kind { kStaged = MI_PREFILL_STAGED, kRing = MI_PREFILL_RING, kDuo = MI_PREFILL_DUO, kTall = MI_PREFILL_TALL };
+enum Kind { kStaged = MI_PREFILL_STAGED, kRing = MI_PREFILL_RING, kDuo = MI_PREFILL_DUO, kTall = MI_PREFILL_TALL,
+            kBand = 5 /* the duo kernel's windowed form: in layout words only */ };
 constexpr int layout_word(int kind, int D, int rows) { return (kind << 20) | (D << 8) | rows; }
 constexpr int layout_kind(int layout) { return layout >> 20; }
 constexpr int layout_d(int layout) { return (layout >> 8) & 0xfff; }
@@ -2355,7 +2401,7 @@ int launch2(const void* q, const void* k, const void* v, void* out, const int32_
         hipLaunchKernelGGL((varlen_prefill_duo_kernel<T, D>), dim3(n_work), dim3(Duo<D>::THREADS), 0, s,
                            static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
                            static_cast<T*>(out), sched, partials, H, H_kv, H / H_kv, scale_log2, causal, err,
-                           g_wait_limit);
+                           g_wait_limit, 0, 0);
         if (n_merge > 0) {
           hipLaunchKernelGGL((varlen_prefill_merge_kernel<T, D, Duo<D>::BQ>),
                              dim3(H, n_merge, (Duo<D>::BQ + kRowsPerBlock - 1) / kRowsPerBlock), dim3(256), 0, s,
@@ -2387,6 +2433,26 @@ int launch1(int D, const void* q, const void* k, const void* v, void* out, const
               D);
 }
 
+// The windowed form: the duo kernel over its own item lists, merged as the plain one's pieces are.
+template <typename T, int D>
+int launch_window(const void* q, const void* k, const void* v, void* out, const int32_t* cu, const int32_t* sched,
+                  int n_work, int n_merge, void* workspace, int H, int H_kv, float scale_log2, int window, int sinks,
+                  int32_t* err, hipStream_t s) {
+  constexpr int kRowsPerBlock = 256 / (D / 32);
+  float* partials = static_cast<float*>(workspace);
+  hipLaunchKernelGGL((varlen_prefill_duo_kernel<T, D, true>), dim3(n_work), dim3(Duo<D>::THREADS), 0, s,
+                     static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                     static_cast<T*>(out), sched, partials, H, H_kv, H / H_kv, scale_log2, 1, err, g_wait_limit,
+                     window, sinks);
+  if (n_merge > 0) {
+    hipLaunchKernelGGL((varlen_prefill_merge_kernel<T, D, Duo<D>::BQ>),
+                       dim3(H, n_merge, (Duo<D>::BQ + kRowsPerBlock - 1) / kRowsPerBlock), dim3(256), 0, s, cu,
+                       sched + kSchedHeader + Duo<D>::ENTRY_WORDS * n_work, static_cast<const float*>(partials),
+                       static_cast<T*>(out), H);
+  }
+  return launch_status("mi_varlen_prefill_window");
+}
+
 // One schedule piece: a query tile's key range (w0 = seq << 16 | tile, w1 = split << 28 |
 // (n_split - 1) << 24 | first partial slot), or a merge entry, with its cost in key tiles.
 struct Piece { int work, w0, w1; };
@@ -2405,7 +2471,7 @@ struct Piece { int work, w0, w1; };
 // head_dim 256 (one workgroup per CU, ~1.15 us steps, ~6 us per item's ends) 5: config-3
 // lengths 40.3 us against 42.0 with 8, 40.8 with 2, 44.1 with 1 and 11, 40.2-40.4 with 3-6.
 int duo_schedule(const int32_t* cu, const std::vector<Piece>& pieces, const std::vector<Piece>& merges,
-                 int n_partials, int H, int H_kv, int D, int32_t* out, int capacity) {
+                 int n_partials, int H, int H_kv, int D, int32_t* out, int capacity, int kind = kDuo) {
   constexpr int kCUs = 256;
   const int kItemOverhead = D == 256 ? 5 : 8;
   const int kSlots = kCUs * kind_per_cu(kDuo, D);
@@ -2452,7 +2518,7 @@ int duo_schedule(const int32_t* cu, const std::vector<Piece>& pieces, const std:
   out[0] = n_wg;
   out[1] = n_merge;
   out[2] = n_partials;
-  out[3] = layout_word(kDuo, D, Duo<128>::BQ);
+  out[3] = layout_word(kind, D, Duo<128>::BQ);
   int32_t* table = out + kSchedHeader;
   int32_t* mw = table + EW * n_wg;
   for (const Piece& pc : merges) { *mw++ = pc.w0; *mw++ = pc.w1; }
@@ -2479,6 +2545,43 @@ int duo_schedule(const int32_t* cu, const std::vector<Piece>& pieces, const std:
     }
   }
   return words;
+}
+
+// A query tile of a segment and its key tiles.
+struct Tile { int work, seq, tile; };
+
+// The tiles as pieces, longest first, and the merges of those that are cut; returns the partial slots.
+int cut_tiles(const std::vector<Tile>& tiles, int64_t total, int H, int D, int kind, std::vector<Piece>& pieces,
+              std::vector<Piece>& merges) {
+  // Split-K for launches that cannot fill the MI355X's 256 CUs (fewer query tiles x heads
+  // than CUs, one ring workgroup per CU): the long tiles' key ranges are cut so that no
+  // piece exceeds the even share of the launch over the CUs, none drops below kMinPiece
+  // key tiles, and no tile splits into more than kMaxSplit pieces. A launch that fills
+  // the chip is not split: its pieces would only add per-workgroup start-up and merge
+  // cost (measured slower on the config-3 batch, 46 + 8 us against 42 us unsplit).
+  constexpr int kCUs = 256, kMinPiece = 8;
+  const int slots = kCUs * kind_per_cu(kind, D);  // workgroups the chip runs at once
+  const int64_t share = (total * H + slots - 1) / slots;
+  const bool underfilled = int64_t(tiles.size()) * H < slots;
+  const int cap = underfilled ? int(std::max<int64_t>(share, kMinPiece)) : INT32_MAX;
+  int n_partials = 0;
+  for (const Tile& t : tiles) {
+    int ns = kind != kStaged && MIATTN_PREFILL_SPLIT ? int((int64_t(t.work) + cap - 1) / cap) : 1;
+    ns = std::max(1, std::min(ns, std::min(kMaxSplit, t.work)));
+    const int w0 = (t.seq << 16) | t.tile;
+    const int slot = ns > 1 ? n_partials : 0;
+    for (int sp = 0; sp < ns; ++sp) {
+      const int work = (sp + 1) * t.work / ns - sp * t.work / ns;
+      pieces.push_back({work, w0, int((uint32_t(sp) << 28) | (uint32_t(ns - 1) << 24) | uint32_t(slot))});
+    }
+    if (ns > 1) {
+      merges.push_back({t.work, w0, int((uint32_t(ns) << 24) | uint32_t(slot))});
+      n_partials += ns;
+    }
+  }
+  if (n_partials >= (1 << 24)) return fail(MI_ERR_UNSUPPORTED, "mi_varlen_schedule: too many split tiles");
+  std::stable_sort(pieces.begin(), pieces.end(), [](const Piece& a, const Piece& b) { return a.work > b.work; });
+  return n_partials;
 }
 
 // Tall kernel schedule: {n_workgroups, n_counters, n_partials, layout}, n_workgroups entries
@@ -2718,10 +2821,8 @@ extern "C" int mi_varlen_schedule_for(const int32_t* host_cu_seqlens, int n_seqs
   if (kind == kTall) {
     return tall_schedule(host_cu_seqlens, n_seqs, H, H_kv, D, causal, host_schedule, capacity);
   }
-  const bool ring = kind != kStaged;  // one workgroup per CU, split-K capable
   const int RW = kind_rows(kind);
   const int BN = kind_keys(kind);
-  struct Tile { int work, seq, tile; };
   std::vector<Tile> tiles;
   int64_t total = 0;
   for (int s = 0; s < n_seqs; ++s) {
@@ -2736,35 +2837,9 @@ extern "C" int mi_varlen_schedule_for(const int32_t* host_cu_seqlens, int n_seqs
       total += work;
     }
   }
-  // Split-K for launches that cannot fill the MI355X's 256 CUs (fewer query tiles x heads
-  // than CUs, one ring workgroup per CU): the long tiles' key ranges are cut so that no
-  // piece exceeds the even share of the launch over the CUs, none drops below kMinPiece
-  // key tiles, and no tile splits into more than kMaxSplit pieces. A launch that fills
-  // the chip is not split: its pieces would only add per-workgroup start-up and merge
-  // cost (measured slower on the config-3 batch, 46 + 8 us against 42 us unsplit).
-  constexpr int kCUs = 256, kMinPiece = 8;
-  const int slots = kCUs * kind_per_cu(kind, D);  // workgroups the chip runs at once
-  const int64_t share = (total * H + slots - 1) / slots;
-  const bool underfilled = int64_t(tiles.size()) * H < slots;
-  const int cap = underfilled ? int(std::max<int64_t>(share, kMinPiece)) : INT32_MAX;
   std::vector<Piece> pieces, merges;
-  int n_partials = 0;
-  for (const Tile& t : tiles) {
-    int ns = ring && MIATTN_PREFILL_SPLIT ? int((int64_t(t.work) + cap - 1) / cap) : 1;
-    ns = std::max(1, std::min(ns, std::min(kMaxSplit, t.work)));
-    const int w0 = (t.seq << 16) | t.tile;
-    const int slot = ns > 1 ? n_partials : 0;
-    for (int sp = 0; sp < ns; ++sp) {
-      const int work = (sp + 1) * t.work / ns - sp * t.work / ns;
-      pieces.push_back({work, w0, int((uint32_t(sp) << 28) | (uint32_t(ns - 1) << 24) | uint32_t(slot))});
-    }
-    if (ns > 1) {
-      merges.push_back({t.work, w0, int((uint32_t(ns) << 24) | uint32_t(slot))});
-      n_partials += ns;
-    }
-  }
-  if (n_partials >= (1 << 24)) return fail(MI_ERR_UNSUPPORTED, "mi_varlen_schedule: too many split tiles");
-  std::stable_sort(pieces.begin(), pieces.end(), [](const Piece& a, const Piece& b) { return a.work > b.work; });
+  const int n_partials = cut_tiles(tiles, total, H, D, kind, pieces, merges);
+  if (n_partials < 0) return n_partials;
   if (kind == kDuo) {
     return duo_schedule(host_cu_seqlens, pieces, merges, n_partials, H, H_kv, D, host_schedule, capacity);
   }
@@ -2861,4 +2936,110 @@ extern "C" int mi_varlen_prefill(const void* q, const void* k, const void* v, vo
   }
   return launch1<f16_t>(D, q, k, v, out, cu_seqlens, schedule, n_work, n_merge, kind, workspace, H,
                         H_kv, sl2, causal, error_word, s);
+}
+
+// The windowed form's schedule and launch. A window (or sinks) past the longest segment hides nothing, so both are
+// held to it; the launch takes the same two numbers (with others the items' key ranges would not be
+// those that the schedule dealt out, which costs balance and nothing else).
+namespace miattn {
+namespace {
+
+int check_window(const char* what, int window, int sinks) {
+  if (window < 1 || sinks < 0) {
+    return fail(MI_ERR_INVALID, "%s: window must be >= 1 and sinks >= 0, got %d and %d", what, window, sinks);
+  }
+  return MI_OK;
+}
+
+}  // namespace
+}  // namespace miattn
+
+extern "C" int mi_varlen_schedule_window(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int D,
+                                         int window, int sinks, int32_t* host_schedule, int capacity) {
+  using namespace miattn;
+  int rc = check_window("mi_varlen_schedule_window", window, sinks);
+  if (rc != MI_OK) return rc;
+  if (D != 64 && D != 128 && D != 256) {
+    return fail(MI_ERR_UNSUPPORTED, "mi_varlen_schedule_window: head_dim 64, 128 or 256, got %d", D);
+  }
+  if (host_cu_seqlens == nullptr || n_seqs < 1 || n_seqs > 65535) {
+    return fail(MI_ERR_INVALID, "mi_varlen_schedule_window: need 1..65535 segments, got %d", n_seqs);
+  }
+  if (H < 1 || H_kv < 1 || H % H_kv != 0) {
+    return fail(MI_ERR_INVALID, "mi_varlen_schedule_window: n_head (%d) must be a multiple of n_kv_head (%d)", H, H_kv);
+  }
+  if (H > 255) return fail(MI_ERR_UNSUPPORTED, "mi_varlen_schedule_window: at most 255 heads, got %d", H);
+  const int BQ = Duo<128>::BQ, BK = Duo<128>::BK;
+  std::vector<Tile> tiles;
+  int64_t total = 0;
+  for (int s = 0; s < n_seqs; ++s) {
+    const int L = host_cu_seqlens[s + 1] - host_cu_seqlens[s];
+    if (L <= 0) return fail(MI_ERR_INVALID, "mi_varlen_schedule_window: segment %d is empty", s);
+    const int n = (L + BQ - 1) / BQ;
+    if (n > 65535) return fail(MI_ERR_UNSUPPORTED, "mi_varlen_schedule_window: segment %d too long", s);
+    for (int t = 0; t < n; ++t) {
+      const int work = band_of(t * BQ, std::min(L, (t + 1) * BQ), std::min(window, L), std::min(sinks, L), BK).n;
+      tiles.push_back({work, s, t});
+      total += work;
+    }
+  }
+  std::vector<Piece> pieces, merges;
+  const int n_partials = cut_tiles(tiles, total, H, D, kDuo, pieces, merges);
+  if (n_partials < 0) return n_partials;
+  return duo_schedule(host_cu_seqlens, pieces, merges, n_partials, H, H_kv, D, host_schedule, capacity, kBand);
+}
+
+extern "C" int mi_varlen_prefill_window(const void* q, const void* k, const void* v, void* out,
+                                        const int32_t* cu_seqlens, int n_seqs, int total_tokens, int max_seqlen,
+                                        const int32_t* schedule, int n_work, int n_merge, int n_partials, int layout,
+                                        int H, int H_kv, int D, float scale, int window, int sinks, int dtype,
+                                        void* workspace, size_t workspace_bytes, int32_t* error_word, void* stream) {
+  using namespace miattn;
+  int rc = check_window("mi_varlen_prefill_window", window, sinks);
+  if (rc != MI_OK) return rc;
+  if (!(scale > 0.0f)) {  // masked scores are -inf before they are scaled
+    return fail(MI_ERR_INVALID, "mi_varlen_prefill_window: scale must be positive, got %g", double(scale));
+  }
+  if (dtype != MI_BF16 && dtype != MI_F16) {
+    return fail(MI_ERR_UNSUPPORTED, "mi_varlen_prefill_window: the MFMA prefill computes fp16/bf16 only (dtype code %d)", dtype);
+  }
+  if (H < 1 || H > 255 || H_kv < 1 || H % H_kv != 0) {
+    return fail(MI_ERR_INVALID, "mi_varlen_prefill_window: n_head (%d, at most 255) must be a multiple of n_kv_head (%d)", H, H_kv);
+  }
+  if (n_seqs < 1 || total_tokens < 1 || max_seqlen < 1 || n_work < 1 || n_work > 65535 || n_merge < 0 ||
+      n_merge > 65535 || n_partials < 0 || (n_merge > 0) != (n_partials > 0)) {
+    return fail(MI_ERR_INVALID, "mi_varlen_prefill_window: bad sizes n_seqs=%d total=%d max_seqlen=%d work=%d merge=%d",
+                n_seqs, total_tokens, max_seqlen, n_work, n_merge);
+  }
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || cu_seqlens == nullptr || schedule == nullptr) {
+    return fail(MI_ERR_INVALID, "mi_varlen_prefill_window: NULL pointer argument");
+  }
+  if ((D != 64 && D != 128 && D != 256) || layout != layout_word(kBand, D, Duo<128>::BQ)) {
+    return fail(MI_ERR_INVALID, "mi_varlen_prefill_window: schedule (layout 0x%x) does not match head_dim %d", layout, D);
+  }
+  const size_t need = partial_bytes(n_partials, H, D, Duo<128>::BQ);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
+    return fail(MI_ERR_WORKSPACE, "mi_varlen_prefill_window: workspace of %zu bytes needed, got %zu", need,
+                workspace == nullptr ? size_t(0) : workspace_bytes);
+  }
+  auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  if (!al(q) || !al(k) || !al(v) || !al(out) || (need > 0 && !al(workspace))) {
+    return fail(MI_ERR_UNSUPPORTED, "mi_varlen_prefill_window: q/k/v/out/workspace must be 16-byte aligned");
+  }
+  if (error_word != nullptr && reinterpret_cast<uintptr_t>(error_word) % 4 != 0) {
+    return fail(MI_ERR_INVALID, "mi_varlen_prefill_window: error_word must be 4-byte aligned");
+  }
+  window = std::min(window, max_seqlen);
+  sinks = std::min(sinks, max_seqlen);
+  const float sl2 = float(double(scale) * 1.4426950408889634);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  auto go = [&](auto type, auto dim) {
+    return launch_window<decltype(type), decltype(dim)::value>(q, k, v, out, cu_seqlens, schedule, n_work, n_merge,
+                                                               workspace, H, H_kv, sl2, window, sinks, error_word, s);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  using D256 = std::integral_constant<int, 256>;
+  if (dtype == MI_BF16) return D == 64 ? go(bf16_t{}, D64{}) : D == 128 ? go(bf16_t{}, D128{}) : go(bf16_t{}, D256{});
+  return D == 64 ? go(f16_t{}, D64{}) : D == 128 ? go(f16_t{}, D128{}) : go(f16_t{}, D256{});
 }

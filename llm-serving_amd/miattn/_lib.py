@@ -157,6 +157,47 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
          _c_int, _p_int64, _c_float, _c_int, _c_void_p, _c_size_t, _c_void_p],
     ),
+    "mi_paged_decode_window": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_int, _p_int64, _c_float, _c_int, _c_int, _c_int, _c_void_p, _c_size_t, _c_void_p],
+    ),
+    "mi_paged_decode_fused_window": (
+        _c_int,
+        [_c_void_p, _c_int64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int, _c_void_p,
+         _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
+         _c_int, _c_int, _c_int, _c_int64, _p_int64, _c_float, _c_float, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+         _c_size_t, _c_void_p, _c_void_p],
+    ),
+    "mi_varlen_schedule_window": (
+        _c_int, [_p_int32, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _p_int32, _c_int]
+    ),
+    "mi_varlen_prefill_window": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
+         _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int,
+         _c_int, _c_void_p, _c_size_t, _c_void_p, _c_void_p],
+    ),
+    "mi_paged_decode_weigh_workspace_size": (_c_size_t, [_c_int] * 7),
+    "mi_paged_decode_weigh": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_int, _p_int64, _c_float, _c_int, _c_void_p, _c_int64, _c_int64, _c_void_p, _c_size_t, _c_void_p],
+    ),
+    "mi_prompt_weights_schedule": (_c_int, [_p_int32, _c_int, _c_int, _c_int, _c_int, _p_int32, _c_int]),
+    "mi_prompt_weights_workspace_size": (_c_size_t, [_p_int32, _c_int]),
+    "mi_prompt_weights": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _p_int32, _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_int64,
+         _c_int64, _c_int, _c_void_p, _c_size_t, _c_void_p],
+    ),
+    "mi_cache_evict_workspace_size": (_c_size_t, [_c_int] * 4),
+    "mi_cache_evict": (
+        _c_int,
+        [_p_void_p, _p_void_p, _c_int, _c_int64, _c_int, _c_int, _c_int, _c_void_p, _c_int64, _c_int, _c_void_p,
+         _c_int64, _c_int, _c_void_p, _c_void_p, _p_int64, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_size_t,
+         _c_void_p, _c_void_p],
+    ),
     "mi_copy_pages": (
         _c_int,
         [_p_void_p, _c_int, _c_int64, _c_int64, _p_int32, _p_int32, _c_int, _c_void_p],

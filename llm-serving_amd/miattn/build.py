@@ -37,7 +37,8 @@ HIPCC_FLAGS = [
 ]
 
 SOURCES = ["capi.hip", "slot_write.hip", "paged_decode.hip", "varlen_prefill.hip", "decode_epilogue.hip",
-           "decode_step.hip", "rows_gemm.hip", "fp4_cache.hip", "paged_decode_fp4.hip", "copy_pages.hip"]
+           "decode_step.hip", "rows_gemm.hip", "fp4_cache.hip", "paged_decode_fp4.hip", "copy_pages.hip",
+           "paged_decode_window.hip", "paged_decode_weigh.hip", "prompt_weights.hip", "cache_evict.hip"]
 
 
 def _hipcc() -> str:

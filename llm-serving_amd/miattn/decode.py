@@ -10,6 +10,10 @@ Public surface (names, signatures, ownership and exception split as in the refer
   :class:`PagedDecodePlan`, whose ``run(layer, q)`` launches one layer. The plan checks all
   layers once and afterwards only the query of each call; it keeps the pools, the table
   and ``seqlen`` by reference, so in-place ``seqlen`` updates between steps are seen;
+* ``window=`` and ``sinks=`` on both (no reference counterpart) -- each row's query sees its last ``window``
+  tokens and its first ``sinks`` only; the other tokens' pages are not read;
+* ``PagedDecodePlan.run_weighed(layer, q, weights)`` -- :meth:`~PagedDecodePlan.run`, which also adds each token's
+  attention weights to an account, for ``PagedPool.evict`` (no reference counterpart either);
 * ``TRITON_AVAILABLE`` -- the flag the reference's callers import. It names the decode
   backend being present, which here means ``libmiattn.so`` loaded.
 
@@ -34,7 +38,7 @@ from types import SimpleNamespace
 import torch
 
 from . import _lib
-from ._contract import Rule, enforce, is_pow2
+from ._contract import Rule, as_index, enforce, is_pow2
 
 __all__ = ["TRITON_AVAILABLE", "HIP_AVAILABLE", "paged_decode", "paged_decode_plan", "PagedDecodePlan"]
 
@@ -193,6 +197,23 @@ def _check(q, k_cache, v_cache, block_table, seqlen) -> DecodeGeometry:
     return g
 
 
+def check_window(window, sinks) -> tuple[int, int] | None:
+    """``(window, sinks)`` as the C calls take them, None for attention over the whole row."""
+    sinks = as_index(sinks, "sinks")
+    if sinks < 0:
+        raise ValueError(f"sinks must be >= 0, got {sinks}")
+    if window is None:
+        if sinks:
+            raise ValueError(f"sinks={sinks} needs a window: without one every token is seen")
+        return None
+    if isinstance(window, bool) or as_index(window, "window") < 1:
+        raise ValueError(f"window must be a positive int or None, got {window!r}")
+    return min(as_index(window, "window"), _MOST_INT), min(sinks, _MOST_INT)
+
+
+_MOST_INT = 2**31 - 1
+
+
 def _workspace_bytes(g: DecodeGeometry, dtype: torch.dtype) -> int:
     return int(_lib.lib.mi_paged_decode_workspace_size(*g.dims(), _lib.dtype_code(dtype)))
 
@@ -206,9 +227,12 @@ def _launch(g: DecodeGeometry, q, k_ptr: int, v_ptr: int, table_ptr: int, seqlen
     _lib.check(rc, what)
 
 
-def paged_decode(q, k_cache, v_cache, block_table, seqlen, *, scale: float | None = None):
+def paged_decode(q, k_cache, v_cache, block_table, seqlen, *, scale: float | None = None, window: int | None = None,
+                 sinks: int = 0):
     """Decode one query token per row against a paged KV pool (reference
-    ``model/triton_decode.py:250-328``)."""
+    ``model/triton_decode.py:250-328``). With ``window``, row ``b`` sees its last ``window`` tokens (the last is the
+    query's own) and its first ``sinks``; table entries of blocks without a seen token are not read."""
+    band = check_window(window, sinks)
     _require_backend()
     _require_device_tensors((("q", q), ("k_cache", k_cache), ("v_cache", v_cache),
                              ("block_table", block_table), ("seqlen", seqlen)))
@@ -224,6 +248,15 @@ def paged_decode(q, k_cache, v_cache, block_table, seqlen, *, scale: float | Non
                                 table.stride(0)))
     n_ws = _workspace_bytes(g, q.dtype)
     ws = torch.empty(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
+    if band is not None:
+        with _lib.on_device(q.device):
+            rc = _lib.lib.mi_paged_decode_window(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lens.data_ptr(), out.data_ptr(),
+                *g.dims(), strides, float(1.0 / math.sqrt(g.head_dim) if scale is None else scale),
+                _lib.dtype_code(q.dtype), *band, None if ws is None else ws.data_ptr(), n_ws,
+                _lib.current_stream(q.device))
+        _lib.check(rc, "paged_decode")
+        return out
     _launch(g, q, k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lens.data_ptr(), out, strides,
             float(1.0 / math.sqrt(g.head_dim) if scale is None else scale),
             None if ws is None else ws.data_ptr(), n_ws, "paged_decode")
@@ -259,13 +292,16 @@ class PagedDecodePlan:
     and requires them to share one shape and one stride layout; it then freezes the
     launch arguments (geometry, stride block, scale, workspace). ``run`` only compares
     the query against the layout it was built for. Pools, table and ``seqlen`` are held
-    by reference.
+    by reference. With ``window``, every run is under that window with its ``sinks``
+    (:func:`paged_decode`).
     """
 
     __slots__ = ("n_layer", "geometry", "q_signature", "_k_ptrs", "_v_ptrs", "_pools",
-                 "_table", "_seqlen", "_strides", "_scale", "_ws", "_ws_bytes", "_frozen")
+                 "_table", "_seqlen", "_strides", "_scale", "_ws", "_ws_bytes", "_frozen", "_band", "_banded",
+                 "_weigh_ws", "_weigh_shape")
 
-    def __init__(self, q, k_caches, v_caches, block_table, seqlen, *, scale=None) -> None:
+    def __init__(self, q, k_caches, v_caches, block_table, seqlen, *, scale=None, window=None, sinks=0) -> None:
+        self._band = check_window(window, sinks)
         _require_backend()
         _require_device_tensors((("q", q), ("block_table", block_table), ("seqlen", seqlen)))
         ks, vs = list(k_caches), list(v_caches)
@@ -294,6 +330,9 @@ class PagedDecodePlan:
         # the launch arguments after ``out`` that no run changes (the plan owns the workspace)
         self._frozen = (*g.dims(), self._strides, self._scale, _lib.dtype_code(q.dtype),
                         None if self._ws is None else self._ws.data_ptr(), self._ws_bytes)
+        self._banded = None if self._band is None else (*self._frozen[:-2], *self._band, *self._frozen[-2:])
+        self._weigh_ws = None  # run_weighed's workspace, taken at its first call
+        self._weigh_shape = torch.Size((g.rows, g.kv_heads, g.capacity))
 
     def run(self, layer: int, q):
         """Launch one layer; ``q`` must have the layout the plan was built with."""
@@ -308,10 +347,53 @@ class PagedDecodePlan:
             )
         out = torch.empty_like(q)
         layer = int(layer)
+        if self._banded is not None:
+            with _lib.on_device(q.device):
+                rc = _lib.lib.mi_paged_decode_window(
+                    q.data_ptr(), self._k_ptrs[layer], self._v_ptrs[layer], self._table.data_ptr(),
+                    self._seqlen.data_ptr(), out.data_ptr(), *self._banded, _lib.current_stream(q.device))
+            if rc:
+                _lib.check(rc, "paged_decode_plan.run")
+            return out
         rc = _lib.lib.mi_paged_decode(q.data_ptr(), self._k_ptrs[layer], self._v_ptrs[layer], self._table.data_ptr(),
                                       self._seqlen.data_ptr(), out.data_ptr(), *self._frozen,
                                       _lib.current_stream(q.device))
         _lib.check(rc, "paged_decode_plan.run")
+        return out
+
+    def run_weighed(self, layer: int, q, weights: torch.Tensor) -> torch.Tensor:
+        """:meth:`run`, and the attention weights of each token added to an account: ``weights[b, kv, t]`` (fp32,
+        ``(B, n_kv_head, width * block_size)``, last dimension contiguous) gains the sum over the query heads
+        of ``kv`` of their softmax weights on token ``t``, for ``t < seqlen[b]``; later entries stay as they are.
+        ``head_dim`` 32 to 256. The output is :meth:`run`'s up to the order of its sums. The scores of a
+        call wait in a workspace of the plan's own (4 bytes per token of the tables and query head, taken at
+        the first call), so weighed runs, too, stay ordered on one stream. A plan under a window does not weigh."""
+        layer = int(layer)
+        if not 0 <= layer < self.n_layer:
+            raise IndexError(f"layer {layer} is outside the plan's {self.n_layer} layers")
+        if self._band is not None:
+            raise ValueError("run_weighed accounts for every token of a row; this plan is under a window")
+        signature = (tuple(q.shape), q.dtype, q.device, q.stride())
+        if signature != self.q_signature:
+            raise ValueError("paged_decode_plan.run_weighed: the query does not match the validated layout "
+                             f"(built for shape/dtype/device/strides {self.q_signature}, got {signature}); "
+                             "build a new plan for a new layout")
+        if (weights.shape != self._weigh_shape or weights.dtype != torch.float32 or weights.stride(2) != 1
+                or weights.device != q.device):
+            raise ValueError(f"weights must be fp32 {tuple(self._weigh_shape)} on {q.device} with contiguous rows, got "
+                             f"{weights.dtype} {tuple(weights.shape)} strides {weights.stride()} on {weights.device}")
+        with _lib.on_device(q.device):
+            if self._weigh_ws is None:
+                n = int(_lib.lib.mi_paged_decode_weigh_workspace_size(*self.geometry.dims(), self._frozen[8]))
+                self._weigh_ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+            out = torch.empty_like(q)
+            ws = self._weigh_ws
+            rc = _lib.lib.mi_paged_decode_weigh(
+                q.data_ptr(), self._k_ptrs[layer], self._v_ptrs[layer], self._table.data_ptr(), self._seqlen.data_ptr(),
+                out.data_ptr(), *self._frozen[:-2], weights.data_ptr(), weights.stride(0), weights.stride(1),
+                ws.data_ptr(), ws.numel(), _lib.current_stream(q.device))
+        if rc:
+            _lib.check(rc, "paged_decode_plan.run_weighed")
         return out
 
     def fused_supported(self, dtype: torch.dtype, rotary_dim: int, zero_centred_norm: bool = False) -> bool:
@@ -361,19 +443,22 @@ class PagedDecodePlan:
             raise ValueError("pos must be int64 (B,) and slot_ids int32/int64 (B,)")
         out = torch.empty(self.q_signature[0], dtype=dtype, device=self.q_signature[2])
         k, v = self._pools[0][layer], self._pools[1][layer]
-        rc = _lib.lib.mi_paged_decode_fused(
+        fused, band = (_lib.lib.mi_paged_decode_fused, ()) if self._band is None else \
+            (_lib.lib.mi_paged_decode_fused_window, self._band)
+        rc = fused(
             source.data_ptr(), row_stride, n_parts, q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(),
             sin.data_ptr(), int(cos.shape[0]), rotary, pos.data_ptr(), slot_ids.data_ptr(),
             8 * slot_ids.element_size(), k.data_ptr(), v.data_ptr(), self._table.data_ptr(), self._seqlen.data_ptr(),
             out.data_ptr(), *g.dims(), int(k.shape[0]) * int(k.shape[1]), self._strides, self._scale, float(eps), 0,
-            _lib.dtype_code(dtype), None if self._ws is None else self._ws.data_ptr(), self._ws_bytes,
+            _lib.dtype_code(dtype), *band, None if self._ws is None else self._ws.data_ptr(), self._ws_bytes,
             None if error_word is None else error_word.data_ptr(), _lib.current_stream(out.device),
         )
         _lib.check(rc, "paged_decode_plan.run_fused")
         return out
 
 
-def paged_decode_plan(q, k_caches, v_caches, block_table, seqlen, *, scale=None) -> PagedDecodePlan:
+def paged_decode_plan(q, k_caches, v_caches, block_table, seqlen, *, scale=None, window: int | None = None,
+                      sinks: int = 0) -> PagedDecodePlan:
     """Check one container's decode tensors once and freeze their launch arguments
-    (reference ``model/triton_decode.py:523-538``)."""
-    return PagedDecodePlan(q, k_caches, v_caches, block_table, seqlen, scale=scale)
+    (reference ``model/triton_decode.py:523-538``); ``window`` and ``sinks`` as for :func:`paged_decode`."""
+    return PagedDecodePlan(q, k_caches, v_caches, block_table, seqlen, scale=scale, window=window, sinks=sinks)

@@ -172,7 +172,10 @@ class Fp4PagedPool(PagedPool):
                 B, H, *self._sizes, float(eps), int(bool(zero_centred_norm)), self._code, self._write_error.data_ptr(),
                 _lib.current_stream(self._home))
 
-    def decode_plan(self, q, block_table, seqlen, *, scale=None) -> "Fp4DecodePlan":
+    def decode_plan(self, q, block_table, seqlen, *, scale=None, window: int | None = None,
+                    sinks: int = 0) -> "Fp4DecodePlan":
+        if window is not None or sinks:
+            raise ValueError("the attention over a 4-bit pool has no window: it sees whole rows")
         return paged_decode_fp4_plan(q, self.keys, self.values, block_table, seqlen, scale=scale)
 
     def bytes(self) -> int:

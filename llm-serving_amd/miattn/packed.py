@@ -218,14 +218,25 @@ class PackedPrefill:
                                     k_out=k, v_out=v, rotary_dim=rotary_dim, zero_centred_norm=zero_centred_norm)
         return q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
 
-    def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+    def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None,
+               sinks: int = 0) -> torch.Tensor:
         """Causal attention inside each request over the packed axis (reference
-        ``model/packed.py:204-218``)."""
+        ``model/packed.py:204-218``), under a window with sinks where one is given."""
         if q.dim() != 4 or q.shape[0] != 1 or q.shape[1] != self.total_tokens:
             raise ValueError(f"attend needs packed (1, {self.total_tokens}, H, D) q, got {tuple(q.shape)}")
         out = self.backend.prefill_varlen(q[0].contiguous(), k[0].contiguous(), v[0].contiguous(),
-                                          cu_seqlens=self.cu_seqlens, max_seqlen=self.max_seqlen, causal=True)
+                                          cu_seqlens=self.cu_seqlens, max_seqlen=self.max_seqlen, causal=True,
+                                          **({} if window is None and not sinks else {"window": window, "sinks": sinks}))
         return out.unsqueeze(0)
+
+    def weigh(self, q: torch.Tensor, k: torch.Tensor, *, observe: int | None = 32, out: torch.Tensor | None = None):
+        """Where each request's last ``observe`` queries look, ``(n_seqs, n_kv_head, max_seqlen)``
+        (``HipVarlen.prompt_weights`` over :meth:`write_rope`'s packed q and k)."""
+        if q.dim() != 4 or q.shape[0] != 1 or q.shape[1] != self.total_tokens or k.dim() != 4 or k.shape[0] != 1:
+            raise ValueError(f"weigh needs packed (1, {self.total_tokens}, heads, D) q and k, got {tuple(q.shape)} / "
+                             f"{tuple(k.shape)}")
+        return self.backend.prompt_weights(q[0], k[0], cu_seqlens=self.cu_seqlens, max_seqlen=self.max_seqlen,
+                                           observe=observe, out=out)
 
     @property
     def backend_name(self) -> str:

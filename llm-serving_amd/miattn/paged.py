@@ -35,8 +35,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._contract import Rule, enforce, positive_int, same_device
-from .decode import TRITON_AVAILABLE, paged_decode_plan
+from ._contract import Rule, as_index, enforce, is_pow2, positive_int, same_device
+from .decode import TRITON_AVAILABLE, check_window, paged_decode_plan
 from .rows import Parts
 
 __all__ = ["PagedPool", "PagedKV", "PagedWriteSink"]
@@ -64,6 +64,36 @@ _WRITE_SLOTS = _kv_rules("write_slots") + (
 )
 
 _WRITE_PREFILL = _kv_rules("write_prefill")
+
+_EVICT = (
+    Rule(lambda a: a.pool._store_layout()[0][-1] != a.pool.head_dim, ValueError,
+         lambda a: "evict moves rows of a pool that holds them in its dtype; a 4-bit pool's stay where they are"),
+    Rule(lambda a: a.budget < 1 or a.recent < 0 or a.sinks < 0 or a.recent + a.sinks > a.budget, ValueError,
+         lambda a: f"budget ({a.budget}) must be positive and hold recent ({a.recent}) + sinks ({a.sinks}), all >= 0"),
+    Rule(lambda a: any(t.dim() != 2 or t.dtype != torch.int32 or t.stride(1) != 1 for t in (a.table, a.to)), ValueError,
+         lambda a: "block_table and to must be int32 (B, blocks) tables with contiguous rows, got "
+                   f"{a.table.dtype} {tuple(a.table.shape)} and {a.to.dtype} {tuple(a.to.shape)}"),
+    Rule(lambda a: a.table.shape[1] < 1 or a.to.shape[0] != a.table.shape[0], ValueError,
+         lambda a: f"to must have a row for each of block_table's, got {tuple(a.to.shape)} for {tuple(a.table.shape)}"),
+    Rule(lambda a: a.to.shape[1] * a.pool.block_size < min(a.budget, a.table.shape[1] * a.pool.block_size), ValueError,
+         lambda a: f"to has {a.to.shape[1]} blocks of {a.pool.block_size} per row, too few for {a.budget} tokens"),
+    Rule(lambda a: a.seqlen.dtype != torch.int32 or a.seqlen.shape != a.table.shape[:1] or not a.seqlen.is_contiguous(),
+         ValueError, lambda a: f"seqlen must be a contiguous int32 tensor of {a.table.shape[0]} lengths (it is updated in "
+                               f"place), got {a.seqlen.dtype} {tuple(a.seqlen.shape)}"),
+    Rule(lambda a: a.weights.dtype != torch.float32 or tuple(a.weights.shape) != (
+        a.pool.n_layer, a.table.shape[0], a.pool.n_kv_head, a.table.shape[1] * a.pool.block_size)
+        or a.weights.stride(3) != 1, ValueError,
+         lambda a: f"weights must be fp32 ({a.pool.n_layer}, {a.table.shape[0]}, {a.pool.n_kv_head}, "
+                   f"{a.table.shape[1] * a.pool.block_size}) with contiguous rows, got {a.weights.dtype} "
+                   f"{tuple(a.weights.shape)}"),
+    Rule(lambda a: not all(same_device(t.device, a.pool.device) for t in (a.table, a.to, a.seqlen, a.weights)), ValueError,
+         lambda a: f"the pool is on {a.pool.device}; got block_table on {a.table.device}, to on {a.to.device}, seqlen on "
+                   f"{a.seqlen.device}, weights on {a.weights.device}"),
+    Rule(lambda a: a.pool._on_device and not (is_pow2(a.pool.head_dim * a.pool.dtype.itemsize)
+                                              and 16 <= a.pool.head_dim * a.pool.dtype.itemsize <= 1024), ValueError,
+         lambda a: f"evict on a HIP pool moves rows of 16 to 1024 bytes, a power of two; head_dim {a.pool.head_dim} in "
+                   f"{a.pool.dtype} is not"),
+)
 
 
 class PagedPool:
@@ -94,7 +124,7 @@ class PagedPool:
         # device word: 1 + index of the first token a HIP write skipped, 0 when none
         self._write_error = torch.zeros(1, dtype=torch.int32, device=self.device) if self._on_device else None
         self._slot_memo: tuple[tuple, torch.Tensor] | None = None
-        self._copy_stores: tuple[list[torch.Tensor], array] = ([], array("Q"))  # that copy_blocks has looked over
+        self._copy_stores: tuple[list[torch.Tensor], array] = ([], array("Q"))  # that _check_stores has looked over
 
     def _check_storage(self) -> None:
         """What a pool of another storage requires of its sizes, dtype and device."""
@@ -342,11 +372,7 @@ class PagedPool:
                 store[b] = store[a]
             return
         _lib.require_library("PagedPool.copy_blocks on a HIP pool")
-        addresses = array("Q", map(torch.Tensor.data_ptr, stores))
-        known, at = self._copy_stores
-        if len(known) != len(stores) or not all(map(is_, stores, known)) or at != addresses:
-            self._check_copy_stores(stores)
-            self._copy_stores = (stores, addresses)
+        addresses = self._addresses(stores, "copy_blocks")
         pools = (ctypes.c_void_p * len(stores)).from_buffer(addresses)
         page = stores[0].stride(0) * stores[0].element_size()
         with _lib.on_device(self.keys[0].device):
@@ -355,21 +381,108 @@ class PagedPool:
                                         _lib.current_stream(self.keys[0].device))
         _lib.check(rc, "PagedPool.copy_blocks")
 
-    def _check_copy_stores(self, stores) -> None:
-        """The page copy takes addresses: what ``keys`` and ``values`` hold has to be the pool's layout, on one device."""
+    def _check_stores(self, stores, what: str) -> None:
+        """Kernels that take every layer take addresses: what ``keys`` and ``values`` hold has to be the pool's layout, on one device."""
         shape, dtype = self._store_layout()
         for t in stores:
             if tuple(t.shape) != shape or t.dtype != dtype:
-                raise ValueError(f"copy_blocks needs keys and values of shape {shape} and {dtype}, got {tuple(t.shape)} {t.dtype}")
+                raise ValueError(f"{what} needs keys and values of shape {shape} and {dtype}, got {tuple(t.shape)} {t.dtype}")
             if not t.is_contiguous():
-                raise ValueError("copy_blocks needs contiguous keys and values")
+                raise ValueError(f"{what} needs contiguous keys and values")
         for t in stores:
             if not t.is_cuda or t.device != stores[0].device:
-                raise ValueError(f"copy_blocks on a HIP pool needs every store on its device, got one on {t.device}")
+                raise ValueError(f"{what} on a HIP pool needs every store on its device, got one on {t.device}")
 
-    def decode_plan(self, q, block_table, seqlen, *, scale=None):
+    # ------------------------------------------------------------------ eviction
+    def evict(self, block_table: torch.Tensor, seqlen: torch.Tensor, weights: torch.Tensor, *, budget: int, recent: int,
+              sinks: int = 0, to: torch.Tensor | None = None) -> None:
+        """Cut every row longer than ``budget`` tokens to it, in every layer, by the weight that attention gave its tokens.
+
+        Per layer, row and KV head, the first ``sinks`` tokens, the last ``recent`` and the heaviest of the others (NaN
+        above every number; of equal ones the lowest index) stay, in their order: their K and V rows and their
+        entries of ``weights`` move up to places ``0 .. budget - 1``, the entries behind them become 0, and
+        ``seqlen`` (int32 ``(B,)``) becomes ``min(seqlen, budget)``, all in place. ``weights`` is the account
+        that ``PagedDecodePlan.run_weighed`` and ``HipVarlen.prompt_weights`` fill: fp32
+        ``(n_layer, B, n_kv_head, width * block_size)``, last dimension contiguous. K rows keep the rotation of
+        the positions that they were written at, so a caller counts positions apart from ``seqlen`` from then on.
+
+        ``block_table`` (int32 ``(B, width)``): without ``to`` the rows stay in its blocks (those past the budget are free
+        afterwards); a block may be in one row only. ``to`` (int32 ``(B, blocks for min(budget, capacity)
+        tokens)``): every row, also one within the budget, is written to these blocks, in none of which a row
+        of ``block_table`` lies, and its old ones stay as they are (shared blocks of a fork, say). No host
+        wait; a row whose tables name a block outside the pool loses those tokens and is reported by
+        :meth:`check_writes` (as token ``b``)."""
+        budget, recent, sinks = (as_index(x, n) for x, n in ((budget, "budget"), (recent, "recent"), (sinks, "sinks")))
+        target = block_table if to is None else to
+        enforce(_EVICT, SimpleNamespace(pool=self, table=block_table, to=target, seqlen=seqlen, weights=weights,
+                                        budget=budget, recent=recent, sinks=sinks))
+        if block_table.shape[0] == 0:
+            return
+        if not self._on_device:
+            self._evict_host(block_table, target, seqlen, weights, budget, recent, sinks)
+            return
+        _lib.require_library("PagedPool.evict on a HIP pool")
+        stores = self.keys + self.values
+        addresses = self._addresses(stores, "evict")
+        n, capacity = self.n_layer, block_table.shape[1] * self.block_size
+        budget = min(budget, capacity)  # a row holds no more
+        sinks = min(sinks, budget)
+        recent = min(recent, budget - sinks)
+        with _lib.on_device(self.keys[0].device):
+            n_ws = int(_lib.lib.mi_cache_evict_workspace_size(n, block_table.shape[0], self.n_kv_head, budget))
+            ws = torch.empty(n_ws, dtype=torch.uint8, device=block_table.device)
+            rc = _lib.lib.mi_cache_evict(
+                (ctypes.c_void_p * n).from_buffer(addresses), (ctypes.c_void_p * n).from_buffer(addresses, 8 * n), n,
+                self.n_blocks, self.block_size, self.n_kv_head, self.head_dim * self.dtype.itemsize,
+                block_table.data_ptr(), block_table.stride(0), block_table.shape[1], target.data_ptr(), target.stride(0),
+                target.shape[1], seqlen.data_ptr(), weights.data_ptr(), _lib.int64_array(weights.stride()[:3]),
+                block_table.shape[0], budget, recent, sinks, ws.data_ptr(), n_ws, self._write_error.data_ptr(),
+                _lib.current_stream(self.keys[0].device))
+        _lib.check(rc, "PagedPool.evict")
+        if self.strict_writes:
+            self.check_writes()
+
+    def _evict_host(self, table, to, seqlen, weights, budget: int, recent: int, sinks: int) -> None:
+        bs = self.block_size
+        heads = torch.arange(self.n_kv_head)
+        for b, n in enumerate(seqlen.tolist()):
+            n = max(0, min(n, table.shape[1] * bs))
+            keep = min(n, budget)
+            if keep == 0 or (n == keep and to is table):
+                continue
+            slot, index = torch.arange(keep), np.arange(n)
+            protected = (index < sinks) | (index >= n - recent)
+            page = to[b].long()[slot // bs]
+            for i in range(self.n_layer):
+                kept = slot.expand(self.n_kv_head, keep)
+                if n > keep:
+                    w = weights[i, b, :, :n].numpy()
+                    nan = np.isnan(w)
+                    value = np.where(nan, 0, w)
+                    # the last key sorts first: protected ones, NaN, the heavier, the earlier
+                    order = [np.lexsort((index, -value[h], ~nan[h], ~protected)) for h in range(self.n_kv_head)]
+                    kept = torch.from_numpy(np.sort(np.stack(order)[:, :keep], axis=-1))
+                source = table[b].long()[kept // bs]  # (heads, keep)
+                for store in (self.keys[i], self.values[i]):
+                    store[page, slot % bs] = store[source, kept % bs, heads.unsqueeze(1)].transpose(0, 1)
+                if n > keep:
+                    held = torch.gather(weights[i, b], 1, kept)
+                    weights[i, b, :, keep:n] = 0
+                    weights[i, b, :, :keep] = held
+            seqlen[b] = keep
+
+    def _addresses(self, stores, what: str) -> array:
+        """The stores' addresses, after a look at their layout where they are others than the last call's."""
+        addresses = array("Q", map(torch.Tensor.data_ptr, stores))
+        known, at = self._copy_stores
+        if len(known) != len(stores) or not all(map(is_, stores, known)) or at != addresses:
+            self._check_stores(stores, what)
+            self._copy_stores = (stores, addresses)
+        return addresses
+
+    def decode_plan(self, q, block_table, seqlen, *, scale=None, window: int | None = None, sinks: int = 0):
         """The decode plan of this pool's layers (``paged_decode_plan`` over ``keys`` and ``values``)."""
-        return paged_decode_plan(q, self.keys, self.values, block_table, seqlen, scale=scale)
+        return paged_decode_plan(q, self.keys, self.values, block_table, seqlen, scale=scale, window=window, sinks=sinks)
 
     # ------------------------------------------------------------------ accounting
     def bytes(self) -> int:
@@ -391,6 +504,9 @@ class PagedKV:
     the decode kernel; ``seqlen`` is an int32 vector refreshed in place each step, so the
     container's launch plan (built at the first ``attend``) sees every step.
 
+    ``window`` and ``sinks`` (no reference counterpart): every ``attend`` is under that window
+    (:func:`~miattn.decode.paged_decode`).
+
     Step protocol::
 
         kv.build_mask(next_token=True)   # seqlen := pos + 1
@@ -404,7 +520,9 @@ class PagedKV:
     block_table_decode = True
 
     def __init__(self, pool: PagedPool, block_tables, lengths, *, rope_len: int, seats=None,
-                 n_head: int | None = None, check_bounds: bool = True) -> None:
+                 n_head: int | None = None, check_bounds: bool = True, window: int | None = None,
+                 sinks: int = 0) -> None:
+        self.band = check_window(window, sinks)
         if not isinstance(pool, PagedPool):
             raise TypeError(f"PagedKV needs a PagedPool, got {type(pool).__name__}")
         if pool.device.type != "cuda":
@@ -541,7 +659,9 @@ class PagedKV:
             raise ValueError(f"attend needs q {want}, got {tuple(q.shape)}")
         q3 = q.squeeze(2).contiguous()
         if self._plan is None:
-            self._plan = self.pool.decode_plan(q3, self._block_table_tensor, self._seqlen, scale=self.head_dim ** -0.5)
+            window, sinks = (None, 0) if self.band is None else self.band
+            self._plan = self.pool.decode_plan(q3, self._block_table_tensor, self._seqlen, scale=self.head_dim ** -0.5,
+                                               window=window, sinks=sinks)
         return self._plan.run(layer, q3).unsqueeze(2)
 
     def advance(self) -> None:

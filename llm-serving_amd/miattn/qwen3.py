@@ -30,12 +30,13 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
+from .decode import check_window
 from .fp4 import Fp4PagedPool
 from .packed import PackedPrefill
 from .paged import PagedKV, PagedPool
 from .rows import Parts, argmax_rows, glu_weight, rows_linear, rows_supported, rows_swiglu, rows_tile_best
 
-__all__ = ["Qwen3Config", "random_weights", "Qwen3", "GraphDecoder"]
+__all__ = ["Qwen3Config", "random_weights", "Qwen3", "GraphDecoder", "BudgetDecoder"]
 
 
 @dataclass(frozen=True)
@@ -52,6 +53,8 @@ class Qwen3Config:
     eps: float = 1e-6
     rope_theta: float = 1e6
     std: float = 0.02
+    window: int | None = None  # attention sees a query's last `window` tokens and the first `sinks` (None: all)
+    sinks: int = 0
 
 
 def random_weights(cfg: Qwen3Config, seed: int, dtype=torch.bfloat16) -> dict:
@@ -241,13 +244,15 @@ class Qwen3:
                     n_head=c.n_head)
 
     # ------------------------------------------------------------------ prefill
-    def prefill(self, prompts: list[list[int]], pool: PagedPool, tables: list[list[int]]) -> torch.Tensor:
+    def prefill(self, prompts: list[list[int]], pool: PagedPool, tables: list[list[int]], *,
+                weights: torch.Tensor | None = None, observe: int | None = 32) -> torch.Tensor:
         """Packed prefill of whole prompts (reference ``MiniLLM.forward`` packed branch,
         ``model/minillm.py:76-106``); writes every layer's K/V into ``pool`` through the
         requests' block tables and returns the last-token logits ``(n_prompts, vocab)``.
         Projections are ``F.linear`` (thousands of rows); q/k norm + RoPE + the K/V write, each
         residual add with the next RMSNorm and SiLU * up are one HIP launch each, as in
-        decode."""
+        decode. ``weights`` (fp32 ``(n_layer, n_prompts, n_kv_head, at least the longest prompt)``) is filled with
+        where each prompt's last ``observe`` queries look, per layer (``PackedPrefill.weigh``)."""
         c = self.cfg
         packed, tokens = PackedPrefill.upload(prompts, pool, tables, self.device)
         x = F.embedding(tokens, self.w["embed"])  # (T, C), the residual stream (updated in place)
@@ -258,7 +263,9 @@ class Qwen3:
             # q/k norm + RoPE + the group's K/V write in one launch over one stacked projection
             q, k, v = packed.write_rope(i, F.linear(h, self.w[p + "wqkv"]), self.w[p + "qn"], self.w[p + "kn"],
                                         self.cos, self.sin, c.eps)
-            y = packed.attend(q, k, v)
+            y = packed.attend(q, k, v, window=c.window, sinks=c.sinks)
+            if weights is not None:
+                packed.weigh(q, k, observe=observe, out=weights[i])
             _, h = add_rms_norm(x, F.linear(y.reshape(T, -1), self.w[p + "wo"]), self.w[p + "ln2"], c.eps)
             m = silu_mul(F.linear(h, self.w[p + "wgu"]))
             nxt = self.w[f"l{i + 1}.ln1"] if i + 1 < c.n_layer else self.w["norm"]
@@ -311,6 +318,9 @@ class Qwen3:
         """One decode step of every row (reference ``MiniLLM.forward`` decode-container
         branch, ``model/minillm.py:111-136``); returns logits ``(B, vocab)``."""
         c = self.cfg
+        if paged.band != check_window(c.window, c.sinks):
+            raise ValueError(f"the model's window is {c.window} with {c.sinks} sinks, the container's (window, sinks) "
+                             f"{paged.band}: build the PagedKV with the model's")
         paged.build_mask(next_token=True)
         x = F.embedding(tokens.view(-1), self.w["embed"])  # (B, C)
         B = x.shape[0]
@@ -363,7 +373,8 @@ class GraphDecoder:
         self.max_new = max_new
         self.B = B
         q0 = torch.zeros(B, c.n_head, c.head_dim, dtype=model.dtype, device=dev)
-        self.plan = pool.decode_plan(q0, self.table, self.seqlen, scale=1.0 / math.sqrt(c.head_dim))
+        self.plan = pool.decode_plan(q0, self.table, self.seqlen, scale=1.0 / math.sqrt(c.head_dim), window=c.window,
+                                     sinks=c.sinks)
         # q/k norm + RoPE + K/V write fused into the decode launch where the shape allows
         self.fused = self.plan.fused_supported(model.dtype, 2 * int(model.cos.shape[-1]))
         self.graph = None
@@ -431,4 +442,109 @@ class GraphDecoder:
             except IndexError:
                 pass
             raise IndexError(f"row {bad - 1}: token or position out of range in a decode step; the row was skipped")
+        self.pool.check_writes()
+
+
+class BudgetDecoder:
+    """Greedy decode steps of a fixed batch whose rows hold a bounded number of tokens, a step replayed from a graph.
+
+    A row grows to ``budget + every`` tokens; then ``PagedPool.evict`` cuts it back to ``budget`` (per layer and KV head:
+    the first ``sinks`` tokens, the last ``recent`` and those that attention gave the most weight). ``weights``
+    ``(n_layer, B, n_kv_head, table capacity)`` is the account: filled by ``Qwen3.prefill(weights=...)``,
+    grown by every step (``PagedDecodePlan.run_weighed``). A token's rotation is that of its position in the
+    text (``pos``); its place in the cache (``held``) is counted apart. ``tables`` hold the prompts and at least ``budget
+    + every`` tokens; prompts past the budget are cut before the first step.
+    """
+
+    def __init__(self, model: Qwen3, pool: PagedPool, tables: list[list[int]], lengths: list[int],
+                 first_tokens: torch.Tensor, max_new: int, weights: torch.Tensor, *, budget: int, recent: int,
+                 sinks: int = 0, every: int = 64) -> None:
+        c, dev = model.cfg, model.device
+        if c.window is not None:
+            raise ValueError("a model under a window sees a bounded number of tokens by itself")
+        self.model, self.pool, self.weights = model, pool, weights
+        self.budget, self.recent, self.sinks, self.every = int(budget), int(recent), int(sinks), int(every)
+        if self.every < 1:
+            raise ValueError(f"every must be >= 1, got {every}")
+        self.B = len(tables)
+        width = max(len(t) for t in tables)
+        for t, n in zip(tables, lengths):
+            most = max(n, min(n + max_new, self.budget + self.every))
+            if len(t) * pool.block_size < most:
+                raise ValueError(f"block table of {len(t)} blocks cannot hold the {most} tokens that a row grows to")
+        bt = torch.full((self.B, width), -1, dtype=torch.int32)
+        for r, t in enumerate(tables):
+            bt[r, : len(t)] = torch.tensor(t, dtype=torch.int32)
+        self.table = bt.to(dev)
+        self.pos = torch.tensor(lengths, dtype=torch.long, device=dev)
+        self.held = self.pos.clone()  # the place of the next token in the row's cache
+        self.seqlen = self.pos.to(torch.int32)
+        self.tokens = first_tokens.to(dev, torch.long).clone()
+        self.history = torch.zeros(self.B, max_new, dtype=torch.long, device=dev)
+        self.step_idx = torch.zeros(self.B, dtype=torch.long, device=dev)
+        self.slots = torch.zeros(self.B, dtype=torch.long, device=dev)
+        self.error = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.max_new, self._most = int(max_new), max(lengths)
+        q0 = torch.zeros(self.B, c.n_head, c.head_dim, dtype=model.dtype, device=dev)
+        self.plan = pool.decode_plan(q0, self.table, self.seqlen, scale=1.0 / math.sqrt(c.head_dim))
+        self.graph = None
+        if self._most > self.budget:
+            self.evict()
+
+    def evict(self) -> None:
+        """Cut every row past the budget now (:meth:`step` does so by itself)."""
+        self.pool.evict(self.table, self.seqlen, self.weights, budget=self.budget, recent=self.recent, sinks=self.sinks)
+        self.held.copy_(self.seqlen)
+        self._most = min(self._most, self.budget)
+
+    def _step(self) -> None:
+        m, c = self.model, self.model.cfg
+        x = torch.empty(self.B, c.hidden, dtype=m.dtype, device=m.device)
+        h0 = torch.empty_like(x)
+        decode_step_begin(self.tokens, self.held, self.table, self.pool.block_size, m.w["embed"], m.w["l0.ln1"], c.eps,
+                          self.seqlen, self.slots, x, h0, self.error)
+
+        def attend(i: int, qkv) -> torch.Tensor:
+            p = f"l{i}."
+            q = self.pool.write_qk_norm_rope(i, self.slots, qkv, m.w[p + "qn"], m.w[p + "kn"], m.cos, m.sin, self.pos,
+                                             c.eps)
+            return self.plan.run_weighed(i, q, self.weights[i]).view(self.B, -1)
+
+        h = m._decode_stack(x, attend, h0)
+        self.held += 1
+        w = m.w["embed"]
+        if rows_supported(h, w) and h.shape[1] <= 1024:
+            greedy_advance_tiles(rows_tile_best(h, w), self.tokens, self.pos, self.history, self.step_idx)
+        else:
+            greedy_advance(m._lm_head(h), self.tokens, self.pos, self.history, self.step_idx)
+
+    def capture(self, stream=None) -> None:
+        """Record one step (run once eagerly first, its effects undone: the K/V that it wrote lie past the rows)."""
+        state = (self.pos, self.held, self.tokens, self.seqlen, self.step_idx, self.weights, self.history)
+        saved = [t.clone() for t in state]
+        self._step()
+        torch.cuda.synchronize()
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph, stream=stream):
+            self._step()
+        for t, was in zip(state, saved):
+            t.copy_(was)
+        torch.cuda.synchronize()
+
+    def step(self) -> None:
+        """One step of every row, after cutting the rows where one has reached ``budget + every`` tokens."""
+        if self._most >= self.budget + self.every:
+            self.evict()
+        if self.graph is None:
+            self._step()
+        else:
+            self.graph.replay()
+        self._most += 1
+
+    def check(self) -> None:
+        """Raise ``IndexError`` if a step or an eviction met an index out of range (host reads)."""
+        bad = int(self.error.item())
+        if bad:
+            self.error.zero_()
+            raise IndexError(f"row {bad - 1}: token or place out of range in a decode step; the row was skipped")
         self.pool.check_writes()

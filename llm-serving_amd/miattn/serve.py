@@ -2,7 +2,8 @@
 
 A minimal engine + scheduler, enough to run the reference's online workload end to end:
 Poisson arrivals, FIFO packed-group admission, one batched greedy decode step at a time,
-retirement at the token budget, blocks returned to the pool. The reference splits this
+retirement at the token budget, blocks returned to the pool (under a model's window, as soon as
+no later step sees them). The reference splits this
 over ``bench/loadgen.py`` (traces), ``serve/scheduler.py`` (admission, ``step``),
 ``serve/engine.py`` (``prefill_group``, ``_decode_paged``, ``_sync_paged_cache``) and
 ``serve/block_manager.py`` (blocks); here it is one loop because only its use of the
@@ -184,7 +185,8 @@ class SeatDecoder:
         self.x = torch.empty(self.S, c.hidden, dtype=model.dtype, device=dev)
         self.h0 = torch.empty_like(self.x)
         q0 = torch.zeros(self.S, c.n_head, c.head_dim, dtype=model.dtype, device=dev)
-        self.plan = pool.decode_plan(q0, self.table, self.seqlen, scale=1.0 / math.sqrt(c.head_dim))
+        self.plan = pool.decode_plan(q0, self.table, self.seqlen, scale=1.0 / math.sqrt(c.head_dim), window=c.window,
+                                     sinks=c.sinks)
         # q/k norm + RoPE + K/V write fused into the decode launch where the shape allows
         self.fused = self.plan.fused_supported(model.dtype, 2 * int(model.cos.shape[-1]))
         self.graph = None
@@ -310,6 +312,8 @@ class ContinuousServer:
         self.seats = SeatDecoder(model, self.pool, max_batch, self.blocks.blocks_for(max_prompt + max_new), max_new)
         self.stream = stream
         self.n_blocks = int(n_blocks)
+        cfg = getattr(model, "cfg", None)
+        self.window, self.sinks = getattr(cfg, "window", None), getattr(cfg, "sinks", 0)
         self.steps_run = 0
         # concurrency seen by the last run(): the most seats active in one decode step,
         # admissions made while other requests were decoding, and retirements that left
@@ -414,6 +418,8 @@ class ContinuousServer:
                     active[seat] = (req, blocks, 1)
                     if req.max_new == 1:
                         self._finish(seat, active, free_seats, records, t_first)
+                    else:
+                        self._give_hidden(seat, active)
             if not active:
                 continue
             # ---- one decode step of every seat
@@ -432,7 +438,9 @@ class ContinuousServer:
                     self._finish(seat, active, free_seats, records, t_step)
                     if active:
                         self.retired_mid_decode += 1
-                elif forced is not None:
+                    continue
+                self._give_hidden(seat, active)
+                if forced is not None:
                     force_seats.append(seat)
                     force_tokens.append(forced[req.idx][n])
             if force_seats:
@@ -441,10 +449,24 @@ class ContinuousServer:
         wall = skew if step_s is not None else time.perf_counter() - t0 + skew
         return [records[r.idx] for r in trace], wall
 
+    def _hidden(self, length: int) -> range:
+        """Logical blocks of a row that no step from row length ``length`` on sees (none without a window)."""
+        bs = self.blocks.block_size
+        return range(0) if self.window is None else range(-(-self.sinks // bs), max(0, length - self.window) // bs)
+
+    def _give_hidden(self, seat, active) -> None:
+        """Hand back the blocks that have left a seat's window; its device table keeps their ids, unread."""
+        req, blocks, n = active[seat]
+        gone = [j for j in self._hidden(len(req.prompt) + n) if blocks[j] is not None]
+        if gone:
+            self.blocks.give_back([blocks[j] for j in gone])
+            for j in gone:
+                blocks[j] = None
+
     def _finish(self, seat, active, free_seats, records, t) -> None:
         req, blocks, n = active.pop(seat)
         rec = records[req.idx]
         rec.tokens = rec.tokens[:1] + self.seats.retire(seat, n - 1)
         rec.finish_s = t
-        self.blocks.give_back(blocks)
+        self.blocks.give_back([b for b in blocks if b is not None])
         free_seats.append(seat)

@@ -6,6 +6,12 @@ Every arm answers the reference's backend interface (``model/attention/varlen.py
     backend.prefill_varlen(q, k, v, *, cu_seqlens, max_seqlen,
                            softmax_scale=None, causal=True) -> (total, H, D)
 
+and two calls without a reference counterpart::
+
+    backend.prefill_varlen(..., window=W, sinks=S)           # query i sees key j <= i if i - j < W or j < S
+    backend.prompt_weights(q, k, *, cu_seqlens, max_seqlen, observe=32,
+                           softmax_scale=None, out=None) -> (n_seqs, H_kv, max_seqlen)  # for PagedPool.evict
+
 ``q`` is ``(total, H, D)`` and ``k``/``v`` ``(total, H_kv, D)`` over one packed token axis;
 ``cu_seqlens`` (a sequence or a 1-D integer tensor) starts at 0, increases strictly and ends
 at ``total``; ``max_seqlen`` equals the longest segment. Layout and offset mistakes raise
@@ -37,6 +43,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from ._contract import Rule, as_index, enforce
+from .decode import check_window
 
 __all__ = ["HipVarlen", "SdpaVarlen", "backend_for", "check_prefill_errors", "segment_bounds", "validate_packed"]
 
@@ -127,6 +134,38 @@ def _scale(softmax_scale, head_dim: int) -> float:
     return float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(head_dim)
 
 
+def _check_band(window, sinks, causal) -> tuple[int, int] | None:
+    band = check_window(window, sinks)
+    if band is not None and not causal:
+        raise ValueError("a window is a causal one: it needs causal=True")
+    return band
+
+
+_OBSERVED = (
+    Rule(lambda a: a.q.dim() != 3 or a.k.dim() != 3, ValueError,
+         lambda a: "prompt_weights takes 3-D (total_tokens, heads, head_dim) tensors, got "
+                   f"q {tuple(a.q.shape)}, k {tuple(a.k.shape)}"),
+)
+
+
+def _observed(q, k, cu_seqlens, max_seqlen, observe, out) -> tuple[list[int], int, torch.Tensor]:
+    """The checks of ``prompt_weights``: segment bounds, queries observed per segment, and the account."""
+    enforce(_OBSERVED, SimpleNamespace(q=q, k=k))
+    bounds = validate_packed(q, k, k, cu_seqlens, max_seqlen)
+    longest = max(b - a for a, b in zip(bounds, bounds[1:]))
+    if observe is not None and (isinstance(observe, bool) or as_index(observe, "observe") < 1):
+        raise ValueError(f"observe must be a positive int or None (all queries), got {observe!r}")
+    observe = longest if observe is None else min(as_index(observe, "observe"), longest)
+    want = (len(bounds) - 1, int(k.shape[1]))
+    if out is None:
+        out = torch.empty((*want, longest), dtype=torch.float32, device=q.device)
+    elif (out.dim() != 3 or tuple(out.shape[:2]) != want or out.shape[2] < longest or out.dtype != torch.float32
+          or out.device != q.device or out.stride(2) != 1):
+        raise ValueError(f"out must be fp32 ({want[0]}, {want[1]}, at least {longest}) on {q.device} with contiguous rows, "
+                         f"got {out.dtype} {tuple(out.shape)} strides {out.stride()} on {out.device}")
+    return bounds, observe, out
+
+
 class SdpaVarlen:
     """Per-segment ``F.scaled_dot_product_attention``: the reference's CPU/MPS arm
     (``model/attention/varlen.py:259-290``). Each segment is its own ``(1, H, L, D)``
@@ -135,16 +174,39 @@ class SdpaVarlen:
     name = "sdpa-varlen"
 
     def prefill_varlen(self, q, k, v, *, cu_seqlens: Sequence[int] | torch.Tensor, max_seqlen: int,
-                       softmax_scale: float | None = None, causal: bool = True):
+                       softmax_scale: float | None = None, causal: bool = True, window: int | None = None,
+                       sinks: int = 0):
+        band = _check_band(window, sinks, causal)
         bounds = validate_packed(q, k, v, cu_seqlens, max_seqlen)
         scale = _scale(softmax_scale, q.shape[-1])
         gqa = q.shape[1] != k.shape[1]
         out = torch.empty_like(q)
         for a, b in zip(bounds, bounds[1:]):
             qs, ks, vs = (t[a:b].transpose(0, 1).unsqueeze(0) for t in (q, k, v))
-            y = F.scaled_dot_product_attention(qs, ks, vs, dropout_p=0.0, is_causal=bool(causal), scale=scale,
-                                               enable_gqa=gqa)
+            mask = None
+            if band is not None:
+                at = torch.arange(b - a, device=q.device)
+                back = at.unsqueeze(1) - at
+                mask = (back >= 0) & ((back < band[0]) | (at < band[1]))
+            y = F.scaled_dot_product_attention(qs, ks, vs, attn_mask=mask, dropout_p=0.0,
+                                               is_causal=bool(causal) and mask is None, scale=scale, enable_gqa=gqa)
             out[a:b] = y[0].transpose(0, 1)
+        return out
+
+    def prompt_weights(self, q, k, *, cu_seqlens: Sequence[int] | torch.Tensor, max_seqlen: int,
+                       observe: int | None = 32, softmax_scale: float | None = None, out=None):
+        """:meth:`HipVarlen.prompt_weights` in host tensor operations, fp32."""
+        bounds, observe, out = _observed(q, k, cu_seqlens, max_seqlen, observe, out)
+        scale = _scale(softmax_scale, q.shape[-1])
+        out.zero_()
+        group = q.shape[1] // k.shape[1]
+        for s, (a, b) in enumerate(zip(bounds, bounds[1:])):
+            first = max(a, b - observe)
+            keys = k[a:b].float().permute(1, 2, 0).repeat_interleave(group, 0)
+            scores = torch.matmul(q[first:b].float().transpose(0, 1), keys) * scale
+            hidden = torch.arange(b - a, device=q.device) > torch.arange(first - a, b - a, device=q.device).unsqueeze(1)
+            w = torch.softmax(scores.masked_fill(hidden, -math.inf), -1).sum(1)
+            out[s, :, : b - a] = w.view(k.shape[1], group, b - a).sum(1)
         return out
 
 
@@ -162,11 +224,21 @@ class _Schedules:
         self._lru: OrderedDict = OrderedDict()
         self._pinned: dict = {}
 
-    def get(self, bounds: list[int], H: int, H_kv: int, D: int, causal: bool, device, kernel: int):
+    def get(self, bounds: list[int], H: int, H_kv: int, D: int, causal: bool, device, kernel: int, band=None):
         key = (tuple(bounds), H, H_kv, D, bool(causal), device, kernel)
+        return self._get(key if band is None else (*key, band), lambda: (
+            self._build(bounds, H, H_kv, D, causal, device, kernel) if band is None else
+            self._build_window(bounds, H, H_kv, D, band, device)))
+
+    def get_weights(self, bounds: list[int], H: int, H_kv: int, observe: int, device):
+        """The launch state of ``prompt_weights``: no workspace in it (no launch depends on the last one's)."""
+        return self._get(("weights", tuple(bounds), H, H_kv, observe, device),
+                         lambda: self._build_weights(bounds, H, H_kv, observe, device))
+
+    def _get(self, key, build):
         entry = self._pinned.get(key) or self._lru.get(key)
         if entry is None:
-            entry = self._build(bounds, H, H_kv, D, causal, device, kernel)
+            entry = build()
             self._lru[key] = entry
             while len(self._lru) > self.capacity:
                 self._lru.popitem(last=False)
@@ -175,6 +247,38 @@ class _Schedules:
         if torch.cuda.is_current_stream_capturing():
             self._pinned[key] = entry
         return entry
+
+    @staticmethod
+    def _words(schedule, what):
+        """The int32 words of a host schedule function called with ``(out, capacity)``."""
+        n_words = schedule(None, 0)
+        if n_words < 0:
+            _lib.check(n_words, what)
+        words = (ctypes.c_int32 * n_words)()
+        rc = schedule(words, n_words)
+        if rc < 0:
+            _lib.check(rc, what)
+        return words
+
+    @classmethod
+    def _build_window(cls, bounds, H, H_kv, D, band, device):
+        host_cu = (ctypes.c_int32 * len(bounds))(*bounds)
+        words = cls._words(lambda out, n: _lib.lib.mi_varlen_schedule_window(
+            host_cu, len(bounds) - 1, H, H_kv, D, *band, out, n), "prefill_varlen schedule")
+        ws_bytes = int(_lib.lib.mi_varlen_workspace_size(words, H))
+        return SimpleNamespace(
+            cu=torch.tensor(bounds, dtype=torch.int32).to(device),
+            sched=torch.frombuffer(bytearray(words), dtype=torch.int32).to(device),
+            header=tuple(int(words[i]) for i in range(4)), ws_bytes=ws_bytes)
+
+    @classmethod
+    def _build_weights(cls, bounds, H, H_kv, observe, device):
+        host_cu = (ctypes.c_int32 * len(bounds))(*bounds)
+        words = cls._words(lambda out, n: _lib.lib.mi_prompt_weights_schedule(
+            host_cu, len(bounds) - 1, H, H_kv, observe, out, n), "prompt_weights schedule")
+        return SimpleNamespace(sched=torch.frombuffer(bytearray(words), dtype=torch.int32).to(device),
+                               header=(ctypes.c_int32 * 4)(*words[:4]),
+                               ws_bytes=int(_lib.lib.mi_prompt_weights_workspace_size(words, H_kv)))
 
     @staticmethod
     def _build(bounds, H, H_kv, D, causal, device, kernel):
@@ -264,7 +368,13 @@ class HipVarlen:
         self._strict = bool(strict)
 
     def prefill_varlen(self, q, k, v, *, cu_seqlens: Sequence[int] | torch.Tensor, max_seqlen: int,
-                       softmax_scale: float | None = None, causal: bool = True):
+                       softmax_scale: float | None = None, causal: bool = True, window: int | None = None,
+                       sinks: int = 0):
+        """Attention inside each segment. With ``window`` (causal only), query ``i`` sees key ``j <= i`` if
+        ``i - j < window`` or ``j < sinks``, at the cost of the keys that are seen; ``head_dim`` 64, 128 or 256, at most
+        255 heads, a positive scale, ``v`` finite (as in the plain product, a weight of 0 does not remove an
+        infinity or NaN from the queries of the same 64-key tile). ``kernel=`` has no say there."""
+        band = _check_band(window, sinks, causal)
         bounds = validate_packed(q, k, v, cu_seqlens, max_seqlen)
         scale = _scale(softmax_scale, q.shape[-1])
         if not (q.is_cuda and k.is_cuda and v.is_cuda):
@@ -276,6 +386,8 @@ class HipVarlen:
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
         total, H, D = q.shape
         H_kv = int(k.shape[1])
+        if band is not None:
+            return self._windowed(q, k, v, bounds, band, int(max_seqlen), scale)
         plan = _SCHEDULES.get(bounds, H, H_kv, D, causal, q.device, self._kernel)
         out = torch.empty_like(q)
         rc = _lib.lib.mi_varlen_prefill(
@@ -287,6 +399,52 @@ class HipVarlen:
         _lib.check(rc, "prefill_varlen")
         if self._strict and not torch.cuda.is_current_stream_capturing():
             check_prefill_errors(q.device)
+        return out
+
+    def _windowed(self, q, k, v, bounds, band, longest: int, scale: float):
+        total, H, D = q.shape
+        H_kv = int(k.shape[1])
+        q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v))
+        band = tuple(min(x, longest) for x in band)  # what lies past the longest segment hides nothing
+        with _lib.on_device(q.device):
+            plan = _SCHEDULES.get(bounds, H, H_kv, D, True, q.device, -1, band)
+            out = torch.empty_like(q)
+            # the pieces' partials: this call's own, so calls on several streams do not share them
+            ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=q.device) if plan.ws_bytes else None
+            rc = _lib.lib.mi_varlen_prefill_window(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), plan.cu.data_ptr(), len(bounds) - 1, total,
+                longest, plan.sched.data_ptr(), *plan.header, H, H_kv, D, scale, *band, _lib.dtype_code(q.dtype),
+                None if ws is None else ws.data_ptr(), plan.ws_bytes, _error_word(q.device).data_ptr(),
+                _lib.current_stream(q.device))
+            _lib.check(rc, "prefill_varlen")
+            if self._strict and not torch.cuda.is_current_stream_capturing():
+                check_prefill_errors(q.device)
+        return out
+
+    def prompt_weights(self, q, k, *, cu_seqlens: Sequence[int] | torch.Tensor, max_seqlen: int,
+                       observe: int | None = 32, softmax_scale: float | None = None, out=None):
+        """Where each prompt's last ``observe`` queries (None: all) look: fp32 ``(n_seqs, n_kv_head, max_seqlen)``, entry
+        ``[s, kv, j]`` the causal softmax weights that they give key ``j`` of segment ``s``, summed over them
+        and the query heads of ``kv``; zeros past a segment's length. ``q``, ``k`` as :meth:`prefill_varlen` takes
+        them (fp16 or bf16, ``head_dim`` 64, 128 or 256, a positive scale). ``out``: an account to fill, fp32
+        ``(n_seqs, n_kv_head, at least max_seqlen)`` with contiguous rows, e.g. the rows of a decode's."""
+        bounds, observe, out = _observed(q, k, cu_seqlens, max_seqlen, observe, out)
+        scale = _scale(softmax_scale, q.shape[-1])
+        if not q.is_cuda:
+            raise RuntimeError(f"HipVarlen is the CUDA (HIP) kernel path, but q/k are on {q.device}; "
+                               "backend_for() gives host tensors the SDPA arm")
+        if q.dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError(f"the MFMA varlen kernels compute fp16/bf16 only, got {q.dtype}")
+        q, k = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.contiguous().clone() for t in (q, k))
+        H, H_kv, D = int(q.shape[1]), int(k.shape[1]), int(q.shape[2])
+        with _lib.on_device(q.device):
+            plan = _SCHEDULES.get_weights(bounds, H, H_kv, observe, q.device)
+            ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=q.device)
+            rc = _lib.lib.mi_prompt_weights(
+                q.data_ptr(), k.data_ptr(), plan.sched.data_ptr(), plan.header, H, H_kv, D, scale,
+                _lib.dtype_code(q.dtype), out.data_ptr(), out.stride(0), out.stride(1), out.shape[2], ws.data_ptr(),
+                plan.ws_bytes, _lib.current_stream(q.device))
+        _lib.check(rc, "prompt_weights")
         return out
 
 
