@@ -441,7 +441,7 @@ int mi_varlen_prefill_window(const void* q, const void* k, const void* v, void* 
  *   head_dim 64, 128 or 256, scale > 0): out[s, kv, j] = the weights that the last `observe` queries of segment s
  *   give key j under causal attention, summed over the query heads of kv; zeros from the segment's length up to `width`
  *   (at least the longest segment). out fp32, element s * out_s0 + kv * out_s1 + j. schedule: a
- *   device copy of mi_prompt_weights_schedule's words (host only; NULL sizes it), host_header their first four.
+ *   device copy of mi_prompt_weights_schedule's words (host only; NULL sizes it), host_header their first eight.
  *   Workspace: mi_prompt_weights_workspace_size() of that header.
  * mi_cache_evict: rows longer than `budget` tokens cut to it, for every layer, row and KV head: the first `sinks` tokens,
  *   the last `recent` and the heaviest of the others by `weights` (NaN above every number, the lowest index
@@ -461,7 +461,7 @@ int mi_paged_decode_weigh(const void* q, const void* k_cache, const void* v_cach
                           int max_blocks, const int64_t* strides, float scale, int dtype, float* weights,
                           int64_t weights_s0, int64_t weights_s1, void* workspace, size_t workspace_bytes,
                           void* stream);
-int mi_prompt_weights_schedule(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int observe,
+int mi_prompt_weights_schedule(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int D, int observe,
                                int32_t* host_schedule, int capacity);
 size_t mi_prompt_weights_workspace_size(const int32_t* host_schedule, int H_kv);
 int mi_prompt_weights(const void* q, const void* k, const int32_t* schedule, const int32_t* host_header, int H, int H_kv,

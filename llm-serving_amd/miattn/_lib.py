@@ -184,7 +184,7 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
          _c_int, _p_int64, _c_float, _c_int, _c_void_p, _c_int64, _c_int64, _c_void_p, _c_size_t, _c_void_p],
     ),
-    "mi_prompt_weights_schedule": (_c_int, [_p_int32, _c_int, _c_int, _c_int, _c_int, _p_int32, _c_int]),
+    "mi_prompt_weights_schedule": (_c_int, [_p_int32, _c_int, _c_int, _c_int, _c_int, _c_int, _p_int32, _c_int]),
     "mi_prompt_weights_workspace_size": (_c_size_t, [_p_int32, _c_int]),
     "mi_prompt_weights": (
         _c_int,

@@ -230,10 +230,10 @@ class _Schedules:
             self._build(bounds, H, H_kv, D, causal, device, kernel) if band is None else
             self._build_window(bounds, H, H_kv, D, band, device)))
 
-    def get_weights(self, bounds: list[int], H: int, H_kv: int, observe: int, device):
+    def get_weights(self, bounds: list[int], H: int, H_kv: int, D: int, observe: int, device):
         """The launch state of ``prompt_weights``: no workspace in it (no launch depends on the last one's)."""
-        return self._get(("weights", tuple(bounds), H, H_kv, observe, device),
-                         lambda: self._build_weights(bounds, H, H_kv, observe, device))
+        return self._get(("weights", tuple(bounds), H, H_kv, D, observe, device),
+                         lambda: self._build_weights(bounds, H, H_kv, D, observe, device))
 
     def _get(self, key, build):
         entry = self._pinned.get(key) or self._lru.get(key)
@@ -272,12 +272,12 @@ class _Schedules:
             header=tuple(int(words[i]) for i in range(4)), ws_bytes=ws_bytes)
 
     @classmethod
-    def _build_weights(cls, bounds, H, H_kv, observe, device):
+    def _build_weights(cls, bounds, H, H_kv, D, observe, device):
         host_cu = (ctypes.c_int32 * len(bounds))(*bounds)
         words = cls._words(lambda out, n: _lib.lib.mi_prompt_weights_schedule(
-            host_cu, len(bounds) - 1, H, H_kv, observe, out, n), "prompt_weights schedule")
+            host_cu, len(bounds) - 1, H, H_kv, D, observe, out, n), "prompt_weights schedule")
         return SimpleNamespace(sched=torch.frombuffer(bytearray(words), dtype=torch.int32).to(device),
-                               header=(ctypes.c_int32 * 4)(*words[:4]),
+                               header=(ctypes.c_int32 * 8)(*words[:8]),
                                ws_bytes=int(_lib.lib.mi_prompt_weights_workspace_size(words, H_kv)))
 
     @staticmethod
@@ -438,7 +438,7 @@ class HipVarlen:
         q, k = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.contiguous().clone() for t in (q, k))
         H, H_kv, D = int(q.shape[1]), int(k.shape[1]), int(q.shape[2])
         with _lib.on_device(q.device):
-            plan = _SCHEDULES.get_weights(bounds, H, H_kv, observe, q.device)
+            plan = _SCHEDULES.get_weights(bounds, H, H_kv, D, observe, q.device)
             ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=q.device)
             rc = _lib.lib.mi_prompt_weights(
                 q.data_ptr(), k.data_ptr(), plan.sched.data_ptr(), plan.header, H, H_kv, D, scale,

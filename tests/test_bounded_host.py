@@ -196,11 +196,11 @@ def test_c_entries_refuse_before_any_launch():
     for scale in (0.0, -1.0, math.nan):
         assert lib.mi_varlen_prefill_window(*launch, 4, 2, 128, scale, 8, 0, 2, *tail) == _lib.MI_ERR_INVALID
     assert lib.mi_varlen_prefill_window(*launch, 4, 2, 128, 1.0, 8, 0, 0, *tail) == _lib.MI_ERR_UNSUPPORTED
-    assert lib.mi_prompt_weights_schedule(cu, 2, 4, 2, 0, None, 0) == _lib.MI_ERR_INVALID
-    n = lib.mi_prompt_weights_schedule(cu, 2, 4, 2, 32, None, 0)
+    assert lib.mi_prompt_weights_schedule(cu, 2, 4, 2, 128, 0, None, 0) == _lib.MI_ERR_INVALID
+    n = lib.mi_prompt_weights_schedule(cu, 2, 4, 2, 128, 32, None, 0)
     words = (ctypes.c_int32 * n)()
-    assert lib.mi_prompt_weights_schedule(cu, 2, 4, 2, 32, words, n) == n
-    head = (ctypes.c_int32 * 4)(*words[:4])
+    assert lib.mi_prompt_weights_schedule(cu, 2, 4, 2, 128, 32, words, n) == n
+    head = (ctypes.c_int32 * 8)(*words[:8])
     assert lib.mi_prompt_weights(64, 64, 64, head, 4, 2, 128, 1.0, 2, 64, 1, 1, 130, None, 0, None) == _lib.MI_ERR_WORKSPACE
     assert lib.mi_prompt_weights(64, 64, 64, head, 4, 2, 128, -1.0, 2, 64, 1, 1, 130, 64, 1 << 30, None) == _lib.MI_ERR_INVALID
     assert lib.mi_prompt_weights(64, 64, 64, head, 4, 2, 96, 1.0, 2, 64, 1, 1, 130, 64, 1 << 30, None) == _lib.MI_ERR_UNSUPPORTED
