@@ -31,6 +31,7 @@ must stay ordered on one stream (a layer loop is).
 
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
 from types import SimpleNamespace
@@ -297,8 +298,8 @@ class PagedDecodePlan:
     """
 
     __slots__ = ("n_layer", "geometry", "q_signature", "_k_ptrs", "_v_ptrs", "_pools",
-                 "_table", "_seqlen", "_strides", "_scale", "_ws", "_ws_bytes", "_frozen", "_band", "_banded",
-                 "_weigh_ws", "_weigh_shape")
+                 "_table", "_seqlen", "_strides", "_scale", "_ws", "_ws_bytes", "_frozen", "_band",
+                 "_weigh_ws", "_weigh_shape", "_layout", "_fixed", "_reads", "_weigh_args")
 
     def __init__(self, q, k_caches, v_caches, block_table, seqlen, *, scale=None, window=None, sinks=0) -> None:
         self._band = check_window(window, sinks)
@@ -330,12 +331,22 @@ class PagedDecodePlan:
         # the launch arguments after ``out`` that no run changes (the plan owns the workspace)
         self._frozen = (*g.dims(), self._strides, self._scale, _lib.dtype_code(q.dtype),
                         None if self._ws is None else self._ws.data_ptr(), self._ws_bytes)
-        self._banded = None if self._band is None else (*self._frozen[:-2], *self._band, *self._frozen[-2:])
-        self._weigh_ws = None  # run_weighed's workspace, taken at its first call
+        # The windowed and weighed calls' arguments as ctypes takes them, and the query's layout as its attributes come:
+        # an eager step of 28 layers over short rows waits for the host, 10 us a call, most of it two launches
+        self._layout = (q.shape, q.dtype, q.stride(), q.get_device())
+        self._fixed = (*map(ctypes.c_int, g.dims()), self._strides, ctypes.c_float(self._scale),
+                       ctypes.c_int(_lib.dtype_code(q.dtype)))
+        self._reads = [tuple(map(ctypes.c_void_p, (k, v, block_table.data_ptr(), seqlen.data_ptr())))
+                       for k, v in zip(self._k_ptrs, self._v_ptrs)]
+        if self._band is not None:
+            self._fixed += (*map(ctypes.c_int, self._band), ctypes.c_void_p(self._frozen[-2]), ctypes.c_size_t(self._ws_bytes))
+        self._weigh_ws = None  # run_weighed's workspace, taken at its first call, and its last arguments
         self._weigh_shape = torch.Size((g.rows, g.kv_heads, g.capacity))
 
     def run(self, layer: int, q):
         """Launch one layer; ``q`` must have the layout the plan was built with."""
+        if self._band is not None:
+            return self._run_window(int(layer), q)
         if not 0 <= int(layer) < self.n_layer:
             raise IndexError(f"layer {layer} is outside the plan's {self.n_layer} layers")
         signature = (tuple(q.shape), q.dtype, q.device, q.stride())
@@ -347,18 +358,28 @@ class PagedDecodePlan:
             )
         out = torch.empty_like(q)
         layer = int(layer)
-        if self._banded is not None:
-            with _lib.on_device(q.device):
-                rc = _lib.lib.mi_paged_decode_window(
-                    q.data_ptr(), self._k_ptrs[layer], self._v_ptrs[layer], self._table.data_ptr(),
-                    self._seqlen.data_ptr(), out.data_ptr(), *self._banded, _lib.current_stream(q.device))
-            if rc:
-                _lib.check(rc, "paged_decode_plan.run")
-            return out
         rc = _lib.lib.mi_paged_decode(q.data_ptr(), self._k_ptrs[layer], self._v_ptrs[layer], self._table.data_ptr(),
                                       self._seqlen.data_ptr(), out.data_ptr(), *self._frozen,
                                       _lib.current_stream(q.device))
         _lib.check(rc, "paged_decode_plan.run")
+        return out
+
+    def _check_query(self, layer: int, q, what: str) -> None:
+        if not 0 <= layer < self.n_layer:
+            raise IndexError(f"layer {layer} is outside the plan's {self.n_layer} layers")
+        if (q.shape, q.dtype, q.stride(), q.get_device()) != self._layout:
+            raise ValueError(f"paged_decode_plan.{what}: the query does not match the validated layout "
+                             f"(built for shape/dtype/device/strides {self.q_signature}, got "
+                             f"{(tuple(q.shape), q.dtype, q.device, q.stride())}); build a new plan for a new layout")
+
+    def _run_window(self, layer: int, q):
+        self._check_query(layer, q, "run")
+        with _lib.on_device(self.q_signature[2]):
+            out = torch.empty_like(q)
+            rc = _lib.lib.mi_paged_decode_window(q.data_ptr(), *self._reads[layer], out.data_ptr(), *self._fixed,
+                                                 _lib.current_stream(self.q_signature[2]))
+        if rc:
+            _lib.check(rc, "paged_decode_plan.run")
         return out
 
     def run_weighed(self, layer: int, q, weights: torch.Tensor) -> torch.Tensor:
@@ -369,29 +390,24 @@ class PagedDecodePlan:
         call wait in a workspace of the plan's own (4 bytes per token of the tables and query head, taken at
         the first call), so weighed runs, too, stay ordered on one stream. A plan under a window does not weigh."""
         layer = int(layer)
-        if not 0 <= layer < self.n_layer:
-            raise IndexError(f"layer {layer} is outside the plan's {self.n_layer} layers")
         if self._band is not None:
             raise ValueError("run_weighed accounts for every token of a row; this plan is under a window")
-        signature = (tuple(q.shape), q.dtype, q.device, q.stride())
-        if signature != self.q_signature:
-            raise ValueError("paged_decode_plan.run_weighed: the query does not match the validated layout "
-                             f"(built for shape/dtype/device/strides {self.q_signature}, got {signature}); "
-                             "build a new plan for a new layout")
-        if (weights.shape != self._weigh_shape or weights.dtype != torch.float32 or weights.stride(2) != 1
-                or weights.device != q.device):
+        self._check_query(layer, q, "run_weighed")
+        row, head, last = weights.stride() if weights.dim() == 3 else (0, 0, 0)
+        if (weights.shape != self._weigh_shape or last != 1 or weights.dtype != torch.float32
+                or weights.get_device() != self._layout[3]):
             raise ValueError(f"weights must be fp32 {tuple(self._weigh_shape)} on {q.device} with contiguous rows, got "
                              f"{weights.dtype} {tuple(weights.shape)} strides {weights.stride()} on {weights.device}")
-        with _lib.on_device(q.device):
+        device = self.q_signature[2]
+        with _lib.on_device(device):
             if self._weigh_ws is None:
-                n = int(_lib.lib.mi_paged_decode_weigh_workspace_size(*self.geometry.dims(), self._frozen[8]))
-                self._weigh_ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+                n = int(_lib.lib.mi_paged_decode_weigh_workspace_size(*self.geometry.dims(), _lib.dtype_code(q.dtype)))
+                self._weigh_ws = torch.empty(n, dtype=torch.uint8, device=device)
+                self._weigh_args = (ctypes.c_void_p(self._weigh_ws.data_ptr()), ctypes.c_size_t(n))
             out = torch.empty_like(q)
-            ws = self._weigh_ws
-            rc = _lib.lib.mi_paged_decode_weigh(
-                q.data_ptr(), self._k_ptrs[layer], self._v_ptrs[layer], self._table.data_ptr(), self._seqlen.data_ptr(),
-                out.data_ptr(), *self._frozen[:-2], weights.data_ptr(), weights.stride(0), weights.stride(1),
-                ws.data_ptr(), ws.numel(), _lib.current_stream(q.device))
+            rc = _lib.lib.mi_paged_decode_weigh(q.data_ptr(), *self._reads[layer], out.data_ptr(), *self._fixed,
+                                                weights.data_ptr(), row, head, *self._weigh_args,
+                                                _lib.current_stream(device))
         if rc:
             _lib.check(rc, "paged_decode_plan.run_weighed")
         return out
