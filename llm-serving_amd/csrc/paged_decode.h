@@ -892,18 +892,20 @@ struct RowsLayout {
   static constexpr size_t lds(int max_blocks) { return (32 * GB * (D + 2) + size_t(max_blocks)) * sizeof(float); }
   static constexpr bool ok = sizeof(T) == 2 && GB <= 2 && (D == 64 || D == 128) && Lay::RPW % TPL == 0 && W >= 4 && W <= 16 && GB * D <= 64 * W;
 };
-template <typename T, int D, int GB, int TPL>
+template <typename T, int D, int GB, int TPL, typename Ext>
 __global__ __launch_bounds__((64 * RowsLayout<T, D, GB, TPL>::W)) void paged_decode_rows_kernel(
     const T* __restrict__ q, const T* __restrict__ kc, const T* __restrict__ vc,
-    const int32_t* __restrict__ block_table, const int32_t* __restrict__ seqlen, T* __restrict__ out, DecodeArgs a) {
+    const int32_t* __restrict__ block_table, const int32_t* __restrict__ seqlen, T* __restrict__ out, DecodeArgs a,
+    Ext ext) {
   using Lay = Layout<T, D, GB>;
   using Rows = RowsLayout<T, D, GB, TPL>;
   constexpr int EPL = Lay::EPL, LPR = Lay::LPR, U = Lay::U, SPW = Rows::SPW, W = Rows::W;
   constexpr int batch = TPL * U, kMost = 32;
-  extern __shared__ float smem[];  // partials [32][GB][D], (m, l) [32][GB][2], page ids
+  extern __shared__ float smem[];  // partials [32][GB][D], (m, l) [32][GB][2], (weighing) scores [capacity][GB], page ids
   float* sm_acc = smem;
   float* sm_ml = sm_acc + kMost * GB * D;
-  int32_t* sm_pg = reinterpret_cast<int32_t*>(sm_ml + kMost * GB * 2);
+  float* sm_sc = sm_ml + kMost * GB * 2;
+  int32_t* sm_pg = reinterpret_cast<int32_t*>(sm_sc + (Ext::kWeigh ? (a.max_blocks << a.bs_log2) * GB : 0));
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -937,7 +939,8 @@ __global__ __launch_bounds__((64 * RowsLayout<T, D, GB, TPL>::W)) void paged_dec
     return;
   }
   int n_first, incl;
-  const int chunk = plan_chunk(len_first, total, a, batch, n_first, incl);
+  int chunk = plan_chunk(len_first, total, a, batch, n_first, incl);
+  if constexpr (Ext::kWeigh) chunk = max(chunk, (len + kMost * batch - 1) / (kMost * batch) * batch);
   const int n_split = (len + chunk - 1) / chunk;  // <= 32 (rows_kernel_fits)
   __syncthreads();
 
@@ -986,6 +989,13 @@ __global__ __launch_bounds__((64 * RowsLayout<T, D, GB, TPL>::W)) void paged_dec
           dot[u][g] = group_allreduce<LPR, SumOp>(dot16<T>(qr[g], kr[u], 0.0f));
           sc[u][g] = dot[u][g] * a.scale_log2;
           if (t0 + u * TPL + tsub >= t_end) sc[u][g] = -INFINITY;
+        }
+        if constexpr (Ext::kWeigh) {
+          const int tok = t0 + u * TPL + tsub;
+          if (c == 0 && tok < t_end) {
+#pragma unroll
+            for (int g = 0; g < GB; ++g) sm_sc[tok * GB + g] = sc[u][g];
+          }
         }
       }
       const bool masked = t0 >= full;
@@ -1063,7 +1073,7 @@ __global__ __launch_bounds__((64 * RowsLayout<T, D, GB, TPL>::W)) void paged_dec
     if (tsub == 0 && sp < n_split) {
 #pragma unroll
       for (int g = 0; g < GB; ++g) {
-        if (n_split == 1) {
+        if (!Ext::kWeigh && n_split == 1) {
           const float inv = 1.0f / fmaxf(l[g], 1.0f);
           float o[EPL];
 #pragma unroll
@@ -1078,8 +1088,31 @@ __global__ __launch_bounds__((64 * RowsLayout<T, D, GB, TPL>::W)) void paged_dec
       }
     }
   }
-  if (n_split == 1) return;  // uniform
-  __syncthreads();
+  if (!Ext::kWeigh && n_split == 1) return;  // uniform
+  if constexpr (Ext::kWeigh) {
+    // the row's scores are in LDS: each thread turns its tokens' into weights once the row's maxima and sums are
+    float* weights = ext.weights + b * ext.ws0 + kvh * ext.ws1;
+    float before = tid < len ? weights[tid] : 0.0f;
+    __syncthreads();
+    float top[GB], inv[GB];
+#pragma unroll
+    for (int g = 0; g < GB; ++g) {
+      const int j = lane & (kMost - 1);
+      const float2 p = *reinterpret_cast<const float2*>(sm_ml + (min(j, n_split - 1) * GB + g) * 2);
+      const float M = group_allreduce<kMost, MaxOp>(p.x);
+      top[g] = M == -INFINITY ? 0.0f : M;
+      const float l = group_allreduce<kMost, SumOp>(j < n_split ? p.y * fast_exp2(p.x - top[g]) : 0.0f);
+      inv[g] = 1.0f / (l < 1.0f ? 1.0f : l);  // the sum holds the maximum's own 1; NaN stays
+    }
+    for (int t = tid; t < len; t += 64 * W) {
+      float w = t == tid ? before : weights[t];
+#pragma unroll
+      for (int g = 0; g < GB; ++g) w = fmaf(fast_exp2(sm_sc[t * GB + g] - top[g]), inv[g], w);
+      weights[t] = w;
+    }
+  } else {
+    __syncthreads();
+  }
   if (tid >= GB * D) return;  // whole waves; no barrier follows
   // the merge kernel's arithmetic, thread = (head, element)
   const int g = tid / D, d = tid - g * D;  // D >= 64: the head is wave-uniform
@@ -1197,6 +1230,16 @@ bool rows_kernel_fits(const DecodeArgs& a, const Plan& p, int D, int waves) {
          int64_t(a.B) * a.H_kv * a.n_hchunks * waves <= 16 * 256;
 }
 
+// Whether a weighing batch does: one workgroup has to hold every query head of a KV head and a row's scores beside its
+// partials; splits are made long enough for 32 to hold a row. The K elements that a workgroup may have to stream: 24576 where a
+// wave's state takes one token at a time, 16384 where two do (us per layer in a graph, two launches against one: H 16 /
+// H_kv 8 / D 128, two: 1 row of 64 tokens 6.8 / 5.4, 4 of 128 7.6 / 6.8, 32 of 128 10.3 / 9.9, but 4 of 192 7.5 / 8.1 and
+// 1 of 304 8.0 / 10.1; H 32 / H_kv 16 / D 128, one: 1 of 64 6.8 / 4.5, 8 of 192 10.4 / 7.3, 1 of 304 8.4 / 8.7).
+bool weighed_rows_fit(const DecodeArgs& a, const Plan& p, int D, int waves) {
+  const int64_t capacity = int64_t(a.max_blocks) << a.bs_log2;
+  return a.n_hchunks == 1 && capacity * D <= (p.TPL == 1 ? 24576 : 16384) && int64_t(a.B) * a.H_kv * waves <= 16 * 256;
+}
+
 // The second launch of the weighing form: merge and weights (paged_decode_weigh.hip, which alone uses it).
 template <typename T, int D, int GB>
 int finish_weighed(const int32_t* seqlen, void* out, const int32_t* ws_rows, const float* ws_ml, const float* ws_acc,
@@ -1212,12 +1255,14 @@ int launch_typed(const void* q, const void* kc, const void* vc, const int32_t* b
   }
   auto try_rows = [&](auto tpl) {
     constexpr int TPL = decltype(tpl)::value;
-    if constexpr (RowsLayout<T, D, GB, TPL>::ok && !Ext::kWindow && !Ext::kWeigh) {
+    if constexpr (RowsLayout<T, D, GB, TPL>::ok && !Ext::kWindow) {
       using Rows = RowsLayout<T, D, GB, TPL>;
-      if (fa != nullptr || p.TPL != TPL || !rows_kernel_fits(a, p, D, Rows::W)) return false;
-      hipLaunchKernelGGL((paged_decode_rows_kernel<T, D, GB, TPL>), dim3(a.B * a.H_kv * a.n_hchunks), dim3(64 * Rows::W),
-                         Rows::lds(a.max_blocks), stream, static_cast<const T*>(q), static_cast<const T*>(kc),
-                         static_cast<const T*>(vc), bt, seqlen, static_cast<T*>(out), a);
+      const bool fits = Ext::kWeigh ? weighed_rows_fit(a, p, D, Rows::W) : rows_kernel_fits(a, p, D, Rows::W);
+      if (fa != nullptr || p.TPL != TPL || !fits) return false;
+      const size_t scores = Ext::kWeigh ? (size_t(a.max_blocks) << a.bs_log2) * GB * sizeof(float) : 0;
+      hipLaunchKernelGGL((paged_decode_rows_kernel<T, D, GB, TPL, Ext>), dim3(a.B * a.H_kv * a.n_hchunks),
+                         dim3(64 * Rows::W), Rows::lds(a.max_blocks) + scores, stream, static_cast<const T*>(q),
+                         static_cast<const T*>(kc), static_cast<const T*>(vc), bt, seqlen, static_cast<T*>(out), a, ext);
       return true;
     }
     return false;

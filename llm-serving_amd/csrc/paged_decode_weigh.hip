@@ -7,6 +7,7 @@
 // reads them back: some of its workgroups fold the splits of a (row, head), as the plain
 // form's second launch does, the others turn the scores of a (row, KV head, stretch of tokens)
 // into weights. Each weight is read, added to and written once, by one lane, in a fixed order of heads.
+// A batch of short rows takes the one-launch kernel, whose scores never leave LDS.
 #include "paged_decode.h"
 
 namespace miattn {

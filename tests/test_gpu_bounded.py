@@ -247,7 +247,7 @@ def test_windowed_prefill_refusals(cuda):
 
 # ------------------------------------------------------------------ accounts
 @pytest.mark.parametrize("heads", [h for h in HEADS if h[2] > 16])
-@pytest.mark.parametrize("lengths", [[0, 1, 2, 17, 300], [1500, 64, 800], [5000]])
+@pytest.mark.parametrize("lengths", [[0, 1, 2, 17, 300], [1500, 64, 800], [5000], [64, 0, 1, 128, 31, 127, 9, 100], [3]])
 def test_weighed_decode(heads, lengths, cuda):
     H, H_kv, D, dt, bs = heads
     q, k, v, table, seqlen = _rows(lengths, H, H_kv, D, dt, bs)
@@ -280,22 +280,24 @@ def test_weighed_decode_of_equal_keys(cuda):
         assert torch.allclose(account[b, :, :n], torch.full((8, n), 2.0 / n, device=cuda), rtol=2e-6, atol=0)
 
 
-def test_weighed_decode_with_scores_that_are_not_finite(cuda):
-    q, k, v, table, seqlen = _rows([40, 40], 4, 2, 64, F16, 16)
+@pytest.mark.parametrize("H,H_kv,D", [(4, 2, 64), (16, 8, 128), (32, 16, 128)])
+def test_weighed_decode_with_scores_that_are_not_finite(H, H_kv, D, cuda):
+    q, k, v, table, seqlen = _rows([40, 40], H, H_kv, D, F16, 16)
     k[table[1, 0], 3, 0] = math.nan
     q, k, v, table, seqlen = _cuda(q, k, v, table, seqlen)
-    account = torch.zeros(2, 2, table.shape[1] * 16, device=cuda)
+    account = torch.zeros(2, H_kv, table.shape[1] * 16, device=cuda)
     out = paged_decode_plan(q, [k], [v], table, seqlen).run_weighed(0, q, account)
     assert torch.isfinite(out[0]).all() and torch.isfinite(account[0]).all()
-    assert torch.isnan(account[1, 0, :40]).all() and torch.isfinite(account[1, 1]).all() and torch.isfinite(out[1, 2:]).all()
+    assert torch.isnan(account[1, 0, :40]).all() and torch.isfinite(account[1, 1:]).all() and torch.isfinite(out[1, 2:]).all()
 
 
-def test_weighed_decode_captured_with_growing_rows(cuda):
-    q, k, v, table, seqlen = _rows([700, 9, 130], 16, 8, 128, BF16, 16, width=60)
+@pytest.mark.parametrize("lengths,width", [([700, 9, 130], 60), ([70, 0, 55], 8)])
+def test_weighed_decode_captured_with_growing_rows(lengths, width, cuda):
+    q, k, v, table, seqlen = _rows(lengths, 16, 8, 128, BF16, 16, width=width)
     table[table < 0] = 0
     q, k, v, table, seqlen = _cuda(q, k, v, table, seqlen)
     plan, other = (paged_decode_plan(q, [k], [v], table, seqlen) for _ in range(2))
-    account, want = (torch.zeros(3, 8, 960, device=cuda) for _ in range(2))
+    account, want = (torch.zeros(3, 8, 16 * width, device=cuda) for _ in range(2))
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):  # the workspace is taken inside the capture
         out = plan.run_weighed(0, q, account)
