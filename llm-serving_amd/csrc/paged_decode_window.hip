@@ -15,6 +15,12 @@ int windowed(Windowed& w, int window, int sinks) {
   return MI_OK;
 }
 
+// Tables that no row outgrows the window in: the plain form's result, which has the one-launch kernel for short
+// rows (1 row of 8 tokens 10.8 -> 7.2 us a call on the host).
+bool hides_nothing(const Windowed& w, int block_size, int max_blocks) {
+  return int64_t(max_blocks) * block_size <= w.most;
+}
+
 }  // namespace
 }  // namespace miattn
 
@@ -27,6 +33,10 @@ extern "C" int mi_paged_decode_window(const void* q, const void* k_cache, const 
   Windowed w{};
   const int rc = windowed(w, window, sinks);
   if (rc != MI_OK) return rc;
+  if (hides_nothing(w, block_size, max_blocks)) {
+    return mi_paged_decode(q, k_cache, v_cache, block_table, seqlen, out, B, H, H_kv, D, block_size, max_blocks, strides,
+                           scale, dtype, workspace, workspace_bytes, stream);
+  }
   return paged_decode_entry(q, k_cache, v_cache, block_table, seqlen, out, B, H, H_kv, D, block_size, max_blocks,
                             strides, scale, dtype, workspace, workspace_bytes, stream, w);
 }
