@@ -316,7 +316,7 @@ extern "C" int mi_cache_evict(void* const* host_k_pools, void* const* host_v_poo
     return fail(MI_ERR_INVALID, "mi_cache_evict: %d destination blocks of %d do not hold %d tokens", to_blocks, block_size, budget);
   }
   if (B == 0 || n_layers == 0) return MI_OK;
-  if (B > 65535 || int64_t(std::min(n_layers, kMaxLayers)) * B * H_kv > INT32_MAX) {
+  if (B > 65535 || int64_t(std::min(n_layers, kMaxLayers)) * B * H_kv >= (1 << 24)  /* 2^32 threads */) {
     return fail(MI_ERR_UNSUPPORTED, "mi_cache_evict: grid too large (B=%d, H_kv=%d)", B, H_kv);
   }
   if (host_k_pools == nullptr || host_v_pools == nullptr || block_table == nullptr || to_table == nullptr ||
@@ -362,7 +362,7 @@ extern "C" int mi_cache_evict(void* const* host_k_pools, void* const* host_v_poo
   a.budget = budget;
   a.recent = recent;
   a.sinks = sinks;
-  a.in_place = to_table == block_table;
+  a.in_place = to_table == block_table && (to_stride == bt_stride || B == 1);
   hipStream_t s = static_cast<hipStream_t>(stream);
   for (int l0 = 0; l0 < n_layers; l0 += kMaxLayers) {
     const int layers = std::min(n_layers - l0, kMaxLayers);

@@ -478,7 +478,7 @@ extern "C" int mi_prompt_weights_schedule(const int32_t* host_cu_seqlens, int n_
     n_keys += (L + kKeys - 1) / kKeys;
     for (int rb = 0; rb < row_blocks(obs); ++rb) steps += last_key(L, obs, rb) / kStep + 1;
   }
-  if (n_units * H_kv > (1 << 26) || n_keys * H_kv > INT32_MAX) {
+  if (n_units * H_kv > (1 << 26) || n_keys * H_kv >= (1 << 24)) {
     return fail(MI_ERR_UNSUPPORTED, "mi_prompt_weights_schedule: too many rows or keys");
   }
   // pieces of at most an even share of the work over 512 workgroups (two per CU), at most kMaxPieces per row block: many
@@ -505,7 +505,7 @@ extern "C" int mi_prompt_weights_schedule(const int32_t* host_cu_seqlens, int n_
   }
   const int64_t words64 = kHeader + int64_t(kPieceWords) * pieces.size() + int64_t(kJoinWords) * joins.size() +
                           int64_t(kBlockWords) * blocks.size();
-  if (words64 > INT32_MAX || int64_t(pieces.size()) * H_kv > INT32_MAX) {
+  if (words64 > INT32_MAX || int64_t(pieces.size()) * H_kv >= (1 << 24)  /* 2^32 threads */) {
     return fail(MI_ERR_UNSUPPORTED, "mi_prompt_weights_schedule: schedule too large");
   }
   const int words = int(words64);

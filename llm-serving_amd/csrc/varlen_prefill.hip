@@ -1377,7 +1377,7 @@ __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefil
       // workgroup-uniform: only a tile that reaches past the segment end or the diagonal
       // needs the mask
       bool hides = (t + 1) * BK > L || (causal && (t + 1) * BK - 1 > it.row0);
-      if constexpr (kWin) {  // a tile at either edge hides nothing from some waves (25.2 us against 24.7, as above)
+      if constexpr (kWin) {  // a tile at either edge hides nothing from some waves (25.2 us against 24.7, 4311 tokens under 256)
         const int k0 = t * BK + kh * 32, q0 = it.row0 + qb * 32;
         hides = k0 + 32 > min(L, q0 + 1) || (k0 + window <= q0 + 31 && k0 + 32 > sinks);
       }

@@ -22,7 +22,7 @@ from typing import Any, Callable, Iterable, NamedTuple
 
 import torch
 
-__all__ = ["Rule", "enforce", "as_index", "is_pow2", "same_device", "positive_int"]
+__all__ = ["Rule", "enforce", "as_index", "is_pow2", "same_device", "positive_int", "rows_apart"]
 
 
 class Rule(NamedTuple):
@@ -57,6 +57,18 @@ def same_device(a: torch.device, b: torch.device) -> bool:
     if a.type != b.type:
         return False
     return a.index is None or b.index is None or a.index == b.index
+
+
+def rows_apart(t: torch.Tensor) -> bool:
+    """Whether no two rows (along the last, contiguous dimension) of a tensor that is written share an element,
+    as those of an expanded one do. Rows woven into each other's gaps are taken to."""
+    extent = t.shape[-1]
+    for stride, size in sorted(zip(t.stride()[:-1], t.shape[:-1])):
+        if size > 1:
+            if stride < extent:
+                return False
+            extent += stride * (size - 1)
+    return True
 
 
 def positive_int(name: str, value) -> int:

@@ -39,7 +39,7 @@ from types import SimpleNamespace
 import torch
 
 from . import _lib
-from ._contract import Rule, as_index, enforce, is_pow2
+from ._contract import Rule, as_index, enforce, is_pow2, rows_apart
 
 __all__ = ["TRITON_AVAILABLE", "HIP_AVAILABLE", "paged_decode", "paged_decode_plan", "PagedDecodePlan"]
 
@@ -299,7 +299,7 @@ class PagedDecodePlan:
 
     __slots__ = ("n_layer", "geometry", "q_signature", "_k_ptrs", "_v_ptrs", "_pools",
                  "_table", "_seqlen", "_strides", "_scale", "_ws", "_ws_bytes", "_frozen", "_band",
-                 "_weigh_ws", "_weigh_shape", "_layout", "_fixed", "_reads", "_weigh_args")
+                 "_weigh_ws", "_weigh_shape", "_weigh_strides", "_layout", "_fixed", "_reads", "_weigh_args")
 
     def __init__(self, q, k_caches, v_caches, block_table, seqlen, *, scale=None, window=None, sinks=0) -> None:
         self._band = check_window(window, sinks)
@@ -342,6 +342,7 @@ class PagedDecodePlan:
             self._fixed += (*map(ctypes.c_int, self._band), ctypes.c_void_p(self._frozen[-2]), ctypes.c_size_t(self._ws_bytes))
         self._weigh_ws = None  # run_weighed's workspace, taken at its first call, and its last arguments
         self._weigh_shape = torch.Size((g.rows, g.kv_heads, g.capacity))
+        self._weigh_strides = None  # that run_weighed has looked over
 
     def run(self, layer: int, q):
         """Launch one layer; ``q`` must have the layout the plan was built with."""
@@ -393,11 +394,13 @@ class PagedDecodePlan:
         if self._band is not None:
             raise ValueError("run_weighed accounts for every token of a row; this plan is under a window")
         self._check_query(layer, q, "run_weighed")
-        row, head, last = weights.stride() if weights.dim() == 3 else (0, 0, 0)
-        if (weights.shape != self._weigh_shape or last != 1 or weights.dtype != torch.float32
-                or weights.get_device() != self._layout[3]):
-            raise ValueError(f"weights must be fp32 {tuple(self._weigh_shape)} on {q.device} with contiguous rows, got "
-                             f"{weights.dtype} {tuple(weights.shape)} strides {weights.stride()} on {weights.device}")
+        strides = weights.stride()
+        if (weights.shape != self._weigh_shape or strides[2] != 1 or weights.dtype != torch.float32
+                or weights.get_device() != self._layout[3]
+                or strides != self._weigh_strides and not rows_apart(weights)):
+            raise ValueError(f"weights must be fp32 {tuple(self._weigh_shape)} on {q.device} with contiguous rows apart, "
+                             f"got {weights.dtype} {tuple(weights.shape)} strides {strides} on {weights.device}")
+        self._weigh_strides = strides
         device = self.q_signature[2]
         with _lib.on_device(device):
             if self._weigh_ws is None:
@@ -406,7 +409,7 @@ class PagedDecodePlan:
                 self._weigh_args = (ctypes.c_void_p(self._weigh_ws.data_ptr()), ctypes.c_size_t(n))
             out = torch.empty_like(q)
             rc = _lib.lib.mi_paged_decode_weigh(q.data_ptr(), *self._reads[layer], out.data_ptr(), *self._fixed,
-                                                weights.data_ptr(), row, head, *self._weigh_args,
+                                                weights.data_ptr(), *strides[:2], *self._weigh_args,
                                                 _lib.current_stream(device))
         if rc:
             _lib.check(rc, "paged_decode_plan.run_weighed")
@@ -461,14 +464,15 @@ class PagedDecodePlan:
         k, v = self._pools[0][layer], self._pools[1][layer]
         fused, band = (_lib.lib.mi_paged_decode_fused, ()) if self._band is None else \
             (_lib.lib.mi_paged_decode_fused_window, self._band)
-        rc = fused(
-            source.data_ptr(), row_stride, n_parts, q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(),
-            sin.data_ptr(), int(cos.shape[0]), rotary, pos.data_ptr(), slot_ids.data_ptr(),
-            8 * slot_ids.element_size(), k.data_ptr(), v.data_ptr(), self._table.data_ptr(), self._seqlen.data_ptr(),
-            out.data_ptr(), *g.dims(), int(k.shape[0]) * int(k.shape[1]), self._strides, self._scale, float(eps), 0,
-            _lib.dtype_code(dtype), *band, None if self._ws is None else self._ws.data_ptr(), self._ws_bytes,
-            None if error_word is None else error_word.data_ptr(), _lib.current_stream(out.device),
-        )
+        with _lib.on_device(out.device):
+            rc = fused(
+                source.data_ptr(), row_stride, n_parts, q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(),
+                sin.data_ptr(), int(cos.shape[0]), rotary, pos.data_ptr(), slot_ids.data_ptr(),
+                8 * slot_ids.element_size(), k.data_ptr(), v.data_ptr(), self._table.data_ptr(), self._seqlen.data_ptr(),
+                out.data_ptr(), *g.dims(), int(k.shape[0]) * int(k.shape[1]), self._strides, self._scale, float(eps), 0,
+                _lib.dtype_code(dtype), *band, None if self._ws is None else self._ws.data_ptr(), self._ws_bytes,
+                None if error_word is None else error_word.data_ptr(), _lib.current_stream(out.device),
+            )
         _lib.check(rc, "paged_decode_plan.run_fused")
         return out
 

@@ -35,7 +35,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._contract import Rule, as_index, enforce, is_pow2, positive_int, same_device
+from ._contract import Rule, as_index, enforce, is_pow2, positive_int, rows_apart, same_device
 from .decode import TRITON_AVAILABLE, check_window, paged_decode_plan
 from .rows import Parts
 
@@ -82,10 +82,10 @@ _EVICT = (
                                f"place), got {a.seqlen.dtype} {tuple(a.seqlen.shape)}"),
     Rule(lambda a: a.weights.dtype != torch.float32 or tuple(a.weights.shape) != (
         a.pool.n_layer, a.table.shape[0], a.pool.n_kv_head, a.table.shape[1] * a.pool.block_size)
-        or a.weights.stride(3) != 1, ValueError,
+        or a.weights.stride(3) != 1 or not rows_apart(a.weights), ValueError,
          lambda a: f"weights must be fp32 ({a.pool.n_layer}, {a.table.shape[0]}, {a.pool.n_kv_head}, "
-                   f"{a.table.shape[1] * a.pool.block_size}) with contiguous rows, got {a.weights.dtype} "
-                   f"{tuple(a.weights.shape)}"),
+                   f"{a.table.shape[1] * a.pool.block_size}) with contiguous rows apart, got {a.weights.dtype} "
+                   f"{tuple(a.weights.shape)} strides {a.weights.stride()}"),
     Rule(lambda a: not all(same_device(t.device, a.pool.device) for t in (a.table, a.to, a.seqlen, a.weights)), ValueError,
          lambda a: f"the pool is on {a.pool.device}; got block_table on {a.table.device}, to on {a.to.device}, seqlen on "
                    f"{a.seqlen.device}, weights on {a.weights.device}"),
@@ -412,10 +412,8 @@ class PagedPool:
         of ``block_table`` lies, and its old ones stay as they are (shared blocks of a fork, say). No host
         wait; a row whose tables name a block outside the pool loses those tokens and is reported by
         :meth:`check_writes` (as token ``b``)."""
-        budget, recent, sinks = (as_index(x, n) for x, n in ((budget, "budget"), (recent, "recent"), (sinks, "sinks")))
         target = block_table if to is None else to
-        enforce(_EVICT, SimpleNamespace(pool=self, table=block_table, to=target, seqlen=seqlen, weights=weights,
-                                        budget=budget, recent=recent, sinks=sinks))
+        budget, recent, sinks = self._check_evict(block_table, target, seqlen, weights, budget, recent, sinks)
         if block_table.shape[0] == 0:
             return
         if not self._on_device:
@@ -441,6 +439,12 @@ class PagedPool:
         _lib.check(rc, "PagedPool.evict")
         if self.strict_writes:
             self.check_writes()
+
+    def _check_evict(self, table, to, seqlen, weights, budget, recent, sinks) -> tuple[int, int, int]:
+        budget, recent, sinks = (as_index(x, n) for x, n in ((budget, "budget"), (recent, "recent"), (sinks, "sinks")))
+        enforce(_EVICT, SimpleNamespace(pool=self, table=table, to=to, seqlen=seqlen, weights=weights, budget=budget,
+                                        recent=recent, sinks=sinks))
+        return budget, recent, sinks
 
     def _evict_host(self, table, to, seqlen, weights, budget: int, recent: int, sinks: int) -> None:
         bs = self.block_size

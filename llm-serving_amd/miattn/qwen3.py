@@ -30,6 +30,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
+from ._contract import as_index
 from .decode import check_window
 from .fp4 import Fp4PagedPool
 from .packed import PackedPrefill
@@ -254,6 +255,8 @@ class Qwen3:
         decode. ``weights`` (fp32 ``(n_layer, n_prompts, n_kv_head, at least the longest prompt)``) is filled with
         where each prompt's last ``observe`` queries look, per layer (``PackedPrefill.weigh``)."""
         c = self.cfg
+        if weights is not None and c.window is not None:
+            raise ValueError("an account is of attention over whole prompts; this model's is under a window")
         packed, tokens = PackedPrefill.upload(prompts, pool, tables, self.device)
         x = F.embedding(tokens, self.w["embed"])  # (T, C), the residual stream (updated in place)
         T = x.shape[0]
@@ -463,7 +466,8 @@ class BudgetDecoder:
         if c.window is not None:
             raise ValueError("a model under a window sees a bounded number of tokens by itself")
         self.model, self.pool, self.weights = model, pool, weights
-        self.budget, self.recent, self.sinks, self.every = int(budget), int(recent), int(sinks), int(every)
+        self.budget, self.recent, self.sinks, self.every = (
+            as_index(x, n) for x, n in ((budget, "budget"), (recent, "recent"), (sinks, "sinks"), (every, "every")))
         if self.every < 1:
             raise ValueError(f"every must be >= 1, got {every}")
         self.B = len(tables)
@@ -479,6 +483,7 @@ class BudgetDecoder:
         self.pos = torch.tensor(lengths, dtype=torch.long, device=dev)
         self.held = self.pos.clone()  # the place of the next token in the row's cache
         self.seqlen = self.pos.to(torch.int32)
+        pool._check_evict(self.table, self.table, self.seqlen, weights, self.budget, self.recent, self.sinks)
         self.tokens = first_tokens.to(dev, torch.long).clone()
         self.history = torch.zeros(self.B, max_new, dtype=torch.long, device=dev)
         self.step_idx = torch.zeros(self.B, dtype=torch.long, device=dev)
@@ -520,6 +525,8 @@ class BudgetDecoder:
 
     def capture(self, stream=None) -> None:
         """Record one step (run once eagerly first, its effects undone: the K/V that it wrote lie past the rows)."""
+        if self._most >= self.budget + self.every:  # as step() does: the step needs a free place
+            self.evict()
         state = (self.pos, self.held, self.tokens, self.seqlen, self.step_idx, self.weights, self.history)
         saved = [t.clone() for t in state]
         self._step()

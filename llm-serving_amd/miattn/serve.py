@@ -457,11 +457,14 @@ class ContinuousServer:
     def _give_hidden(self, seat, active) -> None:
         """Hand back the blocks that have left a seat's window; its device table keeps their ids, unread."""
         req, blocks, n = active[seat]
-        gone = [j for j in self._hidden(len(req.prompt) + n) if blocks[j] is not None]
+        gone = []
+        for j in reversed(self._hidden(len(req.prompt) + n)):
+            if blocks[j] is None:  # and so are those before it
+                break
+            gone.append(blocks[j])
+            blocks[j] = None
         if gone:
-            self.blocks.give_back([blocks[j] for j in gone])
-            for j in gone:
-                blocks[j] = None
+            self.blocks.give_back(gone[::-1])
 
     def _finish(self, seat, active, free_seats, records, t) -> None:
         req, blocks, n = active.pop(seat)

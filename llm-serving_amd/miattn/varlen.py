@@ -42,7 +42,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from ._contract import Rule, as_index, enforce
+from ._contract import Rule, as_index, enforce, rows_apart
 from .decode import check_window
 
 __all__ = ["HipVarlen", "SdpaVarlen", "backend_for", "check_prefill_errors", "segment_bounds", "validate_packed"]
@@ -134,6 +134,12 @@ def _scale(softmax_scale, head_dim: int) -> float:
     return float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(head_dim)
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as the kernels load it: contiguous, from a 16-byte boundary on."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _check_band(window, sinks, causal) -> tuple[int, int] | None:
     band = check_window(window, sinks)
     if band is not None and not causal:
@@ -160,8 +166,8 @@ def _observed(q, k, cu_seqlens, max_seqlen, observe, out) -> tuple[list[int], in
     if out is None:
         out = torch.empty((*want, longest), dtype=torch.float32, device=q.device)
     elif (out.dim() != 3 or tuple(out.shape[:2]) != want or out.shape[2] < longest or out.dtype != torch.float32
-          or out.device != q.device or out.stride(2) != 1):
-        raise ValueError(f"out must be fp32 ({want[0]}, {want[1]}, at least {longest}) on {q.device} with contiguous rows, "
+          or out.device != q.device or out.stride(2) != 1 or not rows_apart(out)):
+        raise ValueError(f"out must be fp32 ({want[0]}, {want[1]}, at least {longest}) on {q.device} with contiguous rows apart, "
                          f"got {out.dtype} {tuple(out.shape)} strides {out.stride()} on {out.device}")
     return bounds, observe, out
 
@@ -226,24 +232,32 @@ class _Schedules:
 
     def get(self, bounds: list[int], H: int, H_kv: int, D: int, causal: bool, device, kernel: int, band=None):
         key = (tuple(bounds), H, H_kv, D, bool(causal), device, kernel)
-        return self._get(key if band is None else (*key, band), lambda: (
+        return self._get(key if band is None else (*key, band), device, lambda: (
             self._build(bounds, H, H_kv, D, causal, device, kernel) if band is None else
             self._build_window(bounds, H, H_kv, D, band, device)))
 
     def get_weights(self, bounds: list[int], H: int, H_kv: int, D: int, observe: int, device):
         """The launch state of ``prompt_weights``: no workspace in it (no launch depends on the last one's)."""
-        return self._get(("weights", tuple(bounds), H, H_kv, D, observe, device),
+        return self._get(("weights", tuple(bounds), H, H_kv, D, observe, device), device,
                          lambda: self._build_weights(bounds, H, H_kv, D, observe, device))
 
-    def _get(self, key, build):
+    def _get(self, key, device, build):
         entry = self._pinned.get(key) or self._lru.get(key)
+        stream = _lib.current_stream(device)
         if entry is None:
             entry = build()
+            entry.stream = stream
             self._lru[key] = entry
             while len(self._lru) > self.capacity:
                 self._lru.popitem(last=False)
-        elif key in self._lru:
-            self._lru.move_to_end(key)
+        else:
+            if key in self._lru:
+                self._lru.move_to_end(key)
+            if stream != entry.stream and not torch.cuda.is_current_stream_capturing():
+                # its memory is given back for use on another stream than this launch's
+                for t in vars(entry).values():
+                    if isinstance(t, torch.Tensor):
+                        t.record_stream(torch.cuda.current_stream(device))
         if torch.cuda.is_current_stream_capturing():
             self._pinned[key] = entry
         return entry
@@ -404,7 +418,7 @@ class HipVarlen:
     def _windowed(self, q, k, v, bounds, band, longest: int, scale: float):
         total, H, D = q.shape
         H_kv = int(k.shape[1])
-        q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v))
+        q, k, v = map(_aligned, (q, k, v))
         band = tuple(min(x, longest) for x in band)  # what lies past the longest segment hides nothing
         with _lib.on_device(q.device):
             plan = _SCHEDULES.get(bounds, H, H_kv, D, True, q.device, -1, band)
@@ -435,7 +449,7 @@ class HipVarlen:
                                "backend_for() gives host tensors the SDPA arm")
         if q.dtype not in (torch.float16, torch.bfloat16):
             raise RuntimeError(f"the MFMA varlen kernels compute fp16/bf16 only, got {q.dtype}")
-        q, k = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.contiguous().clone() for t in (q, k))
+        q, k = map(_aligned, (q, k))
         H, H_kv, D = int(q.shape[1]), int(k.shape[1]), int(q.shape[2])
         with _lib.on_device(q.device):
             plan = _SCHEDULES.get_weights(bounds, H, H_kv, D, observe, q.device)

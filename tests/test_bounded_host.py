@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from miattn import PagedPool, SdpaVarlen, _lib, paged_decode, paged_decode_plan
+from miattn._contract import rows_apart
 from miattn.decode import check_window
 from miattn.qwen3 import Qwen3Config
 from miattn.serve import BlockFreeList, ContinuousServer
@@ -134,11 +135,21 @@ def test_account_refusals():
     for observe in (0, -1, True, 2.0):
         with pytest.raises(ValueError, match="observe"):
             arm.prompt_weights(q, k, cu_seqlens=[0, 5], max_seqlen=5, observe=observe)
-    for out in (torch.zeros(1, 2, 4), torch.zeros(1, 4, 5), torch.zeros(1, 2, 5).double(), torch.zeros(1, 5, 2).transpose(1, 2)):
+    for out in (torch.zeros(1, 2, 4), torch.zeros(1, 4, 5), torch.zeros(1, 2, 5).double(), torch.zeros(1, 5, 2).transpose(1, 2),
+                torch.zeros(1, 1, 5).expand(1, 2, 5), torch.zeros(9).as_strided((1, 2, 5), (9, 4, 1))):
         with pytest.raises(ValueError, match="out must be"):
             arm.prompt_weights(q, k, cu_seqlens=[0, 5], max_seqlen=5, out=out)
     with pytest.raises(ValueError, match="3-D"):
         arm.prompt_weights(q[0], k, cu_seqlens=[0, 5], max_seqlen=5)
+
+
+def test_rows_that_are_written_lie_apart():
+    t = torch.zeros(3, 4, 5, 6)
+    for ok in (t, t.transpose(0, 2), t[:, ::2, 1:, :4], t[:1].expand(1, 4, 5, 6), t[:0], t[:, 0], t[0, 0, 0]):
+        assert rows_apart(ok)
+    for bad in (t[:1].expand(3, 4, 5, 6), t[:, :, :1].expand(3, 4, 5, 6), torch.zeros(20).as_strided((2, 6), (5, 1)),
+                torch.zeros(99).as_strided((3, 4, 6), (12, 6, 1))):
+        assert not rows_apart(bad)
 
 
 def test_eviction_refusals():
@@ -157,7 +168,8 @@ def test_eviction_refusals():
         pool.evict(table, seqlen.long(), weights, **good)
     with pytest.raises(ValueError, match="seqlen"):
         pool.evict(table, torch.zeros(3, dtype=torch.int32), weights, **good)
-    for w in (weights.double(), weights[:1], weights[..., :11], torch.zeros(2, 2, 12, 2).transpose(2, 3)):
+    for w in (weights.double(), weights[:1], weights[..., :11], torch.zeros(2, 2, 12, 2).transpose(2, 3),
+              weights[:, :1].expand(2, 2, 2, 12), weights[:1].expand(2, 2, 2, 12)):
         with pytest.raises(ValueError, match="weights must be"):
             pool.evict(table, seqlen, w, **good)
     with pytest.raises(ValueError, match="a row for each"):

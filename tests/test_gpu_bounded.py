@@ -313,7 +313,8 @@ def test_weighed_decode_refusals(cuda):
     q, k, v, table, seqlen = _cuda(*_rows([40], 4, 2, 64, BF16, 16))
     plan = paged_decode_plan(q, [k], [v], table, seqlen)
     good = torch.zeros(1, 2, 48, device=cuda)
-    for bad in (good[..., :47], good.double(), good.cpu(), good[:, :1], torch.zeros(1, 48, 2, device=cuda).transpose(1, 2)):
+    for bad in (good[..., :47], good.double(), good.cpu(), good[:, :1], torch.zeros(1, 48, 2, device=cuda).transpose(1, 2),
+                good[:, :1].expand(1, 2, 48), good[0]):
         with pytest.raises(ValueError, match="weights must be"):
             plan.run_weighed(0, q, bad)
     with pytest.raises(IndexError, match="outside the plan"):
@@ -626,6 +627,76 @@ def test_budget_decoder_refusals(cuda):
         BudgetDecoder(*args, budget=30, recent=10, every=0)
     with pytest.raises(ValueError, match="by itself"):
         BudgetDecoder(_tiny(cuda, window=8), *args[1:], budget=30, recent=10)
+    with pytest.raises(ValueError, match="must be positive and hold"):
+        BudgetDecoder(*args, budget=30, recent=28, sinks=4, every=10)
+    with pytest.raises(ValueError, match="weights must be"):
+        BudgetDecoder(*args[:6], account[:1], budget=30, recent=10, every=10)
+    with pytest.raises(ValueError, match="4-bit pool"):
+        four = Fp4PagedPool(2, 16, 16, 2, 128, dtype=BF16, device=cuda, n_head=4)
+        BudgetDecoder(m, four, *args[2:], budget=30, recent=10, every=10)
+    with pytest.raises(ValueError, match="under a window"):
+        _tiny(cuda, window=8).prefill([[1, 2]], pool, [[0]], weights=account)
+
+
+def test_budget_decoder_captured_with_its_rows_full(cuda):
+    """The step that is recorded needs a free place: a decoder whose rows have grown to the end of their tables cuts them."""
+    m = _tiny(cuda)
+    pool, account = m.new_pool(8), torch.zeros(2, 1, 2, 48, device=cuda)
+    first = m.prefill([list(range(20))], pool, [[5, 1, 2]], weights=account).argmax(-1)
+    d = BudgetDecoder(m, pool, [[5, 1, 2]], [20], first, 90, account, budget=38, recent=8, sinks=2, every=10)
+    for _ in range(28):
+        d.step()
+    assert d.seqlen.tolist() == [48]
+    d.capture()
+    assert d.held.tolist() == [38]
+    for _ in range(40):
+        d.step()
+    d.check()
+    assert d.pos.tolist() == [88] and d.held.tolist() == [48]
+
+
+def test_calls_beside_each_other_on_two_streams(cuda):
+    """Two plans, two packed groups and two pools, one on a stream each, among other calls that push the groups' schedules
+    out: what each gives is what it gives alone."""
+    g = torch.Generator().manual_seed(11)
+    sides = []
+    for i in range(2):
+        q, k, v, table, seqlen = _cuda(*_rows([900 + 31 * i, 40, 300], 16, 8, 128, BF16, 16, seed=i))
+        prompt = [torch.randn(700 + i, h, 128, generator=g).bfloat16().cuda() for h in (16, 8, 8)]
+        pool = PagedPool(1, 64, 16, 8, 128, dtype=BF16, device=cuda, n_head=16)
+        rows = torch.randperm(64, generator=g).int().view(2, 32).cuda()
+        start = [torch.randn(64, 16, 8, 128, generator=g).bfloat16().cuda() for _ in range(2)]
+        weights = torch.rand(1, 2, 8, 512, generator=g).cuda()
+        sides.append((q, k, v, table, seqlen, prompt, pool, rows, start, weights, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def go(q, k, v, table, seqlen, prompt, pool, rows, start, weights, stream):
+        account = torch.zeros(3, 8, table.shape[1] * 16, device=cuda)
+        outs = [paged_decode_plan(q, [k], [v], table, seqlen, window=200, sinks=3).run(0, q),
+                paged_decode_plan(q, [k], [v], table, seqlen).run_weighed(0, q, account), account]
+        args = dict(cu_seqlens=[0, prompt[0].shape[0]], max_seqlen=prompt[0].shape[0])
+        for j in range(10):  # more groups than are kept
+            x = prompt[0][: 40 + j]
+            HipVarlen().prefill_varlen(x, prompt[1][: 40 + j], prompt[2][: 40 + j], cu_seqlens=[0, 40 + j],
+                                       max_seqlen=40 + j, window=9)
+            outs.append(HipVarlen().prefill_varlen(*prompt, **args, window=90, sinks=5))
+            outs.append(HipVarlen().prompt_weights(*prompt[:2], **args))
+        pool.keys[0].copy_(start[0])
+        pool.values[0].copy_(start[1])
+        w, n = weights.clone(), torch.tensor([500, 200], dtype=torch.int32).to(cuda)
+        pool.evict(rows, n, w, budget=100, recent=30, sinks=4)
+        return outs + [pool.keys[0].clone(), pool.values[0].clone(), w, n]
+
+    alone = [go(*s) for s in sides]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        both = []
+        for s in sides:
+            with torch.cuda.stream(s[-1]):
+                both.append(go(*s))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, both):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 def test_a_windowed_model_served_from_a_pool_that_holds_its_windows_only(cuda):
