@@ -12,8 +12,9 @@
 // (token, KV head), 50 us for 235 MB and 116 us for 510 MB with places drawn at random, 4.4 to 4.7 TB/s of the 5.1 that
 // a large copy reaches. K and V have workgroups of their own; where the rows go to other blocks, so have stretches
 // of a row. In place, one workgroup goes up a row: p <= kept[p], so a stretch's sources are never below the
-// places already written, and a barrier between its loads and its stores is all the order that it needs (a row of
-// 1088 tokens cut to 1024 in 28 layers 109 us with the host's share, 32 of them 1606, 4.7 TB/s).
+// places already written, and a barrier between its loads and its stores is all the order that it needs; it is as large
+// as one may be, for fewer of them (a row of 1088 tokens cut to 1024 in 28 layers 88 us with the host's share, 32 of them
+// 1567, 4.8 TB/s; with 256 threads 110 and 1610).
 #include <algorithm>
 
 #include "common.h"
@@ -198,13 +199,12 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   look_up();
 }
 
-constexpr int kMoveThreads = 256;
 constexpr int kPerThread = 8;  // 16-byte loads of a thread before its first store
 
 // LPR lanes of 16 bytes per (token, KV head) row.
-template <int LPR>
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
-  constexpr int kRows = kMoveThreads / LPR, kStretch = kRows * kPerThread, kRowBytes = LPR * 16;
+template <int LPR, int NT>
+__global__ __launch_bounds__(NT) void evict_move_kernel(EvictArgs a) {
+  constexpr int kRows = NT / LPR, kStretch = kRows * kPerThread, kRowBytes = LPR * 16;
   const int tid = threadIdx.x;
   const int l = blockIdx.x / (a.B * a.H_kv), bh = blockIdx.x - l * (a.B * a.H_kv);
   const int b = bh / a.H_kv, h = bh - b * a.H_kv;
@@ -215,11 +215,11 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
   if (blockIdx.y == 2) {  // the weights, and (once) the row's length: in place, one workgroup
     if (!cut || blockIdx.z != 0) return;
     float* w = a.weights + l * a.ws0 + b * a.ws1 + h * a.ws2;
-    for (int p0 = 0; p0 < keep; p0 += kMoveThreads * kPerThread) {
+    for (int p0 = 0; p0 < keep; p0 += NT * kPerThread) {
       float x[kPerThread];
 #pragma unroll
       for (int j = 0; j < kPerThread; ++j) {
-        const int p = p0 + j * kMoveThreads + tid;
+        const int p = p0 + j * NT + tid;
         x[j] = p < keep ? w[kept[p]] : 0.0f;
       }
 #pragma unroll
@@ -227,11 +227,11 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < kPerThread; ++j) {
-        const int p = p0 + j * kMoveThreads + tid;
+        const int p = p0 + j * NT + tid;
         if (p < keep) w[p] = x[j];
       }
     }
-    for (int i = keep + tid; i < n; i += kMoveThreads) w[i] = 0.0f;
+    for (int i = keep + tid; i < n; i += NT) w[i] = 0.0f;
     if (a.last && l == 0 && h == 0 && tid == 0) a.seqlen[b] = keep;
     return;
   }
@@ -273,9 +273,13 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
 
 template <int LPR>
 int launch_move(const EvictArgs& a, int layers, hipStream_t s) {
-  constexpr int stretch = kMoveThreads / LPR * kPerThread;
-  const int nz = a.in_place ? 1 : std::min((a.budget + stretch - 1) / stretch, 256);
-  hipLaunchKernelGGL((evict_move_kernel<LPR>), dim3(layers * a.B * a.H_kv, 3, nz), dim3(kMoveThreads), 0, s, a);
+  if (a.in_place) {
+    hipLaunchKernelGGL((evict_move_kernel<LPR, 1024>), dim3(layers * a.B * a.H_kv, 3), dim3(1024), 0, s, a);
+  } else {
+    constexpr int stretch = 256 / LPR * kPerThread;
+    const int nz = std::min((a.budget + stretch - 1) / stretch, 256);
+    hipLaunchKernelGGL((evict_move_kernel<LPR, 256>), dim3(layers * a.B * a.H_kv, 3, nz), dim3(256), 0, s, a);
+  }
   return launch_status("mi_cache_evict (move)");
 }
 
@@ -316,7 +320,7 @@ extern "C" int mi_cache_evict(void* const* host_k_pools, void* const* host_v_poo
     return fail(MI_ERR_INVALID, "mi_cache_evict: %d destination blocks of %d do not hold %d tokens", to_blocks, block_size, budget);
   }
   if (B == 0 || n_layers == 0) return MI_OK;
-  if (B > 65535 || int64_t(std::min(n_layers, kMaxLayers)) * B * H_kv >= (1 << 24)  /* 2^32 threads */) {
+  if (B > 65535 || int64_t(std::min(n_layers, kMaxLayers)) * B * H_kv >= (1 << 22)  /* 2^32 threads */) {
     return fail(MI_ERR_UNSUPPORTED, "mi_cache_evict: grid too large (B=%d, H_kv=%d)", B, H_kv);
   }
   if (host_k_pools == nullptr || host_v_pools == nullptr || block_table == nullptr || to_table == nullptr ||
