@@ -12,6 +12,11 @@ Drop-in modules, each mirroring one reference interface:
   4 bits (no reference counterpart);
 * :mod:`miattn.packed`  -- ``PackedPrefill`` (reference ``model/packed.py``).
 
+Caches of bounded length (no reference counterpart): ``window=`` and ``sinks=`` on ``paged_decode``, ``paged_decode_plan``,
+``PagedKV``, ``prefill_varlen`` and ``PackedPrefill.attend``; accounts of attention weights by
+``PagedDecodePlan.run_weighed``, ``prompt_weights`` and ``PackedPrefill.weigh``, and ``PagedPool.evict`` by them;
+``miattn.qwen3`` has the model paths (``Qwen3Config(window=, sinks=)``, ``BudgetDecoder``).
+
 Device work on a HIP device goes through ``libmiattn.so`` (C ABI in ``include/miattn.h``);
 when the library is missing those entry points raise instead of computing anything another
 way. Host (CPU) pools and the CPU prefill arm behave as the reference's own host arms.
