@@ -2953,8 +2953,7 @@ extern "C" int mi_varlen_prefill(const void* q, const void* k, const void* v, vo
 }
 
 // The windowed form's schedule and launch. A window (or sinks) past the longest segment hides nothing, so both are
-// held to it; the launch takes the same two numbers (with others the items' key ranges would not be
-// those that the schedule dealt out, which costs balance and nothing else).
+// held to it; the launch takes the same two numbers, by which an item's piece finds its key tiles.
 namespace miattn {
 namespace {
 
