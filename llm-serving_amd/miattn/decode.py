@@ -331,18 +331,24 @@ class PagedDecodePlan:
         # the launch arguments after ``out`` that no run changes (the plan owns the workspace)
         self._frozen = (*g.dims(), self._strides, self._scale, _lib.dtype_code(q.dtype),
                         None if self._ws is None else self._ws.data_ptr(), self._ws_bytes)
-        # The windowed and weighed calls' arguments as ctypes takes them, and the query's layout as its attributes come:
-        # an eager step of 28 layers over short rows waits for the host, 10 us a call, most of it two launches
-        self._layout = (q.shape, q.dtype, q.stride(), q.get_device())
-        self._fixed = (*map(ctypes.c_int, g.dims()), self._strides, ctypes.c_float(self._scale),
-                       ctypes.c_int(_lib.dtype_code(q.dtype)))
-        self._reads = [tuple(map(ctypes.c_void_p, (k, v, block_table.data_ptr(), seqlen.data_ptr())))
-                       for k, v in zip(self._k_ptrs, self._v_ptrs)]
         if self._band is not None:
+            self._bind(q)
             self._fixed += (*map(ctypes.c_int, self._band), ctypes.c_void_p(self._frozen[-2]), ctypes.c_size_t(self._ws_bytes))
+        else:
+            self._layout = None  # bound by the first weighed run
         self._weigh_ws = None  # run_weighed's workspace, taken at its first call, and its last arguments
         self._weigh_shape = torch.Size((g.rows, g.kv_heads, g.capacity))
         self._weigh_strides = None  # that run_weighed has looked over
+
+    def _bind(self, q) -> None:
+        """The windowed and weighed calls' arguments as ctypes takes them, and the query's layout as its attributes come:
+        an eager step of 28 layers over short rows waits for the host, 10 us a call, most of it two launches."""
+        shape, dtype, device, strides = self.q_signature
+        self._layout = (torch.Size(shape), dtype, strides, q.get_device())
+        self._fixed = (*map(ctypes.c_int, self.geometry.dims()), self._strides, ctypes.c_float(self._scale),
+                       ctypes.c_int(_lib.dtype_code(dtype)))
+        self._reads = [tuple(map(ctypes.c_void_p, (k, v, self._table.data_ptr(), self._seqlen.data_ptr())))
+                       for k, v in zip(self._k_ptrs, self._v_ptrs)]
 
     def run(self, layer: int, q):
         """Launch one layer; ``q`` must have the layout the plan was built with."""
@@ -368,6 +374,8 @@ class PagedDecodePlan:
     def _check_query(self, layer: int, q, what: str) -> None:
         if not 0 <= layer < self.n_layer:
             raise IndexError(f"layer {layer} is outside the plan's {self.n_layer} layers")
+        if self._layout is None and q.device == self.q_signature[2]:
+            self._bind(q)
         if (q.shape, q.dtype, q.stride(), q.get_device()) != self._layout:
             raise ValueError(f"paged_decode_plan.{what}: the query does not match the validated layout "
                              f"(built for shape/dtype/device/strides {self.q_signature}, got "

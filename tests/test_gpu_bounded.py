@@ -156,7 +156,8 @@ def test_fused_decode_under_a_window_equals_the_two_launches(heads, cuda):
 # ------------------------------------------------------------------ prompts under a window
 @pytest.mark.parametrize("heads", [(16, 8, 128, BF16), (8, 2, 256, F16), (4, 4, 64, BF16), (6, 1, 128, F16)])
 @pytest.mark.parametrize("lengths,window,sinks", [([1, 64, 65, 300, 2], 1, 0), ([700, 130], 64, 4), ([333], 100, 70),
-                                                  ([513, 5], 63, 129), ([1500], 200, 0), ([128, 129], 1000, 3)])
+                                                  ([513, 5], 63, 129), ([1500], 200, 0), ([128, 129], 1000, 3),
+                                                  ([1300], 1100, 4), ([1], 1, 9), ([900, 400], 500, 17)])
 def test_prompts_under_a_window(heads, lengths, window, sinks, cuda):
     H, H_kv, D, dt = heads
     cu = _cu(lengths)
@@ -171,6 +172,13 @@ def test_prompts_under_a_window(heads, lengths, window, sinks, cuda):
     assert torch.equal(arm.prefill_varlen(*odd, **args), got)
     wide = [torch.stack([t, t], 1).cuda()[:, 0] for t in (q, k, v)]
     assert torch.equal(arm.prefill_varlen(*wide, **args), got)
+
+
+def test_prompts_under_a_window_with_as_many_heads_as_an_item_names(cuda):
+    cu = _cu([130, 70])
+    q, k, v = (torch.randn(200, h, 64).bfloat16() for h in (255, 85, 85))
+    want, bound = bounded.varlen(q, k, v, cu, 40, 3)
+    _within(HipVarlen().prefill_varlen(*_cuda(q, k, v), cu_seqlens=cu, max_seqlen=130, window=40, sinks=3), want, bound)
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
@@ -328,7 +336,8 @@ def test_weighed_decode_refusals(cuda):
         paged_decode_plan(q, [k], [v], table, seqlen).run_weighed(0, q, good)
 
 
-@pytest.mark.parametrize("heads", [(16, 8, 128, BF16), (8, 2, 256, F16), (4, 4, 64, BF16), (12, 1, 128, F16), (3, 3, 64, F16)])
+@pytest.mark.parametrize("heads", [(16, 8, 128, BF16), (8, 2, 256, F16), (4, 4, 64, BF16), (12, 1, 128, F16), (3, 3, 64, F16),
+                                   (64, 1, 64, BF16)])
 @pytest.mark.parametrize("lengths,observe", [([1, 2, 31, 64, 65, 300], 1), ([700, 5, 129], 32), ([200, 33], None),
                                              ([1000], 77), ([400, 90], 1000)])
 def test_account_of_prompts(heads, lengths, observe, cuda):
