@@ -17,6 +17,7 @@
 // 1742 and 306 tokens, H 16 / H_kv 8 / D 128, all queries (49 GFLOP counted once): 71 + 71 us, of which the exponentials
 // alone are 21 each; 8 prompts of 4311 tokens, last 32 queries: 8.3 + 2.0 (join) + 6.8 us, launches and round trips.
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "common.h"
@@ -442,12 +443,8 @@ int launch_any(const void* q, const void* k, int D, const WeightArgs& a, hipStre
   return D == 64 ? launch<T, 64>(q, k, a, s) : D == 128 ? launch<T, 128>(q, k, a, s) : launch<T, 256>(q, k, a, s);
 }
 
-}  // namespace
-}  // namespace miattn
-
-extern "C" int mi_prompt_weights_schedule(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int D,
-                                          int observe, int32_t* host_schedule, int capacity) {
-  using namespace miattn;
+int schedule_weights(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int D, int observe,
+                     int32_t* host_schedule, int capacity) {
   if (host_cu_seqlens == nullptr || n_seqs < 1) {
     return fail(MI_ERR_INVALID, "mi_prompt_weights_schedule: need at least 1 segment, got %d", n_seqs);
   }
@@ -531,6 +528,19 @@ extern "C" int mi_prompt_weights_schedule(const int32_t* host_cu_seqlens, int n_
     w = std::copy(x, x + kBlockWords, w);
   }
   return words;
+}
+
+}  // namespace
+}  // namespace miattn
+
+extern "C" int mi_prompt_weights_schedule(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int D,
+                                          int observe, int32_t* host_schedule, int capacity) {
+  using namespace miattn;
+  try {
+    return schedule_weights(host_cu_seqlens, n_seqs, H, H_kv, D, observe, host_schedule, capacity);
+  } catch (const std::bad_alloc&) {
+    return fail(MI_ERR_UNSUPPORTED, "mi_prompt_weights_schedule: out of host memory");
+  }
 }
 
 extern "C" size_t mi_prompt_weights_workspace_size(const int32_t* host_schedule, int H_kv) {

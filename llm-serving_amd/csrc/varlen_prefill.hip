@@ -30,6 +30,7 @@
 #include <algorithm>
 #include <climits>
 #include <type_traits>
+#include <new>
 #include <vector>
 
 #include "common.h"
@@ -2964,12 +2965,8 @@ int check_window(const char* what, int window, int sinks) {
   return MI_OK;
 }
 
-}  // namespace
-}  // namespace miattn
-
-extern "C" int mi_varlen_schedule_window(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int D,
-                                         int window, int sinks, int32_t* host_schedule, int capacity) {
-  using namespace miattn;
+int schedule_window(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int D, int window, int sinks,
+                    int32_t* host_schedule, int capacity) {
   int rc = check_window("mi_varlen_schedule_window", window, sinks);
   if (rc != MI_OK) return rc;
   if (D != 64 && D != 128 && D != 256) {
@@ -3000,6 +2997,19 @@ extern "C" int mi_varlen_schedule_window(const int32_t* host_cu_seqlens, int n_s
   const int n_partials = cut_tiles(tiles, total, H, D, kDuo, pieces, merges);
   if (n_partials < 0) return n_partials;
   return duo_schedule(host_cu_seqlens, pieces, merges, n_partials, H, H_kv, D, host_schedule, capacity, kBand);
+}
+
+}  // namespace
+}  // namespace miattn
+
+extern "C" int mi_varlen_schedule_window(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv, int D,
+                                         int window, int sinks, int32_t* host_schedule, int capacity) {
+  using namespace miattn;
+  try {
+    return schedule_window(host_cu_seqlens, n_seqs, H, H_kv, D, window, sinks, host_schedule, capacity);
+  } catch (const std::bad_alloc&) {
+    return fail(MI_ERR_UNSUPPORTED, "mi_varlen_schedule_window: out of host memory");
+  }
 }
 
 extern "C" int mi_varlen_prefill_window(const void* q, const void* k, const void* v, void* out,

@@ -5,6 +5,9 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -268,3 +271,22 @@ def test_hidden_blocks_of_a_seat():
 
 def test_config_defaults_see_everything():
     assert Qwen3Config().window is None and Qwen3Config().sinks == 0
+
+
+def test_schedules_past_the_hosts_memory_are_errors():
+    """A schedule that the host cannot hold comes back as an error code: no exception crosses the C entries."""
+    script = """
+import ctypes, resource, sys
+from miattn import _lib
+import torch
+sizes = [(_lib.lib.mi_varlen_schedule_window, 64, 65535 * 64, (64, 0)), (_lib.lib.mi_prompt_weights_schedule, 1, 1 << 29, (1 << 29,))]
+if __name__ == "__main__":
+    held = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+    resource.setrlimit(resource.RLIMIT_AS, (held + (24 << 20),) * 2)
+    for schedule, n, length, args in sizes:
+        cu = (ctypes.c_int32 * (n + 1))(*(i * min(length, (1 << 31) // (n + 1)) for i in range(n + 1)))
+        print(schedule(cu, n, 1, 1, 64, *args, None, 0), "out of host memory" in _lib.last_error(), flush=True)
+"""
+    done = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=100,
+                          env={**os.environ, "PYTHONPATH": os.pathsep.join(sys.path)})
+    assert done.returncode == 0 and done.stdout.split() == ["-2", "True"] * 2, done.stdout + done.stderr
