@@ -739,3 +739,45 @@ def test_a_windowed_model_decodes_what_its_prefill_computes(cuda):
     assert (step.float() - whole.float()).abs().max() <= 12 * 2.0 ** -8 * whole.float().abs().max()
     with pytest.raises(ValueError, match="build the PagedKV with the model's"):
         m.decode(PagedKV(pool, [list(range(10))], [120], rope_len=160, n_head=4), first)
+
+
+# ------------------------------------------------------------------ far ends
+def test_rows_at_the_far_end_of_a_large_pool(cuda):
+    """Pools and accounts whose offsets pass 32 bits give the bits that small ones do."""
+    H, H_kv, D, bs, far = 16, 8, 128, 16, 140000  # 2.3e9 elements of K
+    lengths = [700, 90]
+    q, k, v, table, seqlen = _cuda(*_rows(lengths, H, H_kv, D, BF16, bs))
+    n, width = k.shape[0], table.shape[1] * bs
+    small, large = (PagedPool(1, m, bs, H_kv, D, dtype=BF16, device=cuda, n_head=H) for m in (n, far))
+    for store, part in ((small.keys, k), (small.values, v)):
+        store[0].copy_(part)
+    for store, part in ((large.keys, k), (large.values, v)):
+        store[0][far - n:].copy_(part)
+    room = torch.empty(2**31 + H_kv * width, device=cuda)
+    far_account = room.as_strided((1, 2, H_kv, width), (0, 2**31, width, 1))
+    near = torch.rand(1, 2, H_kv, width, device=cuda)
+    far_account.copy_(near)
+    got = []
+    for pool, at, account in ((small, table, near), (large, torch.where(table < 0, table, table + far - n), far_account)):
+        left = seqlen.clone()
+        outs = [pool.decode_plan(q, at, left, window=100, sinks=4).run(0, q),
+                pool.decode_plan(q, at, left).run_weighed(0, q, account[0])]
+        pool.evict(at, left, account, budget=64, recent=10, sinks=4)
+        outs += [account.clone(), left, pool.decode_plan(q, at, left).run(0, q)]
+        pool.check_writes()
+        got.append(outs)
+    assert got[0][3].tolist() == [64, 64] and all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_a_group_whose_offsets_pass_32_bits(cuda):
+    """The last of 66 long prompts gets what it gets alone."""
+    L, n, H, H_kv, D = 16384, 66, 16, 8, 128  # 2.2e9 elements of q
+    q, k, v = (torch.empty(n * L, h, D, dtype=BF16, device=cuda).normal_() for h in (H, H_kv, H_kv))
+    last = [t[(n - 1) * L:].clone() for t in (q, k, v)]
+    one, all_of = dict(cu_seqlens=[0, L], max_seqlen=L), dict(cu_seqlens=list(range(0, n * L + 1, L)), max_seqlen=L)
+    out = HipVarlen().prefill_varlen(q, k, v, **all_of, window=300, sinks=4)[(n - 1) * L:]
+    assert torch.equal(out, HipVarlen().prefill_varlen(*last, **one, window=300, sinks=4))
+    w = HipVarlen().prompt_weights(q, k, **all_of)[-1]
+    # cut into fewer pieces than alone, so against other reference maxima: exponents below 2^6 are rounded by up to 2^-19 each in a
+    # weight and in its sum's terms, ln 2 of which a weight moves by, and 512 additions in a row add 2^-24 each
+    assert torch.allclose(w, HipVarlen().prompt_weights(*last[:2], **one)[0], rtol=2 * 0.7 * 2.0 ** -19 + 512 * 2.0 ** -24 + 2.0 ** -20, atol=0)
