@@ -431,13 +431,24 @@ def test_eviction(shape, budget, recent, sinks, moved, cuda):
     _check_evicted(pool, seqlen, w, want)
 
 
-@pytest.mark.parametrize("lengths,budget", [([4090, 4096], 700), ([5000, 16384], 2000), ([20011, 300], 1234)])
+@pytest.mark.parametrize("lengths,budget", [([4090, 4096], 700), ([5000, 16384], 2000), ([20011, 300], 1234),
+                                            ([32768, 16385], 5000), ([65536, 40001], 9000), ([70003], 3000)])
 @pytest.mark.parametrize("moved", [False, True])
 def test_eviction_of_long_rows(lengths, budget, moved, cuda):
-    """Accounts in 256 and 1024 threads' registers, and past them."""
+    """Accounts in the registers of 512 and 1024 threads, to the last of them, and past them."""
     pool, table, seqlen, w, to, want = _evict_case(lengths, budget, 100, 4, 1, 16, BF16, 64, n_layer=1, moved=moved)
     pool.evict(table, seqlen, w, budget=budget, recent=100, sinks=4, **({} if to is None else {"to": to}))
     _check_evicted(pool, seqlen, w, want)
+
+
+@pytest.mark.parametrize("n", [4096, 16384, 32768, 65536])
+def test_eviction_of_long_rows_of_equal_weights(n, cuda):
+    """Every weight is at the threshold, as many as the counts hold."""
+    for recent, sinks in ((0, 0), (5, 2)):
+        pool, table, seqlen, w, _, want = _evict_case([n], n // 2 + 1, recent, sinks, 1, 16, BF16, 64, n_layer=1,
+                                                      weights=lambda capacity: torch.full((1, 1, 1, capacity), 0.25))
+        pool.evict(table, seqlen, w, budget=n // 2 + 1, recent=recent, sinks=sinks)
+        _check_evicted(pool, seqlen, w, want)
 
 
 @pytest.mark.parametrize("kind", ["equal", "nan", "inf", "zeros", "negative", "tiny"])
