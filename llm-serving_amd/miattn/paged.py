@@ -410,8 +410,9 @@ class PagedPool:
         afterwards); a block may be in one row only. ``to`` (int32 ``(B, blocks for min(budget, capacity)
         tokens)``): every row, also one within the budget, is written to these blocks, in none of which a row
         of ``block_table`` lies, and its old ones stay as they are (shared blocks of a fork, say). No host
-        wait; a row whose tables name a block outside the pool loses those tokens and is reported by
-        :meth:`check_writes` (as token ``b``)."""
+        wait; a row whose tables name a block outside the pool where a token that stays lies loses those tokens and is
+        reported by :meth:`check_writes` (as token ``b``). A host pool raises ``IndexError`` instead, before it moves
+        anything."""
         target = block_table if to is None else to
         budget, recent, sinks = self._check_evict(block_table, target, seqlen, weights, budget, recent, sinks)
         if block_table.shape[0] == 0:
@@ -449,6 +450,7 @@ class PagedPool:
     def _evict_host(self, table, to, seqlen, weights, budget: int, recent: int, sinks: int) -> None:
         bs = self.block_size
         heads = torch.arange(self.n_kv_head)
+        moves = []  # (row, its length, tokens kept, per layer which)
         for b, n in enumerate(seqlen.tolist()):
             n = max(0, min(n, table.shape[1] * bs))
             keep = min(n, budget)
@@ -456,7 +458,7 @@ class PagedPool:
                 continue
             slot, index = torch.arange(keep), np.arange(n)
             protected = (index < sinks) | (index >= n - recent)
-            page = to[b].long()[slot // bs]
+            which = []
             for i in range(self.n_layer):
                 kept = slot.expand(self.n_kv_head, keep)
                 if n > keep:
@@ -466,6 +468,16 @@ class PagedPool:
                     # the last key sorts first: protected ones, NaN, the heavier, the earlier
                     order = [np.lexsort((index, -value[h], ~nan[h], ~protected)) for h in range(self.n_kv_head)]
                     kept = torch.from_numpy(np.sort(np.stack(order)[:, :keep], axis=-1))
+                which.append(kept)
+            pages = [to[b, slot // bs], *(table[b, kept // bs] for kept in which)]
+            if any(int(p.min()) < 0 or int(p.max()) >= self.n_blocks for p in pages):
+                raise IndexError(f"row {b}: its tables name a block outside the pool's {self.n_blocks} where a token that "
+                                 "stays lies; nothing was moved")
+            moves.append((b, n, keep, which))
+        for b, n, keep, which in moves:
+            slot = torch.arange(keep)
+            page = to[b].long()[slot // bs]
+            for i, kept in enumerate(which):
                 source = table[b].long()[kept // bs]  # (heads, keep)
                 for store in (self.keys[i], self.values[i]):
                     store[page, slot % bs] = store[source, kept % bs, heads.unsqueeze(1)].transpose(0, 1)

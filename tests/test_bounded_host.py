@@ -110,6 +110,34 @@ def test_host_eviction_against_the_oracle(budget, recent, sinks, moved):
     assert torch.equal(weights.nan_to_num(7), want[2].nan_to_num(7)) and torch.equal(seqlen, want[3])
 
 
+@pytest.mark.parametrize("moved", [False, True])
+@pytest.mark.parametrize("page", [-1, 12, -13, 2**31 - 1])
+def test_host_eviction_refuses_tables_that_leave_the_pool(page, moved):
+    """A row's kept tokens in no block of the pool, or bound for none: refused before any row is moved."""
+    pool = _pool()
+    table = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32)
+    to = torch.tensor([[6, 7], [8, 9]], dtype=torch.int32)
+    seqlen, weights = torch.tensor([12, 11], dtype=torch.int32), torch.rand(2, 2, 2, 12)
+    before = [t.clone() for t in (*pool.keys, *pool.values, weights, seqlen)]
+    args = dict(budget=7, recent=3, sinks=1, **({"to": to} if moved else {}))
+    for at, place in [(table, (1, 2)), (table, (1, 0)), *([(to, (1, 1))] if moved else [])]:
+        was = int(at[place])
+        at[place] = page
+        with pytest.raises(IndexError, match="row 1.*outside the pool"):
+            pool.evict(table, seqlen, weights, **args)
+        at[place] = was
+        assert all(torch.equal(a, b) for a, b in zip((*pool.keys, *pool.values, weights, seqlen), before))
+    # entries behind a row's tokens, and of a block that keeps none of them, name what they like
+    table[1, 2], weights[:, 1, :, 4:8] = page, -1.0
+    table[1, 1], seqlen[1] = page, 8
+    weights[:, 1, :, :4] = 1.0
+    one = torch.tensor([[6, page], [7, page]], dtype=torch.int32)
+    want = bounded.evicted(pool.keys, pool.values, table, seqlen, weights, 4, 0, 0, one if moved else None)
+    pool.evict(table, seqlen, weights, budget=4, recent=0, **({"to": one} if moved else {}))
+    assert all(torch.equal(a, b) for a, b in zip(pool.keys + pool.values, want[0] + want[1]))
+    assert torch.equal(weights, want[2]) and seqlen.tolist() == [4, 4]
+
+
 # ------------------------------------------------------------------ refusals
 @pytest.mark.parametrize("window,sinks", [(0, 0), (-3, 0), (True, 0), (1.5, 0), (4, -1), (None, 2), ("4", 0), (4, 0.5)])
 def test_windows_that_are_refused(window, sinks):
