@@ -455,8 +455,8 @@ class BudgetDecoder:
     the first ``sinks`` tokens, the last ``recent`` and those that attention gave the most weight). ``weights``
     ``(n_layer, B, n_kv_head, table capacity)`` is the account: filled by ``Qwen3.prefill(weights=...)``,
     grown by every step (``PagedDecodePlan.run_weighed``). A token's rotation is that of its position in the
-    text (``pos``); its place in the cache (``held``) is counted apart. ``tables`` hold the prompts and at least ``budget
-    + every`` tokens; prompts past the budget are cut before the first step.
+    text (``pos``), which has to lie in the model's RoPE table; its place in the cache (``held``) is counted apart. ``tables``
+    hold the prompts and at least ``budget + every`` tokens; prompts past the budget are cut before the first step.
     """
 
     def __init__(self, model: Qwen3, pool: PagedPool, tables: list[list[int]], lengths: list[int],
@@ -470,6 +470,9 @@ class BudgetDecoder:
             as_index(x, n) for x, n in ((budget, "budget"), (recent, "recent"), (sinks, "sinks"), (every, "every")))
         if self.every < 1:
             raise ValueError(f"every must be >= 1, got {every}")
+        self._text, self._text_end = max(lengths), model.cos.shape[0]  # position of the next token of the longest row
+        if self._text + max_new > self._text_end:
+            raise ValueError(f"{self._text} + {max_new} tokens run past the RoPE table's {self._text_end} positions")
         self.B = len(tables)
         width = max(len(t) for t in tables)
         for t, n in zip(tables, lengths):
@@ -502,6 +505,13 @@ class BudgetDecoder:
         self.held.copy_(self.seqlen)
         self._most = min(self._most, self.budget)
 
+    def _make_room(self) -> None:
+        """What a step needs: a rotation for every row's next token and a free place for it."""
+        if self._text >= self._text_end:
+            raise IndexError(f"a row's next token is at position {self._text}, past the RoPE table's {self._text_end}")
+        if self._most >= self.budget + self.every:
+            self.evict()
+
     def _step(self) -> None:
         m, c = self.model, self.model.cfg
         x = torch.empty(self.B, c.hidden, dtype=m.dtype, device=m.device)
@@ -525,8 +535,7 @@ class BudgetDecoder:
 
     def capture(self, stream=None) -> None:
         """Record one step (run once eagerly first, its effects undone: the K/V that it wrote lie past the rows)."""
-        if self._most >= self.budget + self.every:  # as step() does: the step needs a free place
-            self.evict()
+        self._make_room()
         state = (self.pos, self.held, self.tokens, self.seqlen, self.step_idx, self.weights, self.history)
         saved = [t.clone() for t in state]
         self._step()
@@ -539,14 +548,15 @@ class BudgetDecoder:
         torch.cuda.synchronize()
 
     def step(self) -> None:
-        """One step of every row, after cutting the rows where one has reached ``budget + every`` tokens."""
-        if self._most >= self.budget + self.every:
-            self.evict()
+        """One step of every row, after cutting the rows where one has reached ``budget + every`` tokens. Raises
+        ``IndexError``, with nothing changed, where a row's text has reached the end of the RoPE table."""
+        self._make_room()
         if self.graph is None:
             self._step()
         else:
             self.graph.replay()
         self._most += 1
+        self._text += 1
 
     def check(self) -> None:
         """Raise ``IndexError`` if a step or an eviction met an index out of range (host reads)."""

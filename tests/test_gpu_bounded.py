@@ -675,6 +675,29 @@ def test_budget_decoder_captured_with_its_rows_full(cuda):
     assert d.pos.tolist() == [88] and d.held.tolist() == [48]
 
 
+def test_budget_decoder_stays_inside_the_rope_table(cuda):
+    """Past the table no K/V could be written, so a text that would get there is refused, and so is the step that does."""
+    cfg = Qwen3Config(**TINY)
+    m = Qwen3(cfg, random_weights(cfg, 3), cuda, max_pos=64)
+    pool, account = m.new_pool(16), torch.zeros(2, 2, 2, 64, device=cuda)
+    tables = [[5, 1, 2, 9], [3, 4, 0, 7]]
+    first = m.prefill([list(range(20)), list(range(9))], pool, tables, weights=account).argmax(-1)
+    args = dict(budget=30, recent=8, sinks=2, every=10)
+    with pytest.raises(ValueError, match="20 \\+ 45 tokens run past the RoPE table's 64"):
+        BudgetDecoder(m, pool, tables, [20, 9], first, 45, account, **args)
+    d = BudgetDecoder(m, pool, tables, [20, 9], first, 44, account, **args)
+    d.capture()
+    for _ in range(44):
+        d.step()
+    d.check()
+    assert d.pos.tolist() == [64, 53]
+    before = [t.clone() for t in (*pool.keys, *pool.values, account, d.pos, d.held, d.seqlen, d.tokens, d.history)]
+    with pytest.raises(IndexError, match="position 64"):
+        d.step()
+    d.check()
+    assert all(torch.equal(a, b) for a, b in zip((*pool.keys, *pool.values, account, d.pos, d.held, d.seqlen, d.tokens, d.history), before))
+
+
 def test_calls_beside_each_other_on_two_streams(cuda):
     """Two plans, two packed groups and two pools, one on a stream each, among other calls that push the groups' schedules
     out: what each gives is what it gives alone."""
