@@ -456,7 +456,8 @@ class BudgetDecoder:
     ``(n_layer, B, n_kv_head, table capacity)`` is the account: filled by ``Qwen3.prefill(weights=...)``,
     grown by every step (``PagedDecodePlan.run_weighed``). A token's rotation is that of its position in the
     text (``pos``), which has to lie in the model's RoPE table; its place in the cache (``held``) is counted apart. ``tables``
-    hold the prompts and at least ``budget + every`` tokens; prompts past the budget are cut before the first step.
+    hold the prompts and at least ``budget + every`` tokens; prompts past the budget are cut before the first step. A row that
+    a step skips (:meth:`check`) holds what it held.
     """
 
     def __init__(self, model: Qwen3, pool: PagedPool, tables: list[list[int]], lengths: list[int],
@@ -501,6 +502,7 @@ class BudgetDecoder:
 
     def evict(self) -> None:
         """Cut every row past the budget now (:meth:`step` does so by itself)."""
+        self.seqlen.copy_(self.held)  # a row that the last step skipped has 0 there
         self.pool.evict(self.table, self.seqlen, self.weights, budget=self.budget, recent=self.recent, sinks=self.sinks)
         self.held.copy_(self.seqlen)
         self._most = min(self._most, self.budget)
@@ -526,7 +528,7 @@ class BudgetDecoder:
             return self.plan.run_weighed(i, q, self.weights[i]).view(self.B, -1)
 
         h = m._decode_stack(x, attend, h0)
-        self.held += 1
+        torch.maximum(self.held, self.seqlen, out=self.held)  # + 1, but for rows that the step skipped: their seqlen is 0
         w = m.w["embed"]
         if rows_supported(h, w) and h.shape[1] <= 1024:
             greedy_advance_tiles(rows_tile_best(h, w), self.tokens, self.pos, self.history, self.step_idx)

@@ -698,6 +698,37 @@ def test_budget_decoder_stays_inside_the_rope_table(cuda):
     assert all(torch.equal(a, b) for a, b in zip((*pool.keys, *pool.values, account, d.pos, d.held, d.seqlen, d.tokens, d.history), before))
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_row_that_a_step_skips_holds_what_it_held(captured, cuda):
+    """A token outside the vocabulary: the row is reported and skipped, keeps its tokens through an eviction right after, and
+    its next token goes behind them."""
+    m = _tiny(cuda)
+    pool, account = m.new_pool(32), torch.zeros(2, 2, 2, 128, device=cuda)
+    tables = [list(range(8)), list(range(8, 16))]
+    first = m.prefill([list(range(50)), list(range(25))], pool, tables, weights=account).argmax(-1)
+    d = BudgetDecoder(m, pool, tables, [50, 25], first, 60, account, budget=40, recent=10, sinks=2, every=12)
+    if captured:
+        d.capture()
+    d.tokens[1] = 512
+    row = torch.tensor([8, 9], device=cuda)
+    before = [s[row].view(32, 2, 128)[:25].clone() for s in pool.keys + pool.values]
+    kept = account[:, 1].clone()
+    d.step()
+    assert d.held.tolist() == [41, 25]
+    with pytest.raises(IndexError, match="row 1"):
+        d.check()
+    d.evict()
+    assert d.held.tolist() == [40, 25] and d.seqlen.tolist() == [40, 25] and torch.equal(account[:, 1], kept)
+    d.step()
+    d.check()
+    assert d.held.tolist() == [41, 26] and d.seqlen.tolist() == [41, 26]
+    assert all(torch.equal(s[row].view(32, 2, 128)[:25], x) for s, x in zip(pool.keys + pool.values, before))
+    for _ in range(29):
+        d.step()
+    d.check()
+    assert d.held.tolist() == [46, 46] and d.pos.tolist() == [81, 56]  # cut 12 and 24 steps after the first cut
+
+
 def test_calls_beside_each_other_on_two_streams(cuda):
     """Two plans, two packed groups and two pools, one on a stream each, among other calls that push the groups' schedules
     out: what each gives is what it gives alone."""
