@@ -441,7 +441,8 @@ int mi_varlen_prefill_window(const void* q, const void* k, const void* v, void* 
  *   head_dim 64, 128 or 256, scale > 0): out[s, kv, j] = the weights that the last `observe` queries of segment s
  *   give key j under causal attention, summed over the query heads of kv; zeros from the segment's length up to `width`
  *   (at least the longest segment). out fp32, element s * out_s0 + kv * out_s1 + j. schedule: a
- *   device copy of mi_prompt_weights_schedule's words (host only; NULL sizes it), host_header their first eight.
+ *   device copy of mi_prompt_weights_schedule's words (host only; NULL sizes it), host_header their first eight (a
+ *   schedule made for other heads, or for a segment longer than `width`, is refused).
  *   Workspace: mi_prompt_weights_workspace_size() of that header.
  * mi_cache_evict: rows longer than `budget` tokens cut to it, for every layer, row and KV head: the first `sinks` tokens,
  *   the last `recent` and the heaviest of the others by `weights` (NaN above every number, the lowest index

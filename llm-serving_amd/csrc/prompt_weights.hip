@@ -38,7 +38,7 @@ __device__ __forceinline__ floatx16 mfma32(const uint4& a, const uint4& b, const
   }
 }
 
-constexpr int kHeader = 8;      // {pieces, joins, key blocks, partial slots, units, 0, 0, 0}
+constexpr int kHeader = 8;      // {pieces, joins, key blocks, partial slots, units, H, H_kv, longest segment}
 constexpr int kPieceWords = 8;  // {seq0, L, observed queries, row block, first step, end step, partial slot or -1, first unit}
 constexpr int kJoinWords = 8;   // {first partial slot, pieces, the segment's first unit, row block, observed queries, 0, 0, 0}
 constexpr int kBlockWords = 8;  // {seq0, L, observed queries, key block, the segment's first unit, segment, 0, 0}
@@ -484,9 +484,10 @@ int schedule_weights(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv
   std::vector<Piece> pieces;
   std::vector<Join> joins;
   std::vector<Block> blocks;
-  int slot = 0, unit0 = 0;
+  int slot = 0, unit0 = 0, longest = 0;
   for (int s = 0; s < n_seqs; ++s) {
     const int L = host_cu_seqlens[s + 1] - host_cu_seqlens[s], obs = std::min(observe, L);
+    longest = std::max(longest, L);
     for (int rb = 0; rb < row_blocks(obs); ++rb) {
       const int n = last_key(L, obs, rb) / kStep + 1;
       const int cuts = std::min(kMaxPieces, (n + share - 1) / share);
@@ -511,7 +512,7 @@ int schedule_weights(const int32_t* host_cu_seqlens, int n_seqs, int H, int H_kv
   // longest first
   std::stable_sort(pieces.begin(), pieces.end(), [](const Piece& x, const Piece& y) { return x.s1 - x.s0 > y.s1 - y.s0; });
   std::stable_sort(blocks.begin(), blocks.end(), [](const Block& x, const Block& y) { return x.units > y.units; });
-  const int32_t head[kHeader] = {int(pieces.size()), int(joins.size()), int(blocks.size()), slot, unit0, 0, 0, 0};
+  const int32_t head[kHeader] = {int(pieces.size()), int(joins.size()), int(blocks.size()), slot, unit0, H, H_kv, longest};
   int32_t* w = std::copy(head, head + kHeader, host_schedule);
   for (const Piece& p : pieces) {
     const int32_t x[kPieceWords] = {host_cu_seqlens[p.seq], host_cu_seqlens[p.seq + 1] - host_cu_seqlens[p.seq], p.obs,
@@ -566,6 +567,11 @@ extern "C" int mi_prompt_weights(const void* q, const void* k, const int32_t* sc
   }
   if (host_header[0] < 1 || host_header[1] < 0 || host_header[2] < 1 || host_header[3] < 0 || host_header[4] < 1 || width < 1) {
     return fail(MI_ERR_INVALID, "mi_prompt_weights: bad schedule header or width %d", width);
+  }
+  // units, pieces and their records are counted by the heads of a group, and every key of a segment is written
+  if (host_header[5] != H || host_header[6] != H_kv || width < host_header[7]) {
+    return fail(MI_ERR_INVALID, "mi_prompt_weights: a schedule of %d heads over %d and segments of up to %d tokens does not fit %d "
+                "over %d and width %d", host_header[5], host_header[6], host_header[7], H, H_kv, width);
   }
   auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const size_t need = mi_prompt_weights_workspace_size(host_header, H_kv);

@@ -259,6 +259,23 @@ def test_c_entries_refuse_before_any_launch():
     assert evict(store=(ctypes.c_void_p * 1)(None)) == _lib.MI_ERR_INVALID and evict(B=0) == _lib.MI_OK
 
 
+def test_accounts_refuse_a_schedule_of_another_call():
+    """Other heads, or an account narrower than the longest segment, before any launch (the workspace holds all that they ask for)."""
+    lib, cu = _lib.lib, (ctypes.c_int32 * 3)(0, 300, 310)
+    n = lib.mi_prompt_weights_schedule(cu, 2, 4, 2, 128, 300, None, 0)
+    words = (ctypes.c_int32 * n)()
+    assert lib.mi_prompt_weights_schedule(cu, 2, 4, 2, 128, 300, words, n) == n
+    head = (ctypes.c_int32 * 8)(*words[:8])
+
+    def account(H, H_kv, width, workspace=None, ws_bytes=0):
+        return lib.mi_prompt_weights(64, 64, 64, head, H, H_kv, 128, 1.0, 2, 64, H_kv * width, width, width, workspace,
+                                     ws_bytes, None)
+    for H, H_kv, width in ((8, 2, 300), (4, 4, 300), (2, 2, 300), (8, 4, 300), (2, 1, 300), (4, 2, 299), (4, 2, 10)):
+        assert account(H, H_kv, width) == _lib.MI_ERR_INVALID and "does not fit" in _lib.last_error()
+    for width in (300, 4096):  # the call that it was made for gets as far as its workspace
+        assert account(4, 2, width) == _lib.MI_ERR_WORKSPACE
+
+
 # ------------------------------------------------------------------ schedules and blocks
 @pytest.mark.parametrize("lengths,window,sinks,D", [([700, 1, 64, 65], 100, 0, 128), ([4096], 512, 4, 128),
                                                     ([3000, 100], 64, 200, 64), ([129], 10**6, 0, 256)])
