@@ -388,9 +388,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_weights_
         float t[4];  // long sums: a unit's weights are added up (in four chains) before they join the others
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float p = fast_exp2(fmaf(sc[e], a.scale_log2, -m[e]));
-          if (decltype(masked)::value && (e >> 2) * 8 + (e & 3) < lim) p = 0.0f;
-          t[e & 3] = e < 4 ? p * by[e] : fmaf(p, by[e], t[e & 3]);
+          const float p = fast_exp2(fmaf(sc[e], a.scale_log2, -m[e]));
+          const float to = e < 4 ? p * by[e] : fmaf(p, by[e], t[e & 3]);
+          // (a row's 1 / sum may be NaN: what does not see the key adds nothing, not 0 times that)
+          const bool hidden = decltype(masked)::value && (e >> 2) * 8 + (e & 3) < lim;
+          t[e & 3] = hidden ? (e < 4 ? 0.0f : t[e & 3]) : to;
         }
         w[kb] += (t[0] + t[1]) + (t[2] + t[3]);
         if (kb + 1 < kHeld) interleave<KS, decltype(masked)::value ? 10 : 6>();

@@ -211,7 +211,8 @@ class SdpaVarlen:
             keys = k[a:b].float().permute(1, 2, 0).repeat_interleave(group, 0)
             scores = torch.matmul(q[first:b].float().transpose(0, 1), keys) * scale
             hidden = torch.arange(b - a, device=q.device) > torch.arange(first - a, b - a, device=q.device).unsqueeze(1)
-            w = torch.softmax(scores.masked_fill(hidden, -math.inf), -1).sum(1)
+            # a query with NaN or infinite scores has NaN weights, of the keys that it sees
+            w = torch.softmax(scores.masked_fill(hidden, -math.inf), -1).masked_fill(hidden, 0.0).sum(1)
             out[s, :, : b - a] = w.view(k.shape[1], group, b - a).sum(1)
         return out
 

@@ -87,6 +87,19 @@ def test_sdpa_arm_of_the_account(observe):
     assert got is out and torch.allclose(got[..., :30].double(), want, atol=1e-5) and not got[..., 30:].any()
 
 
+@pytest.mark.parametrize("observe", [None, 9])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_sdpa_arm_of_the_account_behind_a_query_that_is_not_finite(observe, value):
+    q, k = torch.randn(30, 6, 16), torch.randn(30, 2, 16)
+    args = dict(cu_seqlens=[0, 12, 30], max_seqlen=18, observe=observe)
+    want = SdpaVarlen().prompt_weights(q, k, **args)
+    q[25, 1, 3] = value
+    got = SdpaVarlen().prompt_weights(q, k, **args)
+    assert got[1, 0, :14].isnan().all()
+    got[1, 0, :14] = want[1, 0, :14]
+    assert torch.equal(got, want)
+
+
 def _pool(n_layer=2, n_blocks=12, bs=4, H_kv=2, D=4, dtype=torch.float32):
     pool = PagedPool(n_layer, n_blocks, bs, H_kv, D, dtype=dtype)
     for store in pool.keys + pool.values:

@@ -365,6 +365,26 @@ def test_account_of_a_long_prompt_in_pieces(cuda):
     _within(got, want, bound)
 
 
+@pytest.mark.parametrize("heads", [(16, 8, 128, BF16), (8, 2, 256, F16), (4, 4, 64, BF16), (6, 1, 128, F16)])
+@pytest.mark.parametrize("observe", [None, 37])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_account_of_keys_behind_a_query_that_is_not_finite(heads, observe, value, cuda):
+    """Such a query's weights are NaN, for the keys that it sees; keys behind it, other segments and other KV heads keep their bits."""
+    H, H_kv, D, dtype = heads
+    g = torch.Generator().manual_seed(7)
+    cu = [0, 100, 263, 266]
+    q, k = (torch.randn(266, h, D, generator=g).to(dtype).to(cuda) for h in (H, H_kv))
+    args = dict(cu_seqlens=cu, max_seqlen=163, observe=observe)
+    good = HipVarlen().prompt_weights(q, k, **args)
+    for at in (130, 162):  # of the second segment
+        bad = q.clone()
+        bad[100 + at, 0, 1] = value
+        got = HipVarlen().prompt_weights(bad, k, **args)
+        assert got[1, 0, : at + 1].isnan().all()
+        got[1, 0, : at + 1] = good[1, 0, : at + 1]
+        assert torch.equal(got, good), (at, (got != good).nonzero()[:4].tolist())
+
+
 def test_account_of_prompts_captured(cuda):
     cu = _cu([500, 60])
     sets = [[torch.randn(560, h, 128).bfloat16().cuda() for h in (4, 2)] for _ in range(2)]
