@@ -384,21 +384,23 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_weights_
       for (int kb = 0; kb < kHeld; ++kb) {
         const floatx16 sc = cur;
         if (kb + 1 < kHeld) cur = product<T>(qf, kf[kb + 1]);
-        const int lim = key0 + kb * 32 + col - now.i0 - 4 * g;  // rows below it do not see the key
+        // rows below lim do not see the key, those from `there` on are none: zeros, whose product with an infinite key is NaN
+        const int lim = key0 + kb * 32 + col - now.i0 - 4 * g, there = now.rows - 4 * g;
         float t[4];  // long sums: a unit's weights are added up (in four chains) before they join the others
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float p = fast_exp2(fmaf(sc[e], a.scale_log2, -m[e]));
           const float to = e < 4 ? p * by[e] : fmaf(p, by[e], t[e & 3]);
           // (a row's 1 / sum may be NaN: what does not see the key adds nothing, not 0 times that)
-          const bool hidden = decltype(masked)::value && (e >> 2) * 8 + (e & 3) < lim;
+          const int r = (e >> 2) * 8 + (e & 3);
+          const bool hidden = decltype(masked)::value && (r < lim || r >= there);
           t[e & 3] = hidden ? (e < 4 ? 0.0f : t[e & 3]) : to;
         }
         w[kb] += (t[0] + t[1]) + (t[2] + t[3]);
         if (kb + 1 < kHeld) interleave<KS, decltype(masked)::value ? 10 : 6>();
       }
     };
-    if (key0 + kKeys - 1 > now.i0) {  // some row does not see every key
+    if (key0 + kKeys - 1 > now.i0 || now.rows < 32) {  // some row does not see every key, or is none
       add(std::true_type{});
     } else {
       add(std::false_type{});

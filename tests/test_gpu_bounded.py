@@ -385,6 +385,23 @@ def test_account_of_keys_behind_a_query_that_is_not_finite(heads, observe, value
         assert torch.equal(got, good), (at, (got != good).nonzero()[:4].tolist())
 
 
+@pytest.mark.parametrize("heads", [(16, 8, 128, BF16), (8, 2, 256, F16), (4, 4, 64, BF16), (6, 1, 128, F16)])
+@pytest.mark.parametrize("observe", [None, 5, 37])
+def test_account_of_a_key_of_minus_infinity(heads, observe, cuda):
+    """A key whose every score is -infinity weighs nothing, like one at a score whose exponential is 0, in a prompt whose last 32
+    rows are not all there."""
+    H, H_kv, D, dtype = heads
+    g = torch.Generator().manual_seed(8)
+    q, k = (torch.randn(170, h, D, generator=g).to(dtype).to(cuda) for h in (H, H_kv))
+    q[..., 3] = 2.0
+    k[[20, 163], :, 3] = -30000.0  # times 2 / 16 at least: far below the exponents of fp32
+    args = dict(cu_seqlens=[0, 103, 170], max_seqlen=103, observe=observe)
+    far = HipVarlen().prompt_weights(q, k, **args)
+    assert not far[0, :, 20].any() and not far[1, :, 60].any() and far.isfinite().all()
+    k[[20, 163], :, 3] = -math.inf
+    assert torch.equal(HipVarlen().prompt_weights(q, k, **args), far)
+
+
 def test_account_of_prompts_captured(cuda):
     cu = _cu([500, 60])
     sets = [[torch.randn(560, h, 128).bfloat16().cuda() for h in (4, 2)] for _ in range(2)]
