@@ -34,6 +34,7 @@
 #include <vector>
 
 #include "common.h"
+#include "window_band.h"
 
 namespace miattn {
 namespace {
@@ -1029,27 +1030,12 @@ struct Duo {
 __device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14)); }
 
 // Windowed form (kWin): query i sees key j <= i where i - j < window or j < sinks. Of an item's key tiles those
-// that hold neither a sink nor a key within its first row's window are left out: the others are
-// numbered 0 .. n - 1, tile t < ts being tile t of the segment (sinks) and a later one tile t + jump, and
-// every step below goes by those numbers. So an item of a long segment costs what the window does. P is rounded to 16 bits for
-// PV as without a window (its row sum is taken before). One segment of 16384 under 2048 + 4, H 16 / H_kv 8 / D 128: 308 us,
+// that no row of it sees a key of are left out (window_band.h), the others numbered 0 .. n - 1, and every step below goes by
+// those numbers. So an item of a long segment costs what the window does. P is rounded to 16 bits for PV as without a window
+// (its row sum is taken before). One segment of 16384 under 2048 + 4, H 16 / H_kv 8 / D 128: 308 us,
 // 840 TFLOP/s of what is seen; 8 of 4311 tokens under 256 + 4: 24.7, two thirds of it the items' starts and ends (6 steps each);
 // 5 of 8192 under 500 + 17 at H 8 / H_kv 2 / D 256: 82. Items of 128 rows (the tall kernel's) would have half as many ends but
 // 608 of them for 512 places in the second case, and by their step and item costs without a window gain nothing in the first.
-struct Band {
-  int ts, jump, n;
-};
-__host__ __device__ __forceinline__ Band band_of(int row0, int q_end, int window, int sinks, int BK) {
-  const int first = row0 - window + 1;
-  const int tw = first > 0 ? first / BK : 0;  // first tile of the window
-  const int s = ((sinks < q_end ? sinks : q_end) + BK - 1) / BK;
-  Band b;
-  b.ts = s < tw ? s : tw;
-  b.jump = tw - b.ts;
-  b.n = (q_end + BK - 1) / BK - b.jump;
-  return b;
-}
-
 template <typename T, int D, bool kWin = false>
 __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefill_duo_kernel(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
@@ -1155,7 +1141,7 @@ __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefil
   const int dma_step = int((seg_index(LP) - seg_index(0)) * W::RPS * kv_row_b);
   // the segment's tile that an item's tile t is
   auto tile_of = [&](const Item& it, int t) {
-    if constexpr (kWin) return t < it.ts ? t : t + it.jump;
+    if constexpr (kWin) return band_tile(t, it.ts, it.jump);
     return t;
   };
   auto issue = [&](const char* seg, const Item& it, int tv, uint8_t* dst) {

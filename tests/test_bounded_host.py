@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import random
 import subprocess
 import sys
 
@@ -311,6 +312,73 @@ def test_windowed_items_cover_every_seen_key_once(lengths, window, sinks, D):
     assert set(pieces) == want
     for got in pieces.values():
         assert sorted(got) == [(i, got[0][1]) for i in range(got[0][1])]
+
+
+@pytest.fixture(scope="module")
+def band_tiles(tmp_path_factory):
+    """The key tiles of a query tile, by the header that the schedule and the kernel include, built for the host."""
+    out = tmp_path_factory.mktemp("band")
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llm-serving_amd", "csrc")
+    (out / "band.cpp").write_text('''
+#include "window_band.h"
+extern "C" int tiles(int row0, int q_end, int window, int sinks, int* out) {
+  const miattn::Band b = miattn::band_of(row0, q_end, window, sinks, 64);
+  for (int t = 0; t < b.n; ++t) out[t] = miattn::band_tile(t, b.ts, b.jump);
+  return b.n;
+}
+''')
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-D__host__=", "-D__device__=", "-I", csrc, "-o", str(out / "band.so"),
+                    str(out / "band.cpp")], check=True)
+    lib = ctypes.CDLL(str(out / "band.so"))
+
+    def tiles(row0, q_end, window, sinks):
+        words = (ctypes.c_int * (q_end // 64 + 2))()
+        return words[:lib.tiles(row0, q_end, window, sinks, words)]
+    return tiles
+
+
+def _tiles_seen(row0, q_end, window, sinks):
+    """The 64-key tiles that hold a key which one of the rows sees, by the mask over all of their keys."""
+    i, j = torch.arange(row0, q_end).unsqueeze(1), torch.arange(q_end)
+    seen = ((j <= i) & ((i - j < window) | (j < sinks))).any(0)
+    return sorted({t // 64 for t in seen.nonzero().flatten().tolist()})
+
+
+def test_windowed_key_tiles_are_those_with_a_seen_key(band_tiles):
+    rng = random.Random(4)
+    draws = [(row0, rows, window, sinks) for row0 in (0, 64, 640) for rows in (1, 63, 64) for window in (1, 2, 64, 65, 10**6)
+             for sinks in (0, 1, 64, 65, 700, 2**31 - 1)]
+    draws += [(64 * rng.randrange(60), rng.randrange(1, 65), round(2 ** rng.uniform(0, 13)), rng.choice((0, round(2 ** rng.uniform(0, 13)))))
+              for _ in range(1500)]
+    for row0, rows, window, sinks in draws:
+        assert band_tiles(row0, row0 + rows, window, sinks) == _tiles_seen(row0, row0 + rows, window, sinks), (row0, rows, window, sinks)
+
+
+@pytest.mark.parametrize("lengths,window,sinks", [([700, 1, 64, 65], 100, 0), ([4096], 512, 4), ([3000, 100], 64, 200), ([129], 10**6, 0),
+                                                  ([2500], 1, 0), ([1000, 333], 300, 70), ([2000], 1500, 0)])
+def test_windowed_pieces_take_each_seen_key_tile_once(band_tiles, lengths, window, sinks):
+    """The tiles that the pieces of a query tile walk, each its share of the numbers, and no other ones."""
+    cu = _cu(lengths)
+    args = ((ctypes.c_int32 * len(cu))(*cu), len(lengths), 2, 1, 128, window, sinks)
+    n = _lib.lib.mi_varlen_schedule_window(*args, None, 0)
+    words = (ctypes.c_int32 * n)()
+    assert _lib.lib.mi_varlen_schedule_window(*args, words, n) == n
+    walked, cut = {}, 0
+    for w in range(words[0]):
+        first, count = words[4 + 8 * w], words[5 + 8 * w]
+        for i in range(count):
+            seq0, L, w2, w3 = (words[first + 4 * i + j] & 0xFFFFFFFF for j in range(4))
+            row0, split, n_split = 64 * (w2 >> 16), (w2 >> 8) & 0xFF, (w2 & 0xFF) + 1
+            assert L == dict(zip(cu, lengths))[seq0]
+            tiles = band_tiles(row0, min(L, row0 + 64), window, sinks)
+            piece = tiles[split * len(tiles) // n_split: (split + 1) * len(tiles) // n_split]
+            assert piece  # an item has at least one step
+            cut += n_split > 1
+            walked.setdefault((seq0, L, row0, w3 >> 24), []).extend(piece)
+    assert (cut > 0) == (max(map(len, walked.values())) > 8)  # few items: those of more than 8 tiles are cut
+    assert len(walked) == 2 * sum(-(-n // 64) for n in lengths)
+    for (seq0, L, row0, _), tiles in walked.items():
+        assert sorted(tiles) == _tiles_seen(row0, min(L, row0 + 64), window, sinks)
 
 
 def test_hidden_blocks_of_a_seat():
