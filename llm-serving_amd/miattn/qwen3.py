@@ -24,6 +24,7 @@ measures is ``serve/graph.py:9-10``).
 from __future__ import annotations
 
 import math
+from collections import Counter
 from dataclasses import dataclass
 
 import torch
@@ -456,8 +457,8 @@ class BudgetDecoder:
     ``(n_layer, B, n_kv_head, table capacity)`` is the account: filled by ``Qwen3.prefill(weights=...)``,
     grown by every step (``PagedDecodePlan.run_weighed``). A token's rotation is that of its position in the
     text (``pos``), which has to lie in the model's RoPE table; its place in the cache (``held``) is counted apart. ``tables``
-    hold the prompts and at least ``budget + every`` tokens; prompts past the budget are cut before the first step. A row that
-    a step skips (:meth:`check`) holds what it held.
+    hold the prompts and at least ``budget + every`` tokens, those of a row that is ever cut no block of another row; prompts
+    past the budget are cut before the first step. A row that a step skips (:meth:`check`) holds what it held.
     """
 
     def __init__(self, model: Qwen3, pool: PagedPool, tables: list[list[int]], lengths: list[int],
@@ -480,6 +481,12 @@ class BudgetDecoder:
             most = max(n, min(n + max_new, self.budget + self.every))
             if len(t) * pool.block_size < most:
                 raise ValueError(f"block table of {len(t)} blocks cannot hold the {most} tokens that a row grows to")
+        uses = Counter(b for t in tables for b in t)
+        for r, (t, n) in enumerate(zip(tables, lengths)):
+            shared = [b for b in t if uses[b] > 1]
+            if shared and n + max_new > self.budget:
+                raise ValueError(f"row {r} is cut in place, but its block {shared[0]} is in the tables twice: copy shared "
+                                 "blocks first")
         bt = torch.full((self.B, width), -1, dtype=torch.int32)
         for r, t in enumerate(tables):
             bt[r, : len(t)] = torch.tensor(t, dtype=torch.int32)

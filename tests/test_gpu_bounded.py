@@ -712,6 +712,23 @@ def test_budget_decoder_captured_with_its_rows_full(cuda):
     assert d.pos.tolist() == [88] and d.held.tolist() == [48]
 
 
+def test_budget_decoder_refuses_to_cut_shared_blocks(cuda):
+    """An eviction in place would move one row's tokens under the other's; rows that stay within the budget may share."""
+    m = _tiny(cuda)
+    pool, account = m.new_pool(16), torch.zeros(2, 2, 2, 64, device=cuda)
+    first = torch.zeros(2, dtype=torch.long)
+    good = dict(budget=40, recent=8, every=10)
+    for tables, lengths, max_new in (([[0, 1, 2, 3], [0, 4, 5, 6]], [20, 20], 21), ([[0, 1, 2, 3], [0, 4, 5, 6]], [4, 30], 11),
+                                     ([[0, 1, 2, 3], [4, 5, 6, 4]], [1, 41], 0)):
+        with pytest.raises(ValueError, match="in the tables twice"):
+            BudgetDecoder(m, pool, tables, lengths, first, max_new, account, **good)
+    d = BudgetDecoder(m, pool, [[0, 1, 2, 3], [0, 4, 5, 6]], [20, 17], first, 20, account, **good)
+    for _ in range(20):
+        d.step()
+    d.check()
+    assert d.held.tolist() == [40, 37]
+
+
 def test_budget_decoder_stays_inside_the_rope_table(cuda):
     """Past the table no K/V could be written, so a text that would get there is refused, and so is the step that does."""
     cfg = Qwen3Config(**TINY)
