@@ -58,7 +58,8 @@ __device__ __forceinline__ int slot_of(const int32_t* table, int i, const EvictA
 }
 
 // Items: weights per thread, held in registers; 0 for rows of any length, which read them again in each of up to 5 passes
-// (256 rows of 20000 tokens 57 us so, 29.5 held; 128 of 60000 154 and 72).
+// (256 rows of 20000 tokens 57 us so, 29.5 held; 128 of 60000 154 and 72). With 16, 32 and 64 of them 18, 116 and 358
+// scalars (the ballots of every round, kept for both loops over them) spill to lanes of vector registers, none to memory.
 template <int NT, int Items>
 __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
   constexpr int W = NT / 64, E = Items * W;  // a count per wave and round

@@ -1234,7 +1234,9 @@ bool rows_kernel_fits(const DecodeArgs& a, const Plan& p, int D, int waves) {
 // partials; splits are made long enough for 32 to hold a row. The K elements that a workgroup may have to stream: 24576 where a
 // wave's state takes one token at a time, 16384 where two do (us per layer in a graph, two launches against one: H 16 /
 // H_kv 8 / D 128, two: 1 row of 64 tokens 6.8 / 5.4, 4 of 128 7.6 / 6.8, 32 of 128 10.3 / 9.9, but 4 of 192 7.5 / 8.1 and
-// 1 of 304 8.0 / 10.1; H 32 / H_kv 16 / D 128, one: 1 of 64 6.8 / 4.5, 8 of 192 10.4 / 7.3, 1 of 304 8.4 / 8.7).
+// 1 of 304 8.0 / 10.1; H 32 / H_kv 16 / D 128, one: 1 of 64 6.8 / 4.5, 8 of 192 10.4 / 7.3, 1 of 304 8.4 / 8.7). Two heads
+// and two tokens at a time at head_dim 128, the first of these, spill at 16 waves' 128 registers (40 in bf16, 144 bytes a
+// lane; 27 in fp16; the plain form none): each score is stored by one lane per token. The lower line may be due to that.
 bool weighed_rows_fit(const DecodeArgs& a, const Plan& p, int D, int waves) {
   const int64_t capacity = int64_t(a.max_blocks) << a.bs_log2;
   return a.n_hchunks == 1 && capacity * D <= (p.TPL == 1 ? 24576 : 16384) && int64_t(a.B) * a.H_kv * waves <= 16 * 256;

@@ -14,8 +14,9 @@
 // In the first every wave has keys of its own, in the second rows of its own: nothing is loaded twice by a workgroup, and no
 // barrier stands in the loops. Bound by the vector pipe: per 32 x 32 scores of a wave 16 v_exp_f32 (16 cycles each)
 // and 3 other operations per register, beside 8 matrix instructions of 32 cycles (head_dim 128). Prompts of 4096, 2048,
-// 1742 and 306 tokens, H 16 / H_kv 8 / D 128, all queries (49 GFLOP counted once): 71 + 71 us, of which the exponentials
-// alone are 21 each; 8 prompts of 4311 tokens, last 32 queries: 8.3 + 2.0 (join) + 6.8 us, launches and round trips.
+// 1742 and 306 tokens, H 16 / H_kv 8 / D 128, all queries (49 GFLOP counted once): 68 + 69 us, of which the exponentials
+// alone are 21 each; 8 prompts of 4311 tokens, last 32 queries: 8.6 + 3.0 (join) + 8.2 us under a profiler, 16.8 in all in
+// a replayed graph, launches and round trips.
 #include <algorithm>
 #include <new>
 #include <vector>

@@ -1034,8 +1034,9 @@ __device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(15 | (
 // those numbers. So an item of a long segment costs what the window does. P is rounded to 16 bits for PV as without a window
 // (its row sum is taken before). One segment of 16384 under 2048 + 4, H 16 / H_kv 8 / D 128: 308 us,
 // 840 TFLOP/s of what is seen; 8 of 4311 tokens under 256 + 4: 24.7, two thirds of it the items' starts and ends (6 steps each);
-// 5 of 8192 under 500 + 17 at H 8 / H_kv 2 / D 256: 82. Items of 128 rows (the tall kernel's) would have half as many ends but
-// 608 of them for 512 places in the second case, and by their step and item costs without a window gain nothing in the first.
+// 5 of 8192 under 500 + 17 at H 8 / H_kv 2 / D 256: 82. Items of 128 rows (the tall kernel's) would have half as many ends; they
+// were not built: a simulation of the schedule by their step and item costs without a window gave 608 items for 512 places in
+// the second case and no gain in the first.
 template <typename T, int D, bool kWin = false>
 __global__ __launch_bounds__(Duo<D>::THREADS, Duo<D>::PER_CU) void varlen_prefill_duo_kernel(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
